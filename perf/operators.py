@@ -377,7 +377,7 @@ def _run_step(s):
     need = (rest > 0).long()
     before = torch.cumsum(need, 0) - need
     free, there = _nth_free(ref, n)
-    ok = before + need <= there
+    ok = (need == 0) | (before + need <= there)
     shared = (cols < full[:, None]) & ok[:, None]
     ref.index_add_(0, table[src].clamp(min=0).long().view(-1), shared.int().view(-1))
     part = (need > 0) & ok
@@ -398,7 +398,7 @@ def _run_step(s):
     need = want - have
     before = torch.cumsum(need, 0) - need
     free, there = _nth_free(ref, n * (_pages(s["new"], page) + 1))
-    ok = (before + need <= there) & (want <= stride)
+    ok = ((need == 0) | (before + need <= there)) & (want <= stride)
     put = (cols >= have[:, None]) & (cols < want[:, None]) & ok[:, None]
     fresh = free[(before[:, None] + cols - have[:, None])[put]]
     ref[fresh] = 1
