@@ -42,6 +42,8 @@ EXPORTS = (
     "atlas_b200_dequant_nvfp4_to_bf16", "atlas_b200_quantize_bf16_to_nvfp4", "atlas_b200_nvfp4_global_absmax",
     "atlas_b200_nvfp4_scale2_from_absmax", "atlas_b200_nvfp4_combined_global_scale", "atlas_b200_silu_mul",
     "atlas_b200_silu_mul_quant_nvfp4", "atlas_b200_kv_norm_rope_cache_write", "atlas_b200_kv_norm_mrope_cache_write", "atlas_b200_k_norm_rope_cache_write_fp8", "atlas_b200_qkv_norm_rope_cache_write",
+    "atlas_b200_qkv_norm_rope_cache_write_fp8", "atlas_b200_paged_attention", "atlas_b200_paged_attention_ws_bytes", "atlas_b200_last_attention_shape",
+    "atlas_b200_cache_ws_bytes", "atlas_b200_cache_append", "atlas_b200_cache_fork", "atlas_b200_cache_free", "atlas_b200_cache_compact",
     "atlas_b200_nvfp4_lora_linear", "atlas_b200_nvfp4_lora_linear_noalloc", "atlas_b200_lora_shrink_tiles",
     "atlas_b200_push_columns", "atlas_b200_copy_columns", "atlas_b200_selftest_bounded_wait", "atlas_b200_selftest_ring_wait", "atlas_b200_column_shard",
     "atlas_b200_build_seq_slot", "atlas_b200_routed_prefill_slot_of", "atlas_b200_peft_scaling",
@@ -81,6 +83,22 @@ class LinearDesc(C.Structure):
         ("n_dest", C.c_uint32), ("y_col_offset", C.c_uint32), ("y_dest", C.c_void_p * 8),
         ("a_pool_base", C.c_void_p), ("a_slot_stride", C.c_size_t),
     ]
+
+
+CACHE_BF16, CACHE_E4M3 = 0, 1
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "out", "lse", "k_cache", "v_cache", "block_table", "cu_q", "kv_len", "ws")] + [
+        ("ws_bytes", C.c_size_t)] + [(n, C.c_uint32) for n in (
+            "n_seqs", "n_tokens", "max_q_len", "max_kv_len", "n_pages", "block_size", "table_stride", "cache_dtype", "q_heads", "kv_heads",
+            "head_dim", "q_row_stride", "out_row_stride")] + [(n, C.c_float) for n in ("softmax_scale", "k_scale", "v_scale")]
+
+
+class CacheDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("bases", "refcount", "block_table", "seq_len", "ws")] + [
+        ("ws_bytes", C.c_size_t), ("page_bytes", C.c_size_t)] + [(n, C.c_uint32) for n in (
+            "n_bases", "n_pages", "block_size", "table_stride", "n_seqs", "reserved0")]
 
 
 class PeftConfig(C.Structure):
@@ -126,6 +144,15 @@ def lib() -> C.CDLL:
     L.atlas_b200_k_norm_rope_cache_write_fp8.argtypes = [vp, u32, vp, vp, vp, vp, u32, u32, u32, u32, u32, f32, f32, f32, vp]
     L.atlas_b200_qkv_norm_rope_cache_write.argtypes = [vp, vp, vp, u32, u32, vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, f32, f32,
                                                        C.c_int, vp]
+    L.atlas_b200_qkv_norm_rope_cache_write_fp8.argtypes = [vp, vp, vp, u32, u32, vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, f32, f32,
+                                                           C.c_int, f32, f32, vp]
+    L.atlas_b200_paged_attention.argtypes = [vp, vp]
+    L.atlas_b200_paged_attention_ws_bytes.argtypes, L.atlas_b200_paged_attention_ws_bytes.restype = [vp], sz
+    L.atlas_b200_cache_ws_bytes.argtypes, L.atlas_b200_cache_ws_bytes.restype = [vp, u32], sz
+    L.atlas_b200_cache_append.argtypes = [vp, vp, vp, u32, u32, vp, vp, vp]
+    L.atlas_b200_cache_fork.argtypes = [vp, vp, vp, u32, vp, vp]
+    L.atlas_b200_cache_free.argtypes = [vp, vp, u32, vp]
+    L.atlas_b200_cache_compact.argtypes = [vp, vp, vp, vp, vp, vp]
     L.atlas_b200_lora_shrink_tiles.argtypes = [C.POINTER(LinearDesc), u32, u32, C.POINTER(vp), u32, vp]
     L.atlas_b200_push_columns.argtypes = [vp, u32, C.POINTER(vp), u32, u32, u32, u32, vp]
     L.atlas_b200_copy_columns.argtypes = [vp, u32, C.POINTER(vp), u32, u32, u32, u32, vp]
@@ -388,6 +415,89 @@ def qkv_norm_rope_cache_write(q, k_in, v_in, q_row_stride: int, kv_row_stride: i
         _ptr(q), _ptr(k_in), _ptr(v_in), q_row_stride, kv_row_stride, _ptr(q_norm_weight), _ptr(k_norm_weight), _ptr(positions),
         _ptr(inv_freq), _ptr(slot_mapping), _ptr(k_cache), _ptr(v_cache), tokens, q_heads, kv_heads, head_dim, rotary_dim, block_size,
         rms_eps, attention_factor, 1 if norm_offset_one else 0, _stream_ptr(stream)))
+
+
+def qkv_norm_rope_cache_write_fp8(q, k_in, v_in, q_row_stride: int, kv_row_stride: int, q_norm_weight, k_norm_weight, positions, inv_freq,
+                                  slot_mapping, k_cache_fp8, v_cache_fp8, tokens: int, q_heads: int, kv_heads: int, head_dim: int, rotary_dim: int,
+                                  block_size: int, rms_eps: float, k_inv_scale: float, v_inv_scale: float, attention_factor: float = 1.0,
+                                  norm_offset_one: bool = True, stream=None) -> None:
+    """qkv_norm_rope_cache_write into E4M3 paged caches (one byte per element): value * inv_scale, saturating cast."""
+    _check("atlas_b200_qkv_norm_rope_cache_write_fp8", lib().atlas_b200_qkv_norm_rope_cache_write_fp8(
+        _ptr(q), _ptr(k_in), _ptr(v_in), q_row_stride, kv_row_stride, _ptr(q_norm_weight), _ptr(k_norm_weight), _ptr(positions),
+        _ptr(inv_freq), _ptr(slot_mapping), _ptr(k_cache_fp8), _ptr(v_cache_fp8), tokens, q_heads, kv_heads, head_dim, rotary_dim, block_size,
+        rms_eps, attention_factor, 1 if norm_offset_one else 0, k_inv_scale, v_inv_scale, _stream_ptr(stream)))
+
+
+def make_attention_desc(*, q, out, k_cache, v_cache, block_table, cu_q, kv_len, n_seqs: int, n_tokens: int, max_q_len: int, max_kv_len: int,
+                        n_pages: int, block_size: int, table_stride: int, q_heads: int, kv_heads: int, head_dim: int, softmax_scale: float,
+                        cache_dtype: int = CACHE_BF16, k_scale: float = 1.0, v_scale: float = 1.0, lse=None, q_row_stride=None,
+                        out_row_stride=None, ws=None, ws_bytes: int = 0) -> AttentionDesc:
+    """Descriptor of one attention over the paged cache (atlas_b200_attention_desc).  q / out: tensors or device addresses of the first
+    column of row 0.  Scratch: attention_ws_bytes(desc) bytes, put into desc.ws / desc.ws_bytes."""
+    d = AttentionDesc()
+    d.q, d.out, d.lse, d.k_cache, d.v_cache = _ptr(q), _ptr(out), _ptr(lse), _ptr(k_cache), _ptr(v_cache)
+    d.block_table, d.cu_q, d.kv_len, d.ws, d.ws_bytes = _ptr(block_table), _ptr(cu_q), _ptr(kv_len), _ptr(ws), ws_bytes
+    d.n_seqs, d.n_tokens, d.max_q_len, d.max_kv_len = n_seqs, n_tokens, max_q_len, max_kv_len
+    d.n_pages, d.block_size, d.table_stride, d.cache_dtype = n_pages, block_size, table_stride, cache_dtype
+    d.q_heads, d.kv_heads, d.head_dim = q_heads, kv_heads, head_dim
+    d.q_row_stride = q_row_stride if q_row_stride is not None else q_heads * head_dim
+    d.out_row_stride = out_row_stride if out_row_stride is not None else q_heads * head_dim
+    d.softmax_scale, d.k_scale, d.v_scale = softmax_scale, k_scale, v_scale
+    return d
+
+
+def attention_ws_bytes(desc: AttentionDesc) -> int:
+    """Bytes of scratch that paged_attention wants in desc.ws (on the current device)."""
+    return int(lib().atlas_b200_paged_attention_ws_bytes(C.byref(desc)))
+
+
+def paged_attention(desc: AttentionDesc, stream=None) -> None:
+    """Attention of every sequence's new tokens over its paged cache, up to and including each token itself."""
+    _check("atlas_b200_paged_attention", lib().atlas_b200_paged_attention(C.byref(desc), _stream_ptr(stream)))
+
+
+def last_attention_shape() -> dict:
+    """What this thread's most recent paged_attention launched."""
+    out = (C.c_uint32 * 4)()
+    _check("atlas_b200_last_attention_shape", lib().atlas_b200_last_attention_shape(out))
+    return {"block_rows": out[0], "ctas": out[1], "whole_items": bool(out[2]), "tile_keys": out[3]}
+
+
+def make_cache_desc(*, bases, n_bases: int, page_bytes: int, n_pages: int, block_size: int, refcount, block_table, table_stride: int, seq_len,
+                    n_seqs: int, ws=None, ws_bytes: int = 0) -> CacheDesc:
+    """Descriptor of a paged cache's pages and tables (atlas_b200_cache_desc); bases: device array of the caches' addresses.
+    Scratch: cache_ws_bytes(desc, n) bytes for calls of up to n entries, put into desc.ws / desc.ws_bytes."""
+    d = CacheDesc()
+    d.bases, d.refcount, d.block_table, d.seq_len, d.ws, d.ws_bytes = _ptr(bases), _ptr(refcount), _ptr(block_table), _ptr(seq_len), _ptr(ws), ws_bytes
+    d.page_bytes, d.n_bases, d.n_pages, d.block_size, d.table_stride, d.n_seqs = page_bytes, n_bases, n_pages, block_size, table_stride, n_seqs
+    return d
+
+
+def cache_ws_bytes(desc: CacheDesc, n: int) -> int:
+    """Bytes of scratch that a call of n entries wants in desc.ws."""
+    return int(lib().atlas_b200_cache_ws_bytes(C.byref(desc), n))
+
+
+def cache_append(desc: CacheDesc, seqs, n_new, n: int, slot_mapping, max_tokens: int, status=None, stream=None) -> None:
+    """Pages for n_new[i] more tokens of sequence seqs[i]; the tokens' cache slots into slot_mapping."""
+    _check("atlas_b200_cache_append", lib().atlas_b200_cache_append(
+        C.byref(desc), _ptr(seqs), _ptr(n_new), n, max_tokens, _ptr(slot_mapping), _ptr(status), _stream_ptr(stream)))
+
+
+def cache_fork(desc: CacheDesc, src, dst, n: int, status=None, stream=None) -> None:
+    """The empty sequences dst[i] become copies of src[i]: full pages shared, a part-filled one copied."""
+    _check("atlas_b200_cache_fork", lib().atlas_b200_cache_fork(C.byref(desc), _ptr(src), _ptr(dst), n, _ptr(status), _stream_ptr(stream)))
+
+
+def cache_free(desc: CacheDesc, seqs, n: int, stream=None) -> None:
+    """The sequences give back their pages."""
+    _check("atlas_b200_cache_free", lib().atlas_b200_cache_free(C.byref(desc), _ptr(seqs), n, _stream_ptr(stream)))
+
+
+def cache_compact(desc: CacheDesc, refcount_out, block_table_out, page_map, n_used, stream=None) -> None:
+    """Pages in use move to the front of the pool; tables follow."""
+    _check("atlas_b200_cache_compact", lib().atlas_b200_cache_compact(
+        C.byref(desc), _ptr(refcount_out), _ptr(block_table_out), _ptr(page_map), _ptr(n_used), _stream_ptr(stream)))
 
 
 def make_linear_desc(*, x, m, k, n, y, w_packed=None, w_scale=None, scale2=1.0, w_bf16=None,

@@ -1,5 +1,6 @@
 // C ABI of the B200 NVFP4 + multi-LoRA linear path: argument validation, variant dispatch and
-// kernel launches.  Single translation unit (the kernels share one device status word).
+// kernel launches.  One translation unit (the kernels share one device status word); the attention over the paged cache and the
+// operators on its pages are another, cache_ops.cu.
 //
 // Host-side operator layer (namespace atlas::ops) mirrors the reference's launch wrappers:
 //   ops::apply_lora_bgmv   <- crates/spark-model/src/layers/ops/lora_delta.rs:269-314
@@ -23,6 +24,7 @@
 #include <new>
 
 #include "common.cuh"
+#include "host_launch.hpp"
 #include "kernel_tc.cuh"
 #include "kernel_tc_persist.cuh"
 #include "kernel_decode_mma.cuh"
@@ -41,24 +43,6 @@ static thread_local int t_last_variant = ATLAS_B200_VARIANT_NONE;
 static thread_local uint32_t t_last_shape[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 static unsigned long long* g_profile_buf = nullptr;   // device buffer for per-CTA cycle counters (diagnostics)
 static size_t g_profile_words = 0;
-
-static inline int cuda_status(cudaError_t e) { return e == cudaSuccess ? ATLAS_B200_OK : ATLAS_B200_ERR_CUDA_BASE - int(e); }
-static inline int launch_status() { return cuda_status(cudaGetLastError()); }
-// A launch of a kernel that begins with pdl_wait(): it may start while its predecessor in the stream finishes.
-template <typename... P, typename... A>
-static int launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t st, A... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
-}
-static inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // ---------------------------------------------------------------------------------------------
 // device capability and the tensor-map encoder (resolved from the driver at first use; the
@@ -118,6 +102,8 @@ static DeviceState* device_state() {
 }
 
 static int rt_sm_count() { DeviceState* st = device_state(); return st ? st->sm_count : 148; }
+int device_sm_count() { return rt_sm_count(); }
+bool device_is_sm100() { DeviceState* st = device_state(); return st && st->sm100 && g_encode; }
 
 // Encoded tensor maps are a pure function of (address, shape, strides, box, type, swizzle): a serving loop calls with the
 // same tensors step after step, so recent encodings are kept per host thread and a repeated call costs a compare instead of a
@@ -184,6 +170,11 @@ static bool encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, uint32_t rank
     if (rc != CUDA_SUCCESS) return false;
     if (e) { e->key = key; e->map = *map; e->used = ++t_map_tick; }
     return true;
+}
+
+bool encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dt, uint32_t rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                       const uint32_t* box, CUtensorMapSwizzle swz) {
+    return encode_tiled(map, dt, rank, base, dims, strides, box, swz);
 }
 
 static bool encode_2d(CUtensorMap* map, CUtensorMapDataType dt, size_t elem, const void* base, uint64_t inner,
@@ -1491,11 +1482,12 @@ int atlas_b200_kv_norm_mrope_cache_write(const void* k_in, const void* v_in, uin
                                     kv_heads, head_dim, rotary_dim, block_size, rms_eps, theta, stream);
 }
 
-int atlas_b200_qkv_norm_rope_cache_write(void* q, const void* k_in, const void* v_in, uint32_t q_row_stride, uint32_t kv_row_stride,
-                                         const void* q_norm_weight, const void* k_norm_weight, const uint32_t* positions,
-                                         const float* inv_freq, const long long* slot_mapping, void* k_cache, void* v_cache,
-                                         uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rotary_dim,
-                                         uint32_t block_size, float rms_eps, float attention_factor, int norm_offset_one, void* stream) {
+static int qkv_norm_rope_cache_write(void* q, const void* k_in, const void* v_in, uint32_t q_row_stride, uint32_t kv_row_stride,
+                                     const void* q_norm_weight, const void* k_norm_weight, const uint32_t* positions,
+                                     const float* inv_freq, const long long* slot_mapping, void* k_cache, void* v_cache,
+                                     uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rotary_dim,
+                                     uint32_t block_size, float rms_eps, float attention_factor, int norm_offset_one, void* stream, bool fp8 = false,
+                                     float k_inv_scale = 0.0f, float v_inv_scale = 0.0f) {
     if (!q || !k_in || !v_in || !q_norm_weight || !k_norm_weight || !positions || !slot_mapping || !k_cache || !v_cache ||
         (rotary_dim && !inv_freq))
         return ATLAS_B200_ERR_NULL;
@@ -1519,14 +1511,46 @@ int atlas_b200_qkv_norm_rope_cache_write(void* q, const void* k_in, const void* 
     p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = kv_heads; p.head_dim = head_dim; p.rotary_dim = rotary_dim;
     p.block_size = block_size; p.q_row_stride = q_row_stride; p.kv_row_stride = kv_row_stride;
     p.rms_eps = rms_eps; p.attention_factor = attention_factor; p.norm_offset_one = norm_offset_one ? 1u : 0u;
+    p.k_inv_scale = k_inv_scale; p.v_inv_scale = v_inv_scale;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool exact = rotary_dim == 64 && (head_dim == 64 || head_dim == 128 || head_dim == 256);
+    if (fp8) {
+        if (head_dim <= 64) return exact ? launch_chained(qkv_norm_rope_cache_kernel<1, true, true>, tokens, KVE_WARPS * 32, st, p)
+                                  : launch_chained(qkv_norm_rope_cache_kernel<1, false, true>, tokens, KVE_WARPS * 32, st, p);
+        if (head_dim <= 128) return exact ? launch_chained(qkv_norm_rope_cache_kernel<2, true, true>, tokens, KVE_WARPS * 32, st, p)
+                                        : launch_chained(qkv_norm_rope_cache_kernel<2, false, true>, tokens, KVE_WARPS * 32, st, p);
+        return exact ? launch_chained(qkv_norm_rope_cache_kernel<4, true, true>, tokens, KVE_WARPS * 32, st, p)
+                   : launch_chained(qkv_norm_rope_cache_kernel<4, false, true>, tokens, KVE_WARPS * 32, st, p);
+    }
     if (head_dim <= 64) return exact ? launch_chained(qkv_norm_rope_cache_kernel<1, true>, tokens, KVE_WARPS * 32, st, p)
                               : launch_chained(qkv_norm_rope_cache_kernel<1, false>, tokens, KVE_WARPS * 32, st, p);
     if (head_dim <= 128) return exact ? launch_chained(qkv_norm_rope_cache_kernel<2, true>, tokens, KVE_WARPS * 32, st, p)
                                     : launch_chained(qkv_norm_rope_cache_kernel<2, false>, tokens, KVE_WARPS * 32, st, p);
     return exact ? launch_chained(qkv_norm_rope_cache_kernel<4, true>, tokens, KVE_WARPS * 32, st, p)
                : launch_chained(qkv_norm_rope_cache_kernel<4, false>, tokens, KVE_WARPS * 32, st, p);
+}
+
+int atlas_b200_qkv_norm_rope_cache_write(void* q, const void* k_in, const void* v_in, uint32_t q_row_stride, uint32_t kv_row_stride,
+                                         const void* q_norm_weight, const void* k_norm_weight, const uint32_t* positions,
+                                         const float* inv_freq, const long long* slot_mapping, void* k_cache, void* v_cache,
+                                         uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rotary_dim,
+                                         uint32_t block_size, float rms_eps, float attention_factor, int norm_offset_one, void* stream) {
+    return qkv_norm_rope_cache_write(q, k_in, v_in, q_row_stride, kv_row_stride, q_norm_weight, k_norm_weight, positions, inv_freq, slot_mapping,
+                                     k_cache, v_cache, tokens, q_heads, kv_heads, head_dim, rotary_dim, block_size, rms_eps, attention_factor,
+                                     norm_offset_one, stream);
+}
+
+int atlas_b200_qkv_norm_rope_cache_write_fp8(void* q, const void* k_in, const void* v_in, uint32_t q_row_stride, uint32_t kv_row_stride,
+                                             const void* q_norm_weight, const void* k_norm_weight, const uint32_t* positions,
+                                             const float* inv_freq, const long long* slot_mapping, void* k_cache_fp8, void* v_cache_fp8,
+                                             uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rotary_dim,
+                                             uint32_t block_size, float rms_eps, float attention_factor, int norm_offset_one,
+                                             float k_inv_scale, float v_inv_scale, void* stream) {
+    if (!(k_inv_scale > 0.0f) || !(v_inv_scale > 0.0f) || !std::isfinite(k_inv_scale) || !std::isfinite(v_inv_scale)) return ATLAS_B200_ERR_DIMS;
+    if (!aligned(k_cache_fp8, 2) || !aligned(v_cache_fp8, 4)) return ATLAS_B200_ERR_ALIGN;   // (pairs of codes are written as 16-bit words)
+    return qkv_norm_rope_cache_write(q, k_in, v_in, q_row_stride, kv_row_stride, q_norm_weight, k_norm_weight, positions, inv_freq, slot_mapping,
+                                     k_cache_fp8, v_cache_fp8, tokens, q_heads, kv_heads, head_dim, rotary_dim, block_size, rms_eps,
+                                     attention_factor, norm_offset_one, stream, true, k_inv_scale, v_inv_scale);
 }
 
 int atlas_b200_copy_columns(const void* src, uint32_t src_row_stride, void* const* dest, uint32_t n_dest, uint32_t dst_row_stride,
@@ -1650,8 +1674,12 @@ int atlas_b200_device_status(uint32_t* out_word, int clear) {
     if (clear) {
         const uint32_t zero = 0;
         e = cudaMemcpyToSymbol(g_status_word, &zero, sizeof(uint32_t));
+        if (e != cudaSuccess) return cuda_status(e);
     }
-    return cuda_status(e);
+    uint32_t more = 0;                                       // the cache operators' kernels have a word of their own
+    const int rc = cache_device_status(&more, clear);
+    if (*out_word == 0) *out_word = more;
+    return rc;
 }
 
 int atlas_b200_selftest_bounded_wait(uint64_t limit_ns, uint32_t out_host[3]) {

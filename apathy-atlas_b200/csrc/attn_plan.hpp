@@ -1,0 +1,103 @@
+// How the attention over the paged cache is cut into pieces of equal work, in plain C++ so that it is checked on the CPU.
+//
+// Of one sequence and one KV head, the chunk's rows are its new tokens times the `group` query heads that share the KV head: row r is
+// token r / group, head r % group of them.  `block_rows` rows make a block; a block reads the keys its last row sees, in tiles of
+// `tile_keys`.  An item is one (sequence, block, KV head).  All items' tiles in a row (sequence, block, KV head, tile; the last fastest)
+// are the line that CTAs cut into contiguous ranges of equal length, whatever the sequences' lengths: a range may begin and end inside
+// an item, whose pieces are joined afterwards.
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifndef ATLAS_HD
+#ifdef __CUDACC__
+#define ATLAS_HD __host__ __device__
+#else
+#define ATLAS_HD
+#endif
+#endif
+
+namespace atlas {
+
+// sum of floor((a i + b) / m) over i = 0 .. n - 1, by Euclid's algorithm on (a, m)
+ATLAS_HD inline uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+    uint64_t sum = 0;
+    while (n > 0) {
+        if (a >= m) { sum += (a / m) * (n * (n - 1) / 2); a %= m; }
+        if (b >= m) { sum += (b / m) * n; b %= m; }
+        const uint64_t last = a * n + b;
+        if (last < m) break;
+        n = last / m;
+        b = last % m;
+        const uint64_t t = m;
+        m = a;
+        a = t;
+    }
+    return sum;
+}
+
+// One sequence's blocks.  Without new tokens it has none; with fewer cached tokens than new ones (the first rows see nothing) all of
+// its blocks count as if they saw the whole cache.
+struct AttnSeq {
+    uint32_t q_len, kv_len, blocks, whole;      // whole: tiles of the cached tokens, one at least
+    uint32_t group, block_rows, tile_keys;
+    ATLAS_HD AttnSeq(uint32_t q, uint32_t kv, uint32_t g, uint32_t rows, uint32_t keys) : q_len(q), kv_len(kv), group(g), block_rows(rows), tile_keys(keys) {
+        blocks = uint32_t((uint64_t(q) * g + rows - 1) / rows);
+        whole = kv ? (kv - 1) / keys + 1 : 1;
+    }
+    // the last row of block b is row (b + 1) rows - 1, token floor of it / group; it sees kv_len - q_len + that token + 1 keys
+    ATLAS_HD uint32_t tiles(uint32_t b) const {
+        if (kv_len < q_len || b + 1 >= blocks) return whole;
+        const uint64_t keys_less_1 = uint64_t(kv_len - q_len) + tile_keys;
+        const uint64_t t = (uint64_t(block_rows) * b + block_rows - 1 + uint64_t(group) * keys_less_1) / (uint64_t(group) * tile_keys);
+        return t < whole ? uint32_t(t) : whole;
+    }
+    // tiles of the blocks before b
+    ATLAS_HD uint64_t before(uint32_t b) const {
+        if (b == 0 || blocks == 0) return 0;
+        const uint32_t n = b < blocks ? b : blocks - 1;                                   // by the formula
+        uint64_t sum = kv_len < q_len ? uint64_t(whole) * n
+                                      : floor_sum(n, uint64_t(group) * tile_keys, block_rows, block_rows - 1 + uint64_t(group) * (uint64_t(kv_len - q_len) + tile_keys));
+        return b < blocks ? sum : sum + whole;
+    }
+    ATLAS_HD uint64_t total(uint32_t kv_heads) const { return before(blocks) * kv_heads; }
+};
+
+struct AttnPlace {
+    uint32_t block, head, tile, tiles;          // tile of the item, of `tiles`
+};
+// where place x of a sequence's part of the line lies, x < total(kv_heads)
+ATLAS_HD inline AttnPlace attn_locate(const AttnSeq& s, uint32_t kv_heads, uint64_t x) {
+    uint32_t lo = 0, hi = s.blocks - 1;
+    while (lo < hi) {                                                                     // the last block that begins at or before x
+        const uint32_t mid = (lo + hi + 1) / 2;
+        if (s.before(mid) * kv_heads <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    AttnPlace p;
+    p.block = lo;
+    p.tiles = s.tiles(lo);
+    const uint64_t in_block = x - s.before(lo) * kv_heads;
+    p.head = uint32_t(in_block / p.tiles);
+    p.tile = uint32_t(in_block % p.tiles);
+    return p;
+}
+
+// Range c of `ranges` over a line of `total` places begins here; range_of: the one that place x belongs to.
+ATLAS_HD inline uint64_t attn_range_begin(uint64_t total, uint32_t ranges, uint32_t c) {
+    const uint64_t each = total / ranges, more = total % ranges;                          // the first `more` are one longer
+    return each * c + (c < more ? c : more);
+}
+ATLAS_HD inline uint32_t attn_range_of(uint64_t total, uint32_t ranges, uint64_t x) {
+    const uint64_t each = total / ranges, more = total % ranges;
+    const uint64_t longer = more * (each + 1);
+    return x < longer ? uint32_t(x / (each + 1)) : uint32_t(more + (x - longer) / each);
+}
+// how many of the `ctas` CTAs take part where each is to have `least` places at least
+ATLAS_HD inline uint32_t attn_ranges(uint64_t total, uint32_t ctas, uint32_t least) {
+    const uint64_t n = (total + least - 1) / least;
+    return n < 1 ? 1u : n < ctas ? uint32_t(n) : ctas;
+}
+
+}  // namespace atlas

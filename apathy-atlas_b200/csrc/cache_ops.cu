@@ -1,0 +1,261 @@
+// The operators around the paged K/V cache: attention that reads it, and its pages between two steps.  Argument checks, choice of
+// kernel and launches; like the rest of the library it allocates nothing, does not synchronise and reads no device memory on the host.
+#include "atlas_b200.h"
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <mutex>
+
+#include "common.cuh"
+#include "host_launch.hpp"
+#include "kernel_attn.cuh"
+#include "kernel_attn_mma.cuh"
+#include "kernel_cache_pages.cuh"
+
+namespace atlas {
+
+int cache_device_status(uint32_t* out_word, int clear) {
+    cudaError_t e = cudaMemcpyFromSymbol(out_word, g_status_word, sizeof(uint32_t));
+    if (e == cudaSuccess && clear) {
+        const uint32_t zero = 0;
+        e = cudaMemcpyToSymbol(g_status_word, &zero, sizeof(uint32_t));
+    }
+    return cuda_status(e);
+}
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+std::mutex g_attr_mutex;
+
+// Dynamic shared memory above 48 KB is a setting of a kernel on a device: made at its first launch there.
+template <typename K> int allow_smem(K kernel, int bytes, std::atomic<bool> (&done)[kMaxDevices]) {
+    int dev = -1;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return cuda_status(e);
+    if (dev < 0 || dev >= kMaxDevices) return ATLAS_B200_ERR_LIMIT;
+    if (done[dev].load(std::memory_order_acquire)) return ATLAS_B200_OK;
+    std::lock_guard<std::mutex> lock(g_attr_mutex);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
+    return cuda_status(e);
+}
+
+template <typename... P, typename... A>
+int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+}
+
+// ---------------------------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------------------------
+thread_local uint32_t t_attn_shape[4] = {0, 0, 0, 0};
+
+uint32_t attn_dim(uint32_t head_dim) { return head_dim <= 64 ? 64u : head_dim <= 128 ? 128u : 256u; }
+
+int check_attention(const atlas_b200_attention_desc& d) {
+    if (d.q_heads == 0 || d.kv_heads == 0 || d.q_heads % d.kv_heads || d.head_dim == 0 || d.head_dim % 32 || d.head_dim > 256 || d.block_size == 0 ||
+        d.table_stride == 0 || d.n_pages == 0)
+        return ATLAS_B200_ERR_DIMS;
+    if (d.cache_dtype != ATLAS_B200_CACHE_BF16 && d.cache_dtype != ATLAS_B200_CACHE_E4M3) return ATLAS_B200_ERR_DIMS;
+    if (uint64_t(d.q_heads) * d.head_dim > d.q_row_stride || uint64_t(d.q_heads) * d.head_dim > d.out_row_stride) return ATLAS_B200_ERR_DIMS;
+    if (!(d.softmax_scale > 0.0f) || !std::isfinite(d.softmax_scale) || !(d.k_scale > 0.0f) || !std::isfinite(d.k_scale) || !(d.v_scale > 0.0f) ||
+        !std::isfinite(d.v_scale))
+        return ATLAS_B200_ERR_DIMS;
+    if (d.cache_dtype == ATLAS_B200_CACHE_BF16 && (d.k_scale != 1.0f || d.v_scale != 1.0f)) return ATLAS_B200_ERR_DIMS;
+    // rows of the cache and places of a sequence are counted in 31 bits
+    if (uint64_t(d.n_pages) * d.block_size >= (1ull << 31) || uint64_t(d.table_stride) * d.block_size >= (1ull << 31) || d.n_seqs >= (1u << 24) ||
+        d.n_tokens >= (1u << 31) || uint64_t(d.n_tokens) * (d.q_heads / d.kv_heads) >= (1ull << 31))
+        return ATLAS_B200_ERR_LIMIT;
+    if (!d.q || !d.out || !d.k_cache || !d.v_cache || !d.block_table || !d.cu_q || !d.kv_len) return ATLAS_B200_ERR_NULL;
+    if (!aligned(d.q, 4) || d.q_row_stride % 2 || !aligned(d.out, 2) || !aligned(d.k_cache, 16) || !aligned(d.v_cache, 16) || !aligned(d.block_table, 4) ||
+        !aligned(d.cu_q, 4) || !aligned(d.kv_len, 4) || !aligned(d.lse, 4) || !aligned(d.ws, 16))
+        return ATLAS_B200_ERR_ALIGN;
+    return ATLAS_B200_OK;
+}
+
+AttnParams attention_params(const atlas_b200_attention_desc& d) {
+    AttnParams p{};
+    p.q = static_cast<const uint16_t*>(d.q);
+    p.out = static_cast<uint16_t*>(d.out);
+    p.lse = d.lse;
+    p.k_cache = static_cast<const uint8_t*>(d.k_cache);
+    p.v_cache = static_cast<const uint8_t*>(d.v_cache);
+    p.block_table = d.block_table; p.cu_q = d.cu_q; p.kv_len = d.kv_len;
+    p.parts = static_cast<float*>(d.ws);
+    p.n_seqs = d.n_seqs; p.n_tokens = d.n_tokens; p.n_pages = d.n_pages; p.table_stride = d.table_stride;
+    p.q_heads = d.q_heads; p.kv_heads = d.kv_heads; p.head_dim = d.head_dim; p.block_size = d.block_size; p.group = d.q_heads / d.kv_heads;
+    p.q_row_stride = d.q_row_stride; p.out_row_stride = d.out_row_stride;
+    p.scale = d.softmax_scale; p.k_scale = d.k_scale; p.v_scale = d.v_scale;
+    return p;
+}
+
+// The mma.sync form: how many CTAs, and whether each takes whole items.
+struct MmaPlan {
+    uint32_t ctas, by_item, least;
+    size_t ws_bytes;
+};
+MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms) {
+    const uint32_t dim = attn_dim(d.head_dim);
+    const uint32_t resident = sms * (dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u) >= 512u ? 1u : 2u);
+    const uint64_t group = d.q_heads / d.kv_heads;
+    const uint64_t rows = std::min<uint64_t>(d.max_q_len, d.n_tokens) * group;
+    const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * std::max<uint64_t>((rows + attn::MMA_ROWS - 1) / attn::MMA_ROWS, 1);
+    const uint64_t tiles = std::max<uint64_t>((uint64_t(d.max_kv_len) + attn::MMA_TILE - 1) / attn::MMA_TILE, 1);
+    MmaPlan r{};
+    r.by_item = tiles <= 4;
+    r.least = r.by_item ? 1u : 4u;
+    const uint64_t places = r.by_item ? items : (items * tiles + r.least - 1) / r.least;
+    r.ctas = uint32_t(std::min<uint64_t>(resident, std::max<uint64_t>(places, 1)));
+    r.ws_bytes = r.by_item ? 0 : size_t(resident) * 2 * attn_part_floats(attn::MMA_ROWS, dim) * sizeof(float);
+    return r;
+}
+
+template <int DP, bool FP8> int launch_mma(AttnParams p, const MmaPlan& plan, cudaStream_t st) {
+    using C = attn::MmaCfg<DP, FP8>;
+    static std::atomic<bool> done[kMaxDevices] = {};
+    const int rc = allow_smem(attn::attn_mma_kernel<DP, FP8>, C::SMEM, done);
+    if (rc) return rc;
+    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item;
+    const int rc2 = launch_dependent(attn::attn_mma_kernel<DP, FP8>, plan.ctas, attn::MMA_THREADS, C::SMEM, st, p, attn_divisor(p.block_size));
+    if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
+    return launch_dependent(attn_join_kernel<attn::MMA_ROWS, attn::MMA_TILE, DP, FP8>, plan.ctas - 1, ATTN_JOIN_THREADS, 0, st, p);
+}
+
+int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
+    if (d.n_seqs == 0 || d.n_tokens == 0) return ATLAS_B200_OK;
+    const int bad = check_attention(d);
+    if (bad) return bad;
+    if (!device_is_sm100()) return ATLAS_B200_ERR_ARCH;
+    const uint32_t sms = uint32_t(device_sm_count()), dim = attn_dim(d.head_dim);
+    MmaPlan plan = plan_mma(d, sms);
+    if (d.ws ? d.ws_bytes < plan.ws_bytes : d.ws_bytes != 0) return ATLAS_B200_ERR_WORKSPACE;
+    if (!d.ws && !plan.by_item) { plan.by_item = 1; plan.least = 1; }        // (no scratch: nothing is cut)
+    const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3;
+    const AttnParams p = attention_params(d);
+    t_attn_shape[0] = attn::MMA_ROWS; t_attn_shape[1] = plan.ctas; t_attn_shape[2] = plan.by_item; t_attn_shape[3] = attn::MMA_TILE;
+    if (dim == 64) return fp8 ? launch_mma<64, true>(p, plan, st) : launch_mma<64, false>(p, plan, st);
+    if (dim == 128) return fp8 ? launch_mma<128, true>(p, plan, st) : launch_mma<128, false>(p, plan, st);
+    return fp8 ? launch_mma<256, true>(p, plan, st) : launch_mma<256, false>(p, plan, st);
+}
+
+// ---------------------------------------------------------------------------------------------
+// pages
+// ---------------------------------------------------------------------------------------------
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t pages_ws_bytes(const atlas_b200_cache_desc& d, uint32_t n) {
+    return round256(size_t(d.n_seqs) * 4) + round256(size_t(n) * 16) + round256(size_t(d.n_pages) * 4) + 256;
+}
+
+int check_pages(const atlas_b200_cache_desc& d, uint32_t n, bool copies, pages::PagesParams& p) {
+    if (d.n_pages == 0 || d.block_size == 0 || d.table_stride == 0 || d.n_seqs == 0) return ATLAS_B200_ERR_DIMS;
+    if (copies && (d.page_bytes == 0 || d.page_bytes % d.block_size || d.page_bytes % 16)) return ATLAS_B200_ERR_DIMS;
+    if (d.n_pages >= (1u << 31) || d.n_seqs >= (1u << 31) || uint64_t(d.table_stride) * d.block_size >= (1ull << 31) || n >= (1u << 24) || d.n_bases > 65535u)
+        return ATLAS_B200_ERR_LIMIT;
+    if (!d.refcount || !d.block_table || !d.seq_len || !d.ws || (copies && d.n_bases && !d.bases)) return ATLAS_B200_ERR_NULL;
+    if (!aligned(d.refcount, 4) || !aligned(d.block_table, 4) || !aligned(d.seq_len, 4) || !aligned(d.bases, 8) || !aligned(d.ws, 16)) return ATLAS_B200_ERR_ALIGN;
+    if (d.ws_bytes < pages_ws_bytes(d, n)) return ATLAS_B200_ERR_WORKSPACE;
+    p.bases = d.bases;
+    p.refcount = d.refcount; p.block_table = d.block_table; p.seq_len = d.seq_len;
+    p.n_bases = d.n_bases; p.n_pages = d.n_pages; p.block_size = d.block_size; p.table_stride = d.table_stride; p.n_seqs = d.n_seqs;
+    p.page_bytes = d.page_bytes;
+    uint8_t* ws = static_cast<uint8_t*>(d.ws);
+    p.claim = reinterpret_cast<int32_t*>(ws);
+    p.entry = reinterpret_cast<int32_t*>(ws + round256(size_t(d.n_seqs) * 4));
+    p.list = reinterpret_cast<int32_t*>(ws + round256(size_t(d.n_seqs) * 4) + round256(size_t(n) * 16));
+    p.count = reinterpret_cast<int32_t*>(ws + round256(size_t(d.n_seqs) * 4) + round256(size_t(n) * 16) + round256(size_t(d.n_pages) * 4));
+    return ATLAS_B200_OK;
+}
+
+}  // namespace
+}  // namespace atlas
+
+using namespace atlas;
+
+extern "C" {
+
+int atlas_b200_paged_attention(const atlas_b200_attention_desc* desc, void* stream) {
+    if (!desc) return ATLAS_B200_ERR_NULL;
+    return attention(*desc, static_cast<cudaStream_t>(stream));
+}
+
+size_t atlas_b200_paged_attention_ws_bytes(const atlas_b200_attention_desc* desc) {
+    if (!desc || desc->kv_heads == 0 || desc->q_heads % desc->kv_heads || desc->n_seqs == 0 || desc->n_tokens == 0) return 0;
+    return plan_mma(*desc, uint32_t(device_sm_count())).ws_bytes;
+}
+
+int atlas_b200_last_attention_shape(uint32_t out[4]) {
+    if (!out) return ATLAS_B200_ERR_NULL;
+    for (int i = 0; i < 4; ++i) out[i] = t_attn_shape[i];
+    return ATLAS_B200_OK;
+}
+
+size_t atlas_b200_cache_ws_bytes(const atlas_b200_cache_desc* desc, uint32_t n) { return desc ? pages_ws_bytes(*desc, n) : 0; }
+
+int atlas_b200_cache_append(const atlas_b200_cache_desc* desc, const int32_t* seqs, const int32_t* n_new, uint32_t n, uint32_t max_tokens,
+                            long long* slot_mapping, int32_t* status, void* stream) {
+    if (!desc) return ATLAS_B200_ERR_NULL;
+    if (n == 0 && max_tokens == 0) return ATLAS_B200_OK;
+    if ((n && (!seqs || !n_new)) || (max_tokens && !slot_mapping)) return ATLAS_B200_ERR_NULL;
+    if (max_tokens >= (1u << 31)) return ATLAS_B200_ERR_LIMIT;
+    if (!aligned(seqs, 4) || !aligned(n_new, 4) || !aligned(slot_mapping, 8) || !aligned(status, 4)) return ATLAS_B200_ERR_ALIGN;
+    pages::PagesParams p{};
+    const int bad = check_pages(*desc, n, false, p);
+    if (bad) return bad;
+    return launch_dependent(pages::append_kernel, 1, pages::PLAN_THREADS, 0, static_cast<cudaStream_t>(stream), p, seqs, n_new, n, max_tokens, slot_mapping, status);
+}
+
+int atlas_b200_cache_fork(const atlas_b200_cache_desc* desc, const int32_t* src, const int32_t* dst, uint32_t n, int32_t* status, void* stream) {
+    if (!desc) return ATLAS_B200_ERR_NULL;
+    if (n == 0) return ATLAS_B200_OK;
+    if (!src || !dst) return ATLAS_B200_ERR_NULL;
+    if (!aligned(src, 4) || !aligned(dst, 4) || !aligned(status, 4)) return ATLAS_B200_ERR_ALIGN;
+    pages::PagesParams p{};
+    const int bad = check_pages(*desc, n, true, p);
+    if (bad) return bad;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int rc = launch_dependent(pages::fork_plan_kernel, 1, pages::PLAN_THREADS, 0, st, p, src, dst, n, status);
+    if (rc) return rc;
+    return launch_dependent(pages::fork_copy_kernel, dim3(n, std::max(desc->n_bases, 1u)), pages::COPY_THREADS, 0, st, p, src, dst);
+}
+
+int atlas_b200_cache_free(const atlas_b200_cache_desc* desc, const int32_t* seqs, uint32_t n, void* stream) {
+    if (!desc) return ATLAS_B200_ERR_NULL;
+    if (n == 0) return ATLAS_B200_OK;
+    if (!seqs) return ATLAS_B200_ERR_NULL;
+    if (!aligned(seqs, 4)) return ATLAS_B200_ERR_ALIGN;
+    pages::PagesParams p{};
+    const int bad = check_pages(*desc, n, false, p);
+    if (bad) return bad;
+    return launch_dependent(pages::free_kernel, n, pages::FREE_THREADS, 0, static_cast<cudaStream_t>(stream), p, seqs);
+}
+
+int atlas_b200_cache_compact(const atlas_b200_cache_desc* desc, int32_t* refcount_out, int32_t* block_table_out, int32_t* page_map, int32_t* n_used, void* stream) {
+    if (!desc || !refcount_out || !block_table_out || !page_map || !n_used) return ATLAS_B200_ERR_NULL;
+    if (!aligned(refcount_out, 4) || !aligned(block_table_out, 4) || !aligned(page_map, 4) || !aligned(n_used, 4)) return ATLAS_B200_ERR_ALIGN;
+    pages::PagesParams p{};
+    const int bad = check_pages(*desc, 0, true, p);
+    if (bad) return bad;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int rc = launch_dependent(pages::compact_plan_kernel, 1, pages::PLAN_THREADS, 0, st, p, refcount_out, page_map, n_used);
+    if (rc) return rc;
+    return launch_dependent(pages::compact_move_kernel, uint32_t(device_sm_count()) * 4, pages::COPY_THREADS, 0, st, p, page_map, block_table_out);
+}
+
+}  // extern "C"

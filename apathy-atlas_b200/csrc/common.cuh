@@ -16,6 +16,10 @@ enum : uint32_t {
     STATUS_SLOT_OUT_OF_RANGE = 1,   // seq_slot[i] >= max_loras
     STATUS_NEGATIVE_SCALE = 2,      // FP4-activation mode met a weight scale byte with its sign bit set; the sign was dropped
     STATUS_TILE_CAPACITY = 3,       // the shrink met more (slot, granule) pairs in a token tile than its tile output reserves
+    STATUS_PAGE_OUT_OF_RANGE = 4,   // a block table names a page that the cache does not have; the attention reads it as zeros
+    STATUS_CACHE_LENGTH = 5,        // a sequence is longer than its row of the block table; what fits is taken
+    STATUS_SEQ_OUT_OF_RANGE = 6,    // a page operator was given a sequence that the tables do not have; it does nothing for it
+    STATUS_PAGE_NOT_HELD = 7,       // a sequence gave back a page that nothing referred to; it stays free
     STATUS_WAIT_EXPIRED_PRODUCER = 0x100,
     STATUS_WAIT_EXPIRED_DEQUANT = 0x101,
     STATUS_WAIT_EXPIRED_MMA = 0x102,

@@ -1,0 +1,237 @@
+// Attention of the new tokens of a batch of sequences over their paged K/V cache: what the kernels share.
+//
+//   o[t, h] = sum_j p_j v[j, h / group],   p = softmax_j( scale * q[t, h] . k[j, h / group] ),   j <= kv_len - q_len + (t - first token)
+//
+// with the running maximum and sum of a softmax held in FP32: of each piece of the keys a kernel has M (largest score, in units of
+// log 2), L = sum 2^(s - M) and O = sum 2^(s - M) v; two pieces join as M = max, L = L1 2^(M1 - M) + L2 2^(M2 - M), O likewise.
+// A row that sees no key has L = 0 and gives zeros, and -inf as its logarithm.
+//
+// The line of tiles of all items (attn_plan.hpp) is cut into one range a CTA.  An item that lies in one range is written at once; the
+// pieces of one that does not go to scratch, two slots a CTA (the item its range begins in, the item its range ends in), and
+// attn_join_kernel adds them in the order of their keys: the same call gives the same bits.
+#pragma once
+
+#include <cstdint>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include "attn_plan.hpp"
+#include "common.cuh"
+
+namespace atlas {
+
+constexpr float ATTN_LOG2E = 1.4426950408889634f, ATTN_LN2 = 0.6931471805599453f;
+
+struct AttnParams {
+    const uint16_t* q;            // first column of row 0, rows q_row_stride elements apart
+    uint16_t* out;
+    float* lse;                   // [n_tokens, q_heads], or null
+    const uint8_t* k_cache;       // [n_pages, block_size, kv_heads, head_dim]
+    const uint8_t* v_cache;
+    const int32_t* block_table;   // [n_seqs, table_stride]
+    const int32_t* cu_q;          // [n_seqs + 1]
+    const int32_t* kv_len;        // [n_seqs]
+    float* parts;                 // two slots a range of block_rows rows: O, then M and L (see part_floats)
+    uint32_t n_seqs, n_tokens, n_pages, table_stride, q_heads, kv_heads, head_dim, block_size, group, q_row_stride, out_row_stride;
+    uint32_t ctas, least_tiles;   // ranges: at most `ctas`, of `least_tiles` tiles each at least
+    uint32_t by_item;             // every CTA takes whole items: no pieces
+    float scale, k_scale, v_scale;
+};
+
+// page and place in it of a position: a product with a rounded-up reciprocal is exact for positions below 2^31 (checked at launch by
+// its construction: m = ceil(2^(31 + s) / d) with 2^s >= d)
+struct AttnDivisor {
+    uint32_t d, mul, shift;
+};
+__host__ __device__ inline AttnDivisor attn_divisor(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return AttnDivisor{d, uint32_t(((1ull << (31 + s)) + d - 1) / d), s};
+}
+__device__ __forceinline__ uint32_t attn_div(uint32_t x, const AttnDivisor& v) { return uint32_t((uint64_t(x) * v.mul) >> (31 + v.shift)); }
+
+__host__ __device__ constexpr size_t attn_part_floats(uint32_t block_rows, uint32_t dim) { return size_t(block_rows) * dim + 2 * block_rows; }
+
+struct AttnSeqAt {
+    uint32_t row0, q_len, kv_len;
+};
+// A sequence as its tables have it, held to what the buffers hold.
+__device__ __forceinline__ AttnSeqAt attn_seq(const AttnParams& p, uint32_t s) {
+    const int32_t a = p.cu_q[s], b = p.cu_q[s + 1], n = p.kv_len[s];
+    AttnSeqAt r;
+    r.row0 = a < 0 ? 0u : min(uint32_t(a), p.n_tokens);
+    const uint32_t end = b < 0 ? 0u : min(uint32_t(b), p.n_tokens);
+    r.q_len = end > r.row0 ? end - r.row0 : 0u;
+    const uint64_t room = uint64_t(p.table_stride) * p.block_size;
+    r.kv_len = n < 0 ? 0u : (uint64_t(n) > room ? uint32_t(room) : uint32_t(n));
+    if (n > 0 && uint64_t(n) > room) record_status(STATUS_CACHE_LENGTH);
+    return r;
+}
+
+// How many keys new token i of a sequence sees.
+__device__ __forceinline__ uint32_t attn_row_keys(const AttnSeqAt& s, uint32_t i) {
+    const uint64_t n = uint64_t(s.kv_len) + i + 1;
+    return n <= s.q_len ? 0u : uint32_t(n - s.q_len);
+}
+
+// Length of the line, in places (tiles, or items where p.by_item), and the sequence that place `x` lies in.  By all THREADS threads of a
+// CTA; `sh`: THREADS / 32 + 3 words of 64 bits.
+struct AttnFound {
+    uint64_t total, seq_begin;    // seq_begin: the place where the sequence begins
+    uint32_t seq;
+};
+__device__ __forceinline__ uint64_t attn_seq_places(const AttnParams& p, uint32_t s, uint32_t rows, uint32_t keys) {
+    const AttnSeqAt q = attn_seq(p, s);
+    const AttnSeq a(q.q_len, q.kv_len, p.group, rows, keys);
+    return p.by_item ? uint64_t(a.blocks) * p.kv_heads : a.total(p.kv_heads);
+}
+template <int THREADS, typename F>
+__device__ __forceinline__ AttnFound attn_find(const AttnParams& p, uint32_t rows, uint32_t keys, uint64_t* sh, F place_of_total) {
+    constexpr int WARPS = THREADS / 32;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    const uint32_t each = (p.n_seqs + THREADS - 1) / THREADS, s0 = min(tid * each, p.n_seqs), s1 = min(s0 + each, p.n_seqs);
+    uint64_t mine = 0;
+    for (uint32_t s = s0; s < s1; ++s) mine += attn_seq_places(p, s, rows, keys);
+    uint64_t upto = mine;
+#pragma unroll
+    for (uint32_t o = 1; o < 32; o <<= 1) {
+        const uint64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31u) sh[warp] = upto;
+    __syncthreads();
+    uint64_t before = 0, total = 0;
+    for (int w = 0; w < WARPS; ++w) {
+        if (w < int(warp)) before += sh[w];
+        total += sh[w];
+    }
+    const uint64_t x = place_of_total(total);
+    const uint64_t end = before + upto, begin = end - mine;
+    if (mine && x >= begin && x < end) {                                                  // (one thread at most)
+        uint64_t at = begin;
+        for (uint32_t s = s0; s < s1; ++s) {
+            const uint64_t n = s1 - s0 == 1 ? mine : attn_seq_places(p, s, rows, keys);
+            if (x < at + n) { sh[WARPS] = s; sh[WARPS + 1] = at; break; }
+            at += n;
+        }
+    }
+    __syncthreads();
+    AttnFound f;
+    f.total = total;
+    f.seq = uint32_t(sh[WARPS]);
+    f.seq_begin = sh[WARPS + 1];
+    __syncthreads();
+    return f;
+}
+
+// Row `pos` of a sequence in the cache seen as [pages * block_size, kv_heads, head_dim]; -1 and a record where the table names no page.
+__device__ __forceinline__ int32_t attn_cache_row(const AttnParams& p, const AttnDivisor& div, const int32_t* table, uint32_t pos) {
+    const uint32_t page = attn_div(pos, div), id = uint32_t(table[page]);
+    if (id >= p.n_pages) { record_status(STATUS_PAGE_OUT_OF_RANGE); return -1; }
+    return int32_t(id * p.block_size + (pos - page * p.block_size));
+}
+
+__device__ __forceinline__ float attn_e4m3(uint8_t b) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3))); }
+
+// One row again from its own keys alone, by one warp.  The kernels multiply masked places with zeros, and zero times an infinity or a
+// NaN in the values of a later token is a NaN; a row that came out not finite is computed here instead, which leaves other tokens'
+// values unread.  The cost (a chain over the row's keys) is paid by such rows only.
+static __device__ __noinline__ void attn_row_again(const AttnParams& p, bool fp8, uint32_t seq, uint32_t token, uint32_t head, uint32_t keys) {
+    const uint32_t lane = threadIdx.x & 31u, D = p.head_dim;
+    const AttnDivisor div = attn_divisor(p.block_size);
+    const int32_t* table = p.block_table + size_t(seq) * p.table_stride;
+    const uint16_t* q = p.q + size_t(token) * p.q_row_stride + size_t(head) * D;
+    float qv[8], o[8] = {}, m = -INFINITY, l = 0.0f;
+    for (uint32_t i = 0; i < 8; ++i) qv[i] = lane + 32u * i < D ? __uint_as_float(uint32_t(q[lane + 32u * i]) << 16) : 0.0f;
+    const float c = p.scale * p.k_scale * ATTN_LOG2E;
+    for (uint32_t j = 0; j < keys; ++j) {
+        const int32_t row = attn_cache_row(p, div, table, j);
+        const size_t at = (size_t(row < 0 ? 0 : row) * p.kv_heads + head / p.group) * D;
+        float s = 0.0f, v[8];
+        for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t d = lane + 32u * i;
+            v[i] = 0.0f;
+            if (row < 0 || d >= D) continue;
+            const float k = fp8 ? attn_e4m3(p.k_cache[at + d]) : __uint_as_float(uint32_t(reinterpret_cast<const uint16_t*>(p.k_cache)[at + d]) << 16);
+            v[i] = fp8 ? attn_e4m3(p.v_cache[at + d]) : __uint_as_float(uint32_t(reinterpret_cast<const uint16_t*>(p.v_cache)[at + d]) << 16);
+            s = fmaf(qv[i], k, s);
+        }
+        for (uint32_t x = 16; x; x >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, x);
+        s *= c;
+        const float top = fmaxf(m, s), base = top == -INFINITY ? 0.0f : top;
+        const float keep = exp2f(m - base), w = exp2f(s - base);
+        l = l * keep + w;
+        for (uint32_t i = 0; i < 8; ++i) o[i] = o[i] * keep + w * v[i];
+        m = top;
+    }
+    const float f = l == 0.0f ? 0.0f : p.v_scale / l;
+    for (uint32_t i = 0; i < 8; ++i)
+        if (lane + 32u * i < D) p.out[size_t(token) * p.out_row_stride + size_t(head) * D + lane + 32u * i] = f32_to_bf16_bits(l == 0.0f ? 0.0f : o[i] * f);
+}
+
+// Logarithm of a row's sum of exponentials from its M and L.
+__device__ __forceinline__ float attn_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) * ATTN_LN2; }
+
+// ------------------------------------------------------------------------------------------------------------------
+// Joins the pieces of items that were cut.  CTA c looks at the cut between ranges c and c + 1; the first cut of an item joins it.
+// A piece's slot: 2 c for the item that range c begins inside, 2 c + 1 for one that begins in range c and goes on.
+// ------------------------------------------------------------------------------------------------------------------
+constexpr int ATTN_JOIN_THREADS = 256;
+
+template <int ROWS, int KEYS, int DP, bool FP8>
+__global__ void __launch_bounds__(ATTN_JOIN_THREADS) attn_join_kernel(const __grid_constant__ AttnParams p) {
+    __shared__ uint64_t sh[ATTN_JOIN_THREADS / 32 + 3];
+    // the lengths are read ahead of the wait: the kernel in front has waited for everything before it
+    const uint32_t c = blockIdx.x + 1;
+    const AttnFound f = attn_find<ATTN_JOIN_THREADS>(p, ROWS, KEYS, sh, [&](uint64_t total) {
+        const uint32_t n = attn_ranges(total, p.ctas, p.least_tiles);
+        return c < n ? attn_range_begin(total, n, c) : ~0ull;
+    });
+    pdl_wait();
+    const uint32_t n = attn_ranges(f.total, p.ctas, p.least_tiles);
+    if (c >= n) return;
+    const uint64_t cut = attn_range_begin(f.total, n, c);
+    const AttnSeqAt sq = attn_seq(p, f.seq);
+    const AttnSeq seq(sq.q_len, sq.kv_len, p.group, ROWS, KEYS);
+    const AttnPlace at = attn_locate(seq, p.kv_heads, cut - f.seq_begin);
+    const uint64_t begin = cut - at.tile, end = begin + at.tiles;
+    if (at.tile == 0 || (c > 1 && attn_range_begin(f.total, n, c - 1) > begin)) return;   // not inside an item, or not its first cut
+    const uint32_t last = attn_range_of(f.total, n, end - 1);
+    const uint32_t rows = min(uint32_t(ROWS), sq.q_len * p.group - at.block * ROWS);
+    const size_t part = attn_part_floats(ROWS, DP);
+    auto slot = [&](uint32_t r) { return p.parts + part * (r == c - 1 ? 2 * size_t(r) + 1 : 2 * size_t(r)); };
+    // a warp takes a row at a time; lane l holds elements l, l + 32, ...
+    const uint32_t lane = threadIdx.x & 31u;
+    for (uint32_t r = threadIdx.x >> 5; r < rows; r += ATTN_JOIN_THREADS / 32) {
+        float m = -INFINITY;
+        for (uint32_t i = c - 1 + lane; i <= last; i += 32) m = fmaxf(m, slot(i)[size_t(ROWS) * DP + r]);
+        for (uint32_t x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
+        const float base = m == -INFINITY ? 0.0f : m;
+        float o[DP / 32] = {}, l = 0.0f;
+#pragma unroll 4
+        for (uint32_t i = c - 1; i <= last; ++i) {
+            const float* s = slot(i);
+            const float w = exp2f(s[size_t(ROWS) * DP + r] - base);
+            l += w * s[size_t(ROWS) * DP + ROWS + r];
+#pragma unroll
+            for (uint32_t k = 0; k < DP / 32; ++k) o[k] += w * s[size_t(r) * DP + lane + 32 * k];
+        }
+        const uint32_t row = at.block * ROWS + r, in_seq = row / p.group, token = sq.row0 + in_seq, head = at.head * p.group + row % p.group;
+        const float inv = l == 0.0f ? 0.0f : p.v_scale / l;
+        bool odd = false;
+#pragma unroll
+        for (uint32_t k = 0; k < DP / 32; ++k) {
+            const float y = l == 0.0f ? 0.0f : o[k] * inv;
+            if (lane + 32 * k < p.head_dim) {
+                p.out[size_t(token) * p.out_row_stride + size_t(head) * p.head_dim + lane + 32 * k] = f32_to_bf16_bits(y);
+                odd |= !isfinite(y);
+            }
+        }
+        if (p.lse && lane == 0) p.lse[size_t(token) * p.q_heads + head] = attn_lse(m, l);
+        if (__any_sync(0xFFFFFFFFu, odd) && sq.q_len > 1)
+            attn_row_again(p, FP8, f.seq, token, head, attn_row_keys(sq, in_seq));
+    }
+}
+
+}  // namespace atlas

@@ -242,12 +242,18 @@ struct QkvEpilogueParams {
     uint32_t tokens, q_heads, kv_heads, head_dim, rotary_dim, block_size, q_row_stride, kv_row_stride;
     float rms_eps, attention_factor;
     uint32_t norm_offset_one;
+    float k_inv_scale, v_inv_scale;   // E4M3 caches (k_cache, v_cache: one byte per element): value * inv_scale, saturating cast
 };
+
+__device__ __forceinline__ uint32_t e4m3_pair(const float lo, const float hi, const float inv_scale) {
+    return uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(lo, inv_scale), __fmul_rn(hi, inv_scale)), __NV_SATFINITE, __NV_E4M3));
+}
 
 // MAX_GRP: head_dim / 64 rounded up to 1, 2 or 4.  EXACT: head_dim = 64 MAX_GRP and rotary_dim = 64 (the common shapes),
 // known when the kernel is compiled, so that no lane is masked, a pair's halves meet by one shuffle and the general
-// form with its shared-memory strip drops out.
-template <uint32_t MAX_GRP, bool EXACT>
+// form with its shared-memory strip drops out.  FP8: the caches are E4M3; a rotated K value goes to its code in one rounding
+// (the normed head is rounded to BF16 before the rotation either way, as Q's is).
+template <uint32_t MAX_GRP, bool EXACT, bool FP8 = false>
 __global__ void __launch_bounds__(KVE_WARPS * 32, MAX_GRP == 4 ? 4 : 6)     // (occupancy matters more here than a few held values)
 qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
     pdl_release();
@@ -291,8 +297,9 @@ qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
         for (uint32_t g = 0; g < MAX_GRP; ++g)
             rw[g] = ((have >> g) & 1u) ? *reinterpret_cast<const uint32_t*>(x + 64u * g + 2u * lane) : 0u;
     };
-    // per-head RMS norm, rotation and one rounding of the head held as packed pairs in rw; result to dst
-    auto norm_rope_head = [&](const uint32_t (&rw)[MAX_GRP], const uint16_t* w, uint16_t* dst) {
+    // per-head RMS norm, rotation and one rounding of the head held as packed pairs in rw; result to dst (BF16, or E4M3 codes)
+    auto norm_rope_head = [&](const uint32_t (&rw)[MAX_GRP], const uint16_t* w, auto* dst) {
+        constexpr bool CODES = sizeof(*dst) == 1;
         float x0v[MAX_GRP], x1v[MAX_GRP], sq[MAX_GRP];
 #pragma unroll
         for (uint32_t g = 0; g < MAX_GRP; ++g) {                           // (a group the head does not have was loaded as zero)
@@ -322,9 +329,13 @@ qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
                     const float b0 = __uint_as_float(second << 16), b1 = __uint_as_float(second & 0xFFFF0000u);
                     const float r0 = low ? __fsub_rn(__fmul_rn(a0, c0), __fmul_rn(b0, s0)) : __fadd_rn(__fmul_rn(b0, c0), __fmul_rn(a0, s0));
                     const float r1 = low ? __fsub_rn(__fmul_rn(a1, c1), __fmul_rn(b1, s1)) : __fadd_rn(__fmul_rn(b1, c1), __fmul_rn(a1, s1));
-                    out = pack_bf16x2(r0, r1);
+                    if constexpr (CODES) out = e4m3_pair(r0, r1, p.k_inv_scale);
+                    else out = pack_bf16x2(r0, r1);
+                } else if constexpr (CODES) {
+                    out = e4m3_pair(bf16_lo(own), bf16_hi(own), p.k_inv_scale);
                 }
-                *reinterpret_cast<uint32_t*>(dst + e) = out;
+                if constexpr (CODES) *reinterpret_cast<uint16_t*>(dst + e) = uint16_t(out);
+                else *reinterpret_cast<uint32_t*>(dst + e) = out;
             }
             return;
         }
@@ -346,10 +357,19 @@ qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
                 const float a = __uint_as_float(uint32_t(normed_s[warp][t]) << 16);
                 const float b = __uint_as_float(uint32_t(normed_s[warp][t + pairs]) << 16);
                 const float c = cos_s[t], s = sin_s[t];
-                dst[t] = f32_to_bf16_bits(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)));
-                dst[t + pairs] = f32_to_bf16_bits(__fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s)));
+                const float r0 = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)), r1 = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+                if constexpr (CODES) {
+                    const uint32_t codes = e4m3_pair(r0, r1, p.k_inv_scale);
+                    dst[t] = uint8_t(codes);
+                    dst[t + pairs] = uint8_t(codes >> 8);
+                } else {
+                    dst[t] = f32_to_bf16_bits(r0);
+                    dst[t + pairs] = f32_to_bf16_bits(r1);
+                }
             } else if (t >= p.rotary_dim) {
-                dst[t] = normed_s[warp][t];                                // channels beyond the rotary part pass through
+                // channels beyond the rotary part pass through
+                if constexpr (CODES) dst[t] = uint8_t(e4m3_pair(__uint_as_float(uint32_t(normed_s[warp][t]) << 16), 0.0f, p.k_inv_scale));
+                else dst[t] = normed_s[warp][t];
             }
         }
     };
@@ -388,7 +408,14 @@ qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
             const uint32_t item = i0 + r * KVE_WARPS;
             if (item >= 2u * p.kv_heads) continue;
             if (item < p.kv_heads) {
-                norm_rope_head(raw[r], p.k_norm_w, p.k_cache + cache_at + item * p.head_dim);
+                if constexpr (FP8) norm_rope_head(raw[r], p.k_norm_w, reinterpret_cast<uint8_t*>(p.k_cache) + cache_at + item * p.head_dim);
+                else norm_rope_head(raw[r], p.k_norm_w, p.k_cache + cache_at + item * p.head_dim);
+            } else if constexpr (FP8) {
+                uint8_t* dst = reinterpret_cast<uint8_t*>(p.v_cache) + cache_at + (item - p.kv_heads) * p.head_dim;
+#pragma unroll
+                for (uint32_t g = 0; g < MAX_GRP; ++g)
+                    if ((have >> g) & 1u)
+                        *reinterpret_cast<uint16_t*>(dst + 64u * g + 2u * lane) = uint16_t(e4m3_pair(bf16_lo(raw[r][g]), bf16_hi(raw[r][g]), p.v_inv_scale));
             } else {
                 uint16_t* dst = p.v_cache + cache_at + (item - p.kv_heads) * p.head_dim;
 #pragma unroll

@@ -309,7 +309,7 @@ __device__ __forceinline__ void fence_barrier_init();
 // raise the abort flag; warp 1 waits on the same barrier and must leave through the flag (or its own limit).  The kernel
 // then returns normally: no trap, the context stays usable.  out[0] = 1 if warp 0's wait returned false, out[1] the same
 // for warp 1, out[2] = nanoseconds warp 0 waited.
-__global__ void bounded_wait_selftest_kernel(uint64_t limit_ns, uint32_t code, uint32_t* out) {
+static __global__ void bounded_wait_selftest_kernel(uint64_t limit_ns, uint32_t code, uint32_t* out) {
     __shared__ uint64_t bar;
     __shared__ uint32_t abort_s;
     const uint32_t b = smem_u32(&bar);

@@ -185,6 +185,18 @@ ATLAS_B200_API int atlas_b200_qkv_norm_rope_cache_write(void* q, const void* k_i
                                          uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rotary_dim,
                                          uint32_t block_size, float rms_eps, float attention_factor, int norm_offset_one, void* stream);
 
+/* The same into E4M3 paged caches, K and V side, one byte per element: K after the rotation (which works on the normed head rounded
+ * to BF16, as above) and V as they are, value * inv_scale cast with saturation, one rounding.  No counterpart in the reference, whose
+ * FP8 writer has the K side of a prefill only.  What a code stands for is code / inv_scale: the k_scale and v_scale of the attention
+ * that reads the caches are 1 / k_inv_scale and 1 / v_inv_scale.  Both positive and finite (-1); k_cache 2-byte, v_cache 4-byte
+ * aligned (-3). */
+ATLAS_B200_API int atlas_b200_qkv_norm_rope_cache_write_fp8(void* q, const void* k_in, const void* v_in, uint32_t q_row_stride, uint32_t kv_row_stride,
+                                             const void* q_norm_weight, const void* k_norm_weight, const uint32_t* positions,
+                                             const float* inv_freq, const long long* slot_mapping, void* k_cache_fp8, void* v_cache_fp8,
+                                             uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rotary_dim,
+                                             uint32_t block_size, float rms_eps, float attention_factor, int norm_offset_one,
+                                             float k_inv_scale, float v_inv_scale, void* stream);
+
 /* First phase of the weight quantiser: *global_max (a device float the caller has zeroed) becomes max |in| over `total`
  * BF16 elements.  Replaces `nvfp4_global_absmax` (kernels/gb10/common/quantize_bf16_to_nvfp4.cu:131-167). */
 ATLAS_B200_API int atlas_b200_nvfp4_global_absmax(const void* in_bf16, float* global_max_dev, size_t total, void* stream);
@@ -468,6 +480,96 @@ ATLAS_B200_API uint64_t atlas_b200_registry_adapter_id_for_slot(const atlas_b200
 ATLAS_B200_API int32_t atlas_b200_registry_select_victim(const atlas_b200_registry* reg);
 
 /* ---------------------------------------------------------------------------------------
+ * Attention over the paged K/V cache, for a batch of sequences that each have a chunk of new tokens (one while a sequence decodes,
+ * a few while drafts are verified, many while its prompt is read).  The chunk's keys and values stand in the cache already (the
+ * *_cache_write calls above put them there).  For new token i of a sequence with n cached and c new tokens, and query head h:
+ *     o[i,h] = sum_j p_j v[j, h / group],   p = softmax over j <= n - c + i of  softmax_scale * q[i,h] . k[j, h / group]
+ * with group = q_heads / kv_heads.  A token that sees no key (c > n) gives zeros, and -inf in lse.  Scores, the softmax's maximum and
+ * sum and the outputs' sums are FP32; p is rounded to BF16 (FP16 over an E4M3 cache) for its product with v; o is rounded once.
+ *   q, out       [n_tokens, q_heads * head_dim] BF16, row strides in elements; q may be a column range of a fused QKV buffer;
+ *                they must not overlap
+ *   lse          [n_tokens, q_heads] f32 or NULL: natural logarithm of the sum of the exponentials
+ *   k_cache, v_cache   [n_pages, block_size, kv_heads, head_dim], BF16 or E4M3 (cache_dtype); an E4M3 code stands for code * k_scale
+ *                or code * v_scale (both 1 with BF16)
+ *   block_table  [n_seqs, table_stride] i32: page of tokens block_size * c ..; entries behind the last page are not read
+ *   cu_q         [n_seqs + 1] i32: rows cu_q[s] .. cu_q[s+1] - 1 of q and out are sequence s's new tokens (none: the sequence is
+ *                skipped); rows behind cu_q[n_seqs] are left as they are, so a padded batch may be captured
+ *   kv_len       [n_seqs] i32: cached tokens, the new ones among them
+ *   n_tokens     rows of q and out;  max_q_len, max_kv_len: no sequence has more (launch shapes go by them; more is computed all the
+ *                same, only slower)
+ *   ws           scratch of atlas_b200_paged_attention_ws_bytes(desc) bytes, 16-byte aligned, holding nothing between calls: calls
+ *                that may overlap on the GPU need one each.  NULL: no sequence's cache is split over several SMs, which is slow where
+ *                there are few sequences.
+ * head_dim a multiple of 32 up to 256, any group and block_size; scales positive and finite (-1).  n_pages * block_size and
+ * table_stride * block_size below 2^31 (-5).  Caches 16-byte aligned, q 4-byte with an even stride (-3).  A block table entry outside
+ * the pool reads as zeros and is recorded in the device status word (4), so is a kv_len beyond the table's row (5; what fits is
+ * taken).  The same call gives the same bits; other sequences of the batch move the cuts of a sequence's keys, and with them the
+ * order of its sums. */
+#define ATLAS_B200_CACHE_BF16 0u
+#define ATLAS_B200_CACHE_E4M3 1u
+typedef struct atlas_b200_attention_desc {
+    const void* q;
+    void* out;
+    float* lse;
+    const void* k_cache;
+    const void* v_cache;
+    const int32_t* block_table;
+    const int32_t* cu_q;
+    const int32_t* kv_len;
+    void* ws;
+    size_t ws_bytes;
+    uint32_t n_seqs, n_tokens, max_q_len, max_kv_len;
+    uint32_t n_pages, block_size, table_stride, cache_dtype;
+    uint32_t q_heads, kv_heads, head_dim, q_row_stride;
+    uint32_t out_row_stride;
+    float softmax_scale, k_scale, v_scale;
+} atlas_b200_attention_desc;
+
+ATLAS_B200_API int atlas_b200_paged_attention(const atlas_b200_attention_desc* desc, void* stream);
+/* Scratch for this descriptor (its pointers are not looked at) on the current device. */
+ATLAS_B200_API size_t atlas_b200_paged_attention_ws_bytes(const atlas_b200_attention_desc* desc);
+
+/* ---------------------------------------------------------------------------------------
+ * Pages of the cache between two steps.  All state is on the device, so that a captured step can take and give back pages:
+ *   bases        [n_bases] u64 device addresses: K and V caches of every layer, each [n_pages][page_bytes], 16-byte aligned
+ *   refcount     [n_pages] i32: sequences that hold the page; 0 = free
+ *   block_table  [n_seqs, table_stride] i32; a sequence of n tokens holds the first ceil(n / block_size) entries of its row
+ *   seq_len      [n_seqs] i32
+ *   ws           scratch of atlas_b200_cache_ws_bytes(desc, n) bytes for a call of n entries (0: cache_compact); like the attention's
+ * A part-filled page belongs to one sequence alone: cache_fork copies it, so appending never writes where another sequence reads.
+ * Taken is always the lowest free page, in the order of the call's entries.  Arrays named below are on the device, i32 where nothing is said.
+ * status[i] (status may be NULL) is 0, -1 (no such sequence, the same one named by an earlier entry, or one in no state for it) or -5
+ * (no pages, no room in the table's row or in slot_mapping); an entry that fails changes nothing.  Pages are dealt out before it is
+ * known who goes without: where entry i fails for want of pages, a later one that needs any fails too.
+ *
+ * cache_append: n_new[i] more tokens for sequence seqs[i].  slot_mapping (i64, [max_tokens]) gets the cache slots (page * block_size +
+ *   offset) of all entries' new tokens one after the other, as the writers take them: -1 for those of an entry that failed and behind the last.
+ * cache_fork: sequence dst[i], empty, becomes a copy of src[i] as it was before the call: full pages are shared, a part-filled one is
+ *   copied into a page of its own, the tokens it holds and no more.
+ * cache_free: the sequences give back their pages; their rows become -1 and their lengths 0.  A sequence named twice is freed once.
+ * cache_compact: with U pages in use, the k-th one in use behind the first U moves to the k-th free one among them.  Results into
+ *   refcount_out and block_table_out (may be refcount and block_table), page_map [n_pages] (where a page went, -1 if it was free) and
+ *   *n_used = U.  Contents of pages U .. are left as they are. */
+typedef struct atlas_b200_cache_desc {
+    const uint64_t* bases;
+    int32_t* refcount;
+    int32_t* block_table;
+    int32_t* seq_len;
+    void* ws;
+    size_t ws_bytes;
+    size_t page_bytes;            /* a multiple of 16 and of block_size */
+    uint32_t n_bases, n_pages, block_size, table_stride, n_seqs, reserved0;
+} atlas_b200_cache_desc;
+
+ATLAS_B200_API size_t atlas_b200_cache_ws_bytes(const atlas_b200_cache_desc* desc, uint32_t n);
+ATLAS_B200_API int atlas_b200_cache_append(const atlas_b200_cache_desc* desc, const int32_t* seqs, const int32_t* n_new, uint32_t n, uint32_t max_tokens,
+                            long long* slot_mapping, int32_t* status, void* stream);
+ATLAS_B200_API int atlas_b200_cache_fork(const atlas_b200_cache_desc* desc, const int32_t* src, const int32_t* dst, uint32_t n, int32_t* status, void* stream);
+ATLAS_B200_API int atlas_b200_cache_free(const atlas_b200_cache_desc* desc, const int32_t* seqs, uint32_t n, void* stream);
+ATLAS_B200_API int atlas_b200_cache_compact(const atlas_b200_cache_desc* desc, int32_t* refcount_out, int32_t* block_table_out, int32_t* page_map,
+                             int32_t* n_used, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Diagnostics.
  */
 /* Device status word: 0 = clean; otherwise the first problem a kernel recorded (out-of-range
@@ -496,6 +598,9 @@ ATLAS_B200_API int atlas_b200_last_persistent_shape(uint32_t out[2]);
 /* More of it: out[0] = 1 if the call's MMAs left gaps for the shrink that ran beside it, out[1] = 1 if the kernel for the smallest
  * batches had its weights brought by TMA. */
 ATLAS_B200_API int atlas_b200_last_launch_details(uint32_t out[2]);
+/* The attention launched last on this thread: out[0] = rows of a block (16: the mma.sync form), out[1] = CTAs, out[2] = 1 if every CTA
+ * took whole items, out[3] = keys of a tile. */
+ATLAS_B200_API int atlas_b200_last_attention_shape(uint32_t out[4]);
 /* Per-CTA cycle counters of the tcgen05 kernel, the counterpart of the reference's per-phase timers
  * (crates/spark-model/src/layers/qwen3_attention/trait_impl/multi_seq/mod.rs:125-141).  While a device
  * buffer of `n_words` u64 is set (16 words per CTA, CTA index = blockIdx.y * gridDim.x + blockIdx.x) each

@@ -1,0 +1,100 @@
+"""How the attention over the paged cache is cut into pieces (csrc/attn_plan.hpp), compiled for the host, against counting."""
+import ctypes as C
+import os
+import random
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "apathy-atlas_b200", "csrc")
+
+SOURCE = """
+#include "attn_plan.hpp"
+using namespace atlas;
+extern "C" {
+uint64_t floor_sum_(uint64_t n, uint64_t m, uint64_t a, uint64_t b) { return floor_sum(n, m, a, b); }
+uint32_t tiles(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k, uint32_t b) { return AttnSeq(q, kv, g, r, k).tiles(b); }
+uint32_t blocks(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k) { return AttnSeq(q, kv, g, r, k).blocks; }
+uint64_t total(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k, uint32_t h) { return AttnSeq(q, kv, g, r, k).total(h); }
+void locate(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k, uint32_t h, uint64_t x, uint32_t* out) {
+    const AttnPlace p = attn_locate(AttnSeq(q, kv, g, r, k), h, x);
+    out[0] = p.block; out[1] = p.head; out[2] = p.tile; out[3] = p.tiles;
+}
+uint64_t range_begin(uint64_t t, uint32_t n, uint32_t c) { return attn_range_begin(t, n, c); }
+uint32_t range_of(uint64_t t, uint32_t n, uint64_t x) { return attn_range_of(t, n, x); }
+uint32_t ranges(uint64_t t, uint32_t ctas, uint32_t least) { return attn_ranges(t, ctas, least); }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    d = tmp_path_factory.mktemp("plan")
+    (d / "plan.cpp").write_text(SOURCE)
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Wextra", "-Werror", "-shared", "-fPIC", f"-I{CSRC}", "-o", str(d / "plan.so"), str(d / "plan.cpp")],
+                   check=True)
+    L = C.CDLL(str(d / "plan.so"))
+    u32, u64 = C.c_uint32, C.c_uint64
+    L.floor_sum_.argtypes, L.floor_sum_.restype = [u64] * 4, u64
+    L.total.argtypes, L.total.restype = [u32] * 6, u64
+    L.locate.argtypes = [u32] * 6 + [u64, C.POINTER(u32)]
+    L.range_begin.argtypes, L.range_begin.restype = [u64, u32, u32], u64
+    L.range_of.argtypes, L.range_of.restype = [u64, u32, u64], u32
+    L.ranges.argtypes, L.ranges.restype = [u64, u32, u32], u32
+    return L
+
+
+def test_floor_sum(plan):
+    rng = random.Random(1)
+    for _ in range(300):
+        n, m, a, b = rng.randint(0, 60), rng.randint(1, 40), rng.randint(0, 90), rng.randint(0, 500)
+        assert plan.floor_sum_(n, m, a, b) == sum((a * i + b) // m for i in range(n))
+
+
+def _counted(q, kv, g, rows, keys):
+    """Tiles of every block of rows, by looking at what its last row sees."""
+    n = -(-q * g // rows)
+    out = []
+    for b in range(n):
+        last = min(q - 1, ((b + 1) * rows - 1) // g)
+        seen = kv if kv < q else kv - q + last + 1
+        out.append(max(1, -(-seen // keys)))
+    return out
+
+
+@pytest.mark.parametrize("rows,keys", [(16, 64), (16, 128), (128, 128), (256, 128)])
+def test_blocks_and_places(plan, rows, keys):
+    rng = random.Random(rows + keys)
+    out = (C.c_uint32 * 4)()
+    for _ in range(150):
+        g, h = rng.choice((1, 2, 3, 4, 5, 7, 8, 16, 40)), rng.choice((1, 2, 5))
+        q = rng.choice((1, 1, 2, rng.randint(1, 40), rng.randint(1, 700)))
+        kv = rng.choice((q, q + rng.randint(0, 400), rng.randint(0, q), q + 64, q + 127))
+        tiles = _counted(q, kv, g, rows, keys)
+        assert plan.blocks(q, kv, g, rows, keys) == len(tiles)
+        assert [plan.tiles(q, kv, g, rows, keys, b) for b in range(len(tiles))] == tiles
+        assert plan.total(q, kv, g, rows, keys, h) == h * sum(tiles)
+        x = 0
+        for b, t in enumerate(tiles):
+            for head in range(h):
+                for tile in {0, t // 2, t - 1}:
+                    plan.locate(q, kv, g, rows, keys, h, x + tile, out)
+                    assert tuple(out) == (b, head, tile, t)
+                x += t
+    assert plan.blocks(0, 77, 4, rows, keys) == 0 and plan.total(0, 77, 4, rows, keys, 8) == 0
+
+
+def test_ranges_cover_the_line(plan):
+    rng = random.Random(3)
+    for _ in range(100):
+        total, ctas, least = rng.randint(1, 3000), rng.randint(1, 400), rng.randint(1, 9)
+        n = plan.ranges(total, ctas, least)
+        assert 1 <= n <= ctas and (n == 1 or (n - 1) * least < total)
+        begins = [plan.range_begin(total, n, c) for c in range(n + 1)]
+        assert begins[0] == 0 and begins[-1] == total
+        sizes = [b - a for a, b in zip(begins, begins[1:])]
+        assert max(sizes) - min(sizes) <= 1 and min(sizes) >= 1
+        for c in range(n):
+            assert plan.range_of(total, n, begins[c]) == c and plan.range_of(total, n, begins[c + 1] - 1) == c
+    assert plan.ranges(0, 148, 4) == 1
+    assert plan.range_begin(1 << 45, 148, 147) == (1 << 45) // 148 * 147 + min(147, (1 << 45) % 148)
