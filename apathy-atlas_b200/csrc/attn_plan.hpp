@@ -84,6 +84,16 @@ ATLAS_HD inline AttnPlace attn_locate(const AttnSeq& s, uint32_t kv_heads, uint6
     return p;
 }
 
+// The next item of a sequence's part of the line; false behind the last.
+ATLAS_HD inline bool attn_next(const AttnSeq& s, uint32_t kv_heads, AttnPlace& p) {
+    p.tile = 0;
+    if (++p.head < kv_heads) return true;
+    p.head = 0;
+    if (++p.block >= s.blocks) return false;
+    p.tiles = s.tiles(p.block);
+    return true;
+}
+
 // Range c of `ranges` over a line of `total` places begins here; range_of: the one that place x belongs to.
 ATLAS_HD inline uint64_t attn_range_begin(uint64_t total, uint32_t ranges, uint32_t c) {
     const uint64_t each = total / ranges, more = total % ranges;                          // the first `more` are one longer

@@ -14,6 +14,7 @@
 #include "host_launch.hpp"
 #include "kernel_attn.cuh"
 #include "kernel_attn_mma.cuh"
+#include "kernel_attn_tc.cuh"
 #include "kernel_cache_pages.cuh"
 
 namespace atlas {
@@ -137,12 +138,84 @@ template <int DP, bool FP8> int launch_mma(AttnParams p, const MmaPlan& plan, cu
     return launch_dependent(attn_join_kernel<attn::MMA_ROWS, attn::MMA_TILE, DP, FP8>, plan.ctas - 1, ATTN_JOIN_THREADS, 0, st, p);
 }
 
+// The tcgen05 form.  It reads pages in boxes of the largest power of two that divides page and tile, at least a swizzle atom's eight rows,
+// and Q and the outputs in sixteen bytes.
+struct TcPlan {
+    uint32_t ctas, by_item, least, box_rows;
+    size_t ws_bytes;
+};
+uint32_t tc_box_rows(uint32_t block_size) {
+    uint32_t r = attn::TC_KEYS;
+    while (block_size % r) r /= 2;
+    return r;
+}
+bool takes_tc(const atlas_b200_attention_desc& d) {
+    const uint64_t rows = uint64_t(std::min(d.max_q_len, d.n_tokens)) * (d.q_heads / d.kv_heads);
+    return rows > 32 && tc_box_rows(d.block_size) >= 8 && aligned(d.q, 16) && aligned(d.out, 16) && d.q_row_stride % 8 == 0 && d.out_row_stride % 8 == 0;
+}
+TcPlan plan_tc(const atlas_b200_attention_desc& d, uint32_t sms) {
+    const uint32_t dim = attn_dim(d.head_dim), block_rows = dim <= 128 ? 256u : 128u;
+    const uint64_t rows = uint64_t(std::min(d.max_q_len, d.n_tokens)) * (d.q_heads / d.kv_heads);
+    const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * ((rows + block_rows - 1) / block_rows);
+    const uint64_t tiles = std::max<uint64_t>((uint64_t(d.max_kv_len) + attn::TC_KEYS - 1) / attn::TC_KEYS, 1);
+    TcPlan r{};
+    r.box_rows = tc_box_rows(d.block_size);
+    r.by_item = tiles <= 2;
+    r.least = r.by_item ? 1u : 2u;
+    const uint64_t places = r.by_item ? items : (items * tiles + r.least - 1) / r.least;
+    r.ctas = uint32_t(std::min<uint64_t>(sms, std::max<uint64_t>(places, 1)));
+    r.ws_bytes = r.by_item ? 0 : size_t(sms) * 2 * attn_part_floats(block_rows, dim) * sizeof(float);
+    return r;
+}
+
+template <int DP, bool FP8> int launch_tc(AttnParams p, const TcPlan& plan, cudaStream_t st) {
+    using C = attn::TcCfg<DP, FP8>;
+    static std::atomic<bool> done[kMaxDevices] = {};
+    const int rc = allow_smem(attn::attn_tc_kernel<DP, FP8>, C::SMEM, done);
+    if (rc) return rc;
+    if (C::SOFT_REGS > C::LAUNCH_REGS) {
+        // the split of registers draws on what the block was launched with: a kernel built with fewer would wait for them forever
+        static std::atomic<int> built{0};
+        if (built.load(std::memory_order_relaxed) == 0) {
+            cudaFuncAttributes a{};
+            const cudaError_t e = cudaFuncGetAttributes(&a, attn::attn_tc_kernel<DP, FP8>);
+            if (e != cudaSuccess) return cuda_status(e);
+            built.store(a.numRegs, std::memory_order_relaxed);
+        }
+        if (built.load(std::memory_order_relaxed) < C::LAUNCH_REGS) return ATLAS_B200_ERR_LIMIT;
+    }
+    CUtensorMap map_k, map_v;
+    const uint64_t size = FP8 ? 1 : 2;
+    const uint64_t dims[3] = {p.head_dim, p.kv_heads, uint64_t(p.n_pages) * p.block_size};
+    const uint64_t strides[2] = {p.head_dim * size, uint64_t(p.kv_heads) * p.head_dim * size};
+    const uint32_t box[3] = {FP8 ? uint32_t(DP) : 64u, 1u, plan.box_rows};
+    const CUtensorMapDataType dt = FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUtensorMapSwizzle swz = FP8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+    if (!encode_tensor_map(&map_k, dt, 3, p.k_cache, dims, strides, box, swz) || !encode_tensor_map(&map_v, dt, 3, p.v_cache, dims, strides, box, swz))
+        return ATLAS_B200_ERR_DIMS;
+    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item;
+    const int rc2 = launch_dependent(attn::attn_tc_kernel<DP, FP8>, plan.ctas, C::THREADS, C::SMEM, st, map_k, map_v, p, plan.box_rows);
+    if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
+    return launch_dependent(attn_join_kernel<C::ROWS, int(attn::TC_KEYS), DP, FP8>, plan.ctas - 1, ATTN_JOIN_THREADS, 0, st, p);
+}
+
 int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
     if (d.n_seqs == 0 || d.n_tokens == 0) return ATLAS_B200_OK;
     const int bad = check_attention(d);
     if (bad) return bad;
     if (!device_is_sm100()) return ATLAS_B200_ERR_ARCH;
     const uint32_t sms = uint32_t(device_sm_count()), dim = attn_dim(d.head_dim);
+    if (takes_tc(d)) {
+        TcPlan plan = plan_tc(d, sms);
+        if (d.ws ? d.ws_bytes < plan.ws_bytes : d.ws_bytes != 0) return ATLAS_B200_ERR_WORKSPACE;
+        if (!d.ws && !plan.by_item) { plan.by_item = 1; plan.least = 1; }
+        const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3;
+        const AttnParams p = attention_params(d);
+        t_attn_shape[0] = dim <= 128 ? 256 : 128; t_attn_shape[1] = plan.ctas; t_attn_shape[2] = plan.by_item; t_attn_shape[3] = attn::TC_KEYS;
+        if (dim == 64) return fp8 ? launch_tc<64, true>(p, plan, st) : launch_tc<64, false>(p, plan, st);
+        if (dim == 128) return fp8 ? launch_tc<128, true>(p, plan, st) : launch_tc<128, false>(p, plan, st);
+        return fp8 ? launch_tc<256, true>(p, plan, st) : launch_tc<256, false>(p, plan, st);
+    }
     MmaPlan plan = plan_mma(d, sms);
     if (d.ws ? d.ws_bytes < plan.ws_bytes : d.ws_bytes != 0) return ATLAS_B200_ERR_WORKSPACE;
     if (!d.ws && !plan.by_item) { plan.by_item = 1; plan.least = 1; }        // (no scratch: nothing is cut)
@@ -197,7 +270,9 @@ int atlas_b200_paged_attention(const atlas_b200_attention_desc* desc, void* stre
 
 size_t atlas_b200_paged_attention_ws_bytes(const atlas_b200_attention_desc* desc) {
     if (!desc || desc->kv_heads == 0 || desc->q_heads % desc->kv_heads || desc->n_seqs == 0 || desc->n_tokens == 0) return 0;
-    return plan_mma(*desc, uint32_t(device_sm_count())).ws_bytes;
+    // (which kernel runs also goes by the alignment of pointers that may not be set yet: enough for either)
+    const uint32_t sms = uint32_t(device_sm_count());
+    return std::max(plan_mma(*desc, sms).ws_bytes, plan_tc(*desc, sms).ws_bytes);
 }
 
 int atlas_b200_last_attention_shape(uint32_t out[4]) {

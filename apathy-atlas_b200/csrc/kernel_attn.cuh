@@ -125,6 +125,41 @@ __device__ __forceinline__ AttnFound attn_find(const AttnParams& p, uint32_t row
     return f;
 }
 
+// The items of one CTA's range, one after the other; every thread walks by itself.
+struct AttnWalk {
+    AttnSeqAt sq;
+    AttnPlace at;                 // of the item; its piece is tiles t0 .. t1 - 1
+    uint32_t seq, t0, t1, rows, keys;
+
+    __device__ __forceinline__ AttnWalk(const AttnParams& p, const AttnFound& f, uint64_t begin, uint64_t end, uint32_t block_rows, uint32_t tile_keys)
+        : seq(f.seq), rows(block_rows), keys(tile_keys), left_(end - begin), fresh_(true) {
+        if (!left_) return;
+        sq = attn_seq(p, seq);
+        const uint64_t x = begin - f.seq_begin;
+        if (p.by_item) { at.block = uint32_t(x / p.kv_heads); at.head = uint32_t(x % p.kv_heads); at.tile = 0; at.tiles = plan(p).tiles(at.block); }
+        else at = attn_locate(plan(p), p.kv_heads, x);
+    }
+    __device__ __forceinline__ AttnSeq plan(const AttnParams& p) const { return AttnSeq(sq.q_len, sq.kv_len, p.group, rows, keys); }
+    __device__ __forceinline__ bool next(const AttnParams& p) {
+        if (!left_) return false;
+        if (!fresh_ && !attn_next(plan(p), p.kv_heads, at)) {
+            do { ++seq; sq = attn_seq(p, seq); } while (sq.q_len == 0);      // (the range ends at a sequence that has places)
+            at.block = at.head = at.tile = 0;
+            at.tiles = plan(p).tiles(0);
+        }
+        fresh_ = false;
+        t0 = at.tile;
+        t1 = p.by_item || at.tiles - t0 <= left_ ? at.tiles : t0 + uint32_t(left_);
+        left_ -= p.by_item ? 1u : t1 - t0;
+        return true;
+    }
+    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == at.tiles; }
+
+private:
+    uint64_t left_;
+    bool fresh_;
+};
+
 // Row `pos` of a sequence in the cache seen as [pages * block_size, kv_heads, head_dim]; -1 and a record where the table names no page.
 __device__ __forceinline__ int32_t attn_cache_row(const AttnParams& p, const AttnDivisor& div, const int32_t* table, uint32_t pos) {
     const uint32_t page = attn_div(pos, div), id = uint32_t(table[page]);

@@ -84,18 +84,11 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
         if (blockIdx.x < n) { x = attn_range_begin(total, n, blockIdx.x); x_end = attn_range_begin(total, n, blockIdx.x + 1); }
         return x < x_end ? x : ~0ull;
     });
-    uint32_t seq = f.seq;
-    uint64_t in_seq = x - f.seq_begin;                                       // place within the sequence
-
-    while (x < x_end) {
-        const AttnSeqAt sq = attn_seq(p, seq);
-        const AttnSeq sp(sq.q_len, sq.kv_len, p.group, MMA_ROWS, MMA_TILE);
-        const uint64_t seq_places = p.by_item ? uint64_t(sp.blocks) * p.kv_heads : sp.total(p.kv_heads);
-        if (in_seq >= seq_places) { in_seq -= seq_places; ++seq; continue; }
-        AttnPlace at;
-        if (p.by_item) { at.block = uint32_t(in_seq / p.kv_heads); at.head = uint32_t(in_seq % p.kv_heads); at.tile = 0; at.tiles = sp.tiles(at.block); }
-        else at = attn_locate(sp, p.kv_heads, in_seq);
-        const uint32_t t0 = at.tile, t1 = p.by_item ? at.tiles : uint32_t(min(uint64_t(at.tiles), t0 + (x_end - x)));
+    AttnWalk walk(p, f, x, x_end, MMA_ROWS, MMA_TILE);
+    while (walk.next(p)) {
+        const AttnSeqAt sq = walk.sq;
+        const AttnPlace at = walk.at;
+        const uint32_t seq = walk.seq, t0 = walk.t0, t1 = walk.t1;
         const uint32_t rows_left = sq.q_len * p.group - at.block * MMA_ROWS, rows = min(rows_left, uint32_t(MMA_ROWS));
 
         // this lane's two rows: their tokens, heads and how many keys they see
@@ -306,7 +299,7 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
                 }
         }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == at.tiles;
+        const bool whole = walk.whole();
         float* part = whole ? nullptr : p.parts + attn_part_floats(MMA_ROWS, DP) * (2 * size_t(blockIdx.x) + (t0 == 0 ? 1 : 0));
         for (uint32_t r = warp; r < rows; r += MMA_WARPS) {                  // a warp takes whole rows
             float top = -INFINITY, w[MMA_WARPS], total = 0.0f;
@@ -343,10 +336,6 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
             if (__any_sync(0xFFFFFFFFu, odd) && sq.q_len > 1) attn_row_again(p, FP8, seq, sq.row0 + tok, head, attn_row_keys(sq, tok));
         }
         __syncthreads();                                                     // before the next item's copies land here
-        const uint32_t done = p.by_item ? 1u : t1 - t0;
-        x += done;
-        in_seq += done;
-
     }
 }
 
