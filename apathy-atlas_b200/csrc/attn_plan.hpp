@@ -4,7 +4,8 @@
 // token r / group, head r % group of them.  `block_rows` rows make a block; a block reads the keys its last row sees, in tiles of
 // `tile_keys`.  An item is one (sequence, block, KV head).  All items' tiles in a row (sequence, block, KV head, tile; the last fastest)
 // are the line that CTAs cut into contiguous ranges of equal length, whatever the sequences' lengths: a range may begin and end inside
-// an item, whose pieces are joined afterwards.
+// an item, whose pieces are joined afterwards.  What an item costs besides its tiles (fetching Q, writing the output) stands in the line
+// as `extra` places ahead of its first tile.  A cut among those is none: the item belongs to the range behind it.
 #pragma once
 
 #include <stddef.h>
@@ -41,8 +42,9 @@ ATLAS_HD inline uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t 
 // its blocks count as if they saw the whole cache.
 struct AttnSeq {
     uint32_t q_len, kv_len, blocks, whole;      // whole: tiles of the cached tokens, one at least
-    uint32_t group, block_rows, tile_keys;
-    ATLAS_HD AttnSeq(uint32_t q, uint32_t kv, uint32_t g, uint32_t rows, uint32_t keys) : q_len(q), kv_len(kv), group(g), block_rows(rows), tile_keys(keys) {
+    uint32_t group, block_rows, tile_keys, extra;
+    ATLAS_HD AttnSeq(uint32_t q, uint32_t kv, uint32_t g, uint32_t rows, uint32_t keys, uint32_t more)
+        : q_len(q), kv_len(kv), group(g), block_rows(rows), tile_keys(keys), extra(more) {
         blocks = uint32_t((uint64_t(q) * g + rows - 1) / rows);
         whole = kv ? (kv - 1) / keys + 1 : 1;
     }
@@ -53,19 +55,19 @@ struct AttnSeq {
         const uint64_t t = (uint64_t(block_rows) * b + block_rows - 1 + uint64_t(group) * keys_less_1) / (uint64_t(group) * tile_keys);
         return t < whole ? uint32_t(t) : whole;
     }
-    // tiles of the blocks before b
+    // places of the blocks before b, of one KV head
     ATLAS_HD uint64_t before(uint32_t b) const {
         if (b == 0 || blocks == 0) return 0;
         const uint32_t n = b < blocks ? b : blocks - 1;                                   // by the formula
         uint64_t sum = kv_len < q_len ? uint64_t(whole) * n
                                       : floor_sum(n, uint64_t(group) * tile_keys, block_rows, block_rows - 1 + uint64_t(group) * (uint64_t(kv_len - q_len) + tile_keys));
-        return b < blocks ? sum : sum + whole;
+        return (b < blocks ? sum : sum + whole) + uint64_t(b) * extra;
     }
     ATLAS_HD uint64_t total(uint32_t kv_heads) const { return before(blocks) * kv_heads; }
 };
 
 struct AttnPlace {
-    uint32_t block, head, tile, tiles;          // tile of the item, of `tiles`
+    uint32_t block, head, place, tiles;         // place within the item, which has extra + tiles of them
 };
 // where place x of a sequence's part of the line lies, x < total(kv_heads)
 ATLAS_HD inline AttnPlace attn_locate(const AttnSeq& s, uint32_t kv_heads, uint64_t x) {
@@ -79,14 +81,14 @@ ATLAS_HD inline AttnPlace attn_locate(const AttnSeq& s, uint32_t kv_heads, uint6
     p.block = lo;
     p.tiles = s.tiles(lo);
     const uint64_t in_block = x - s.before(lo) * kv_heads;
-    p.head = uint32_t(in_block / p.tiles);
-    p.tile = uint32_t(in_block % p.tiles);
+    p.head = uint32_t(in_block / (s.extra + p.tiles));
+    p.place = uint32_t(in_block % (s.extra + p.tiles));
     return p;
 }
 
 // The next item of a sequence's part of the line; false behind the last.
 ATLAS_HD inline bool attn_next(const AttnSeq& s, uint32_t kv_heads, AttnPlace& p) {
-    p.tile = 0;
+    p.place = 0;
     if (++p.head < kv_heads) return true;
     p.head = 0;
     if (++p.block >= s.blocks) return false;

@@ -106,6 +106,13 @@ AttnParams attention_params(const atlas_b200_attention_desc& d) {
     return p;
 }
 
+// What an item costs besides its tiles, in tiles of its kernel.
+#ifndef MMA_EXTRA_
+#define MMA_EXTRA_ 1
+#define TC_EXTRA_ 2
+#endif
+constexpr uint32_t MMA_EXTRA = MMA_EXTRA_, TC_EXTRA = TC_EXTRA_;
+
 // The mma.sync form: how many CTAs, and whether each takes whole items.
 struct MmaPlan {
     uint32_t ctas, by_item, least;
@@ -121,7 +128,7 @@ MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms) {
     MmaPlan r{};
     r.by_item = tiles <= 4;
     r.least = r.by_item ? 1u : 4u;
-    const uint64_t places = r.by_item ? items : (items * tiles + r.least - 1) / r.least;
+    const uint64_t places = r.by_item ? items : (items * (tiles + MMA_EXTRA) + r.least - 1) / r.least;
     r.ctas = uint32_t(std::min<uint64_t>(resident, std::max<uint64_t>(places, 1)));
     r.ws_bytes = r.by_item ? 0 : size_t(resident) * 2 * attn_part_floats(attn::MMA_ROWS, dim) * sizeof(float);
     return r;
@@ -132,7 +139,7 @@ template <int DP, bool FP8> int launch_mma(AttnParams p, const MmaPlan& plan, cu
     static std::atomic<bool> done[kMaxDevices] = {};
     const int rc = allow_smem(attn::attn_mma_kernel<DP, FP8>, C::SMEM, done);
     if (rc) return rc;
-    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item;
+    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.extra = MMA_EXTRA;
     const int rc2 = launch_dependent(attn::attn_mma_kernel<DP, FP8>, plan.ctas, attn::MMA_THREADS, C::SMEM, st, p, attn_divisor(p.block_size));
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
     return launch_dependent(attn_join_kernel<attn::MMA_ROWS, attn::MMA_TILE, DP, FP8>, plan.ctas - 1, ATTN_JOIN_THREADS, 0, st, p);
@@ -162,7 +169,7 @@ TcPlan plan_tc(const atlas_b200_attention_desc& d, uint32_t sms) {
     r.box_rows = tc_box_rows(d.block_size);
     r.by_item = tiles <= 2;
     r.least = r.by_item ? 1u : 2u;
-    const uint64_t places = r.by_item ? items : (items * tiles + r.least - 1) / r.least;
+    const uint64_t places = r.by_item ? items : (items * (tiles + TC_EXTRA) + r.least - 1) / r.least;
     r.ctas = uint32_t(std::min<uint64_t>(sms, std::max<uint64_t>(places, 1)));
     r.ws_bytes = r.by_item ? 0 : size_t(sms) * 2 * attn_part_floats(block_rows, dim) * sizeof(float);
     return r;
@@ -193,10 +200,10 @@ template <int DP, bool FP8> int launch_tc(AttnParams p, const TcPlan& plan, cuda
     const CUtensorMapSwizzle swz = FP8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
     if (!encode_tensor_map(&map_k, dt, 3, p.k_cache, dims, strides, box, swz) || !encode_tensor_map(&map_v, dt, 3, p.v_cache, dims, strides, box, swz))
         return ATLAS_B200_ERR_DIMS;
-    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item;
+    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.extra = TC_EXTRA;
     const int rc2 = launch_dependent(attn::attn_tc_kernel<DP, FP8>, plan.ctas, C::THREADS, C::SMEM, st, map_k, map_v, p, plan.box_rows);
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
-    return launch_dependent(attn_join_kernel<C::ROWS, int(attn::TC_KEYS), DP, FP8>, plan.ctas - 1, ATTN_JOIN_THREADS, 0, st, p);
+    return launch_dependent(attn_join_kernel<C::ROWS, int(attn::TC_KEYS), DP, FP8>, dim3(plan.ctas - 1, C::ROWS / ATTN_JOIN_ROWS), ATTN_JOIN_THREADS, 0, st, p);
 }
 
 int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {

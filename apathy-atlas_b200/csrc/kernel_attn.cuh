@@ -36,6 +36,7 @@ struct AttnParams {
     uint32_t n_seqs, n_tokens, n_pages, table_stride, q_heads, kv_heads, head_dim, block_size, group, q_row_stride, out_row_stride;
     uint32_t ctas, least_tiles;   // ranges: at most `ctas`, of `least_tiles` tiles each at least
     uint32_t by_item;             // every CTA takes whole items: no pieces
+    uint32_t extra;               // what an item costs besides its tiles, in tiles
     float scale, k_scale, v_scale;
 };
 
@@ -83,7 +84,7 @@ struct AttnFound {
 };
 __device__ __forceinline__ uint64_t attn_seq_places(const AttnParams& p, uint32_t s, uint32_t rows, uint32_t keys) {
     const AttnSeqAt q = attn_seq(p, s);
-    const AttnSeq a(q.q_len, q.kv_len, p.group, rows, keys);
+    const AttnSeq a(q.q_len, q.kv_len, p.group, rows, keys, p.extra);
     return p.by_item ? uint64_t(a.blocks) * p.kv_heads : a.total(p.kv_heads);
 }
 template <int THREADS, typename F>
@@ -136,22 +137,29 @@ struct AttnWalk {
         if (!left_) return;
         sq = attn_seq(p, seq);
         const uint64_t x = begin - f.seq_begin;
-        if (p.by_item) { at.block = uint32_t(x / p.kv_heads); at.head = uint32_t(x % p.kv_heads); at.tile = 0; at.tiles = plan(p).tiles(at.block); }
+        if (p.by_item) { at.block = uint32_t(x / p.kv_heads); at.head = uint32_t(x % p.kv_heads); at.place = 0; at.tiles = plan(p).tiles(at.block); }
         else at = attn_locate(plan(p), p.kv_heads, x);
     }
-    __device__ __forceinline__ AttnSeq plan(const AttnParams& p) const { return AttnSeq(sq.q_len, sq.kv_len, p.group, rows, keys); }
+    __device__ __forceinline__ AttnSeq plan(const AttnParams& p) const { return AttnSeq(sq.q_len, sq.kv_len, p.group, rows, keys, p.extra); }
     __device__ __forceinline__ bool next(const AttnParams& p) {
         if (!left_) return false;
         if (!fresh_ && !attn_next(plan(p), p.kv_heads, at)) {
             do { ++seq; sq = attn_seq(p, seq); } while (sq.q_len == 0);      // (the range ends at a sequence that has places)
-            at.block = at.head = at.tile = 0;
+            at.block = at.head = at.place = 0;
             at.tiles = plan(p).tiles(0);
         }
         fresh_ = false;
-        t0 = at.tile;
-        t1 = p.by_item || at.tiles - t0 <= left_ ? at.tiles : t0 + uint32_t(left_);
-        left_ -= p.by_item ? 1u : t1 - t0;
-        return true;
+        if (p.by_item) {
+            t0 = 0;
+            t1 = at.tiles;
+            --left_;
+            return true;
+        }
+        const uint32_t there = p.extra + at.tiles, end = there - at.place <= left_ ? there : at.place + uint32_t(left_);
+        left_ -= end - at.place;
+        t0 = at.place > p.extra ? at.place - p.extra : 0u;
+        t1 = end > p.extra ? end - p.extra : 0u;
+        return t1 != 0u;                                                     // (a range that ends ahead of an item's first tile)
     }
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == at.tiles; }
 
@@ -209,10 +217,11 @@ static __device__ __noinline__ void attn_row_again(const AttnParams& p, bool fp8
 __device__ __forceinline__ float attn_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) * ATTN_LN2; }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Joins the pieces of items that were cut.  CTA c looks at the cut between ranges c and c + 1; the first cut of an item joins it.
+// Joins the pieces of items that were cut.  CTA (c, y) looks at the cut between ranges c and c + 1; the first cut of an item joins it, each
+// y some of its rows.
 // A piece's slot: 2 c for the item that range c begins inside, 2 c + 1 for one that begins in range c and goes on.
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int ATTN_JOIN_THREADS = 256;
+constexpr int ATTN_JOIN_THREADS = 256, ATTN_JOIN_ROWS = 16;
 
 template <int ROWS, int KEYS, int DP, bool FP8>
 __global__ void __launch_bounds__(ATTN_JOIN_THREADS) attn_join_kernel(const __grid_constant__ AttnParams p) {
@@ -228,17 +237,17 @@ __global__ void __launch_bounds__(ATTN_JOIN_THREADS) attn_join_kernel(const __gr
     if (c >= n) return;
     const uint64_t cut = attn_range_begin(f.total, n, c);
     const AttnSeqAt sq = attn_seq(p, f.seq);
-    const AttnSeq seq(sq.q_len, sq.kv_len, p.group, ROWS, KEYS);
+    const AttnSeq seq(sq.q_len, sq.kv_len, p.group, ROWS, KEYS, p.extra);
     const AttnPlace at = attn_locate(seq, p.kv_heads, cut - f.seq_begin);
-    const uint64_t begin = cut - at.tile, end = begin + at.tiles;
-    if (at.tile == 0 || (c > 1 && attn_range_begin(f.total, n, c - 1) > begin)) return;   // not inside an item, or not its first cut
+    const uint64_t first_tile = cut - at.place + p.extra, end = first_tile + at.tiles;
+    if (cut <= first_tile || attn_range_begin(f.total, n, c - 1) > first_tile) return;    // not behind an item's first tile, or not its first such cut
     const uint32_t last = attn_range_of(f.total, n, end - 1);
     const uint32_t rows = min(uint32_t(ROWS), sq.q_len * p.group - at.block * ROWS);
     const size_t part = attn_part_floats(ROWS, DP);
     auto slot = [&](uint32_t r) { return p.parts + part * (r == c - 1 ? 2 * size_t(r) + 1 : 2 * size_t(r)); };
     // a warp takes a row at a time; lane l holds elements l, l + 32, ...
     const uint32_t lane = threadIdx.x & 31u;
-    for (uint32_t r = threadIdx.x >> 5; r < rows; r += ATTN_JOIN_THREADS / 32) {
+    for (uint32_t r = blockIdx.y * (ATTN_JOIN_THREADS / 32) + (threadIdx.x >> 5); r < rows; r += gridDim.y * (ATTN_JOIN_THREADS / 32)) {
         float m = -INFINITY;
         for (uint32_t i = c - 1 + lane; i <= last; i += 32) m = fmaxf(m, slot(i)[size_t(ROWS) * DP + r]);
         for (uint32_t x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));

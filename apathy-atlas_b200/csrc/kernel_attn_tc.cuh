@@ -296,6 +296,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     if (j + 1 < n && ++ks == uint32_t(ST)) { ks = 0; kph ^= 1u; }
                 }
             }
+        } else {
+            // ---- Q of the items ahead to L2, so that its rows' latency is that of L2 when their turn comes ----
+            const uint32_t t = (warp - 2) * 32u + lane;
+            while (walk.next(p)) {
+                const uint32_t row0 = walk.at.block * C::ROWS, rows = tile_rows(0) + (NQ == 2 ? tile_rows(NQ - 1) : 0u), lines = (p.head_dim * 2u + 127u) / 128u;
+                for (uint32_t i = t; i < rows * lines; i += 64u) {
+                    const uint32_t row = row0 + i / lines, tok = row / p.group;
+                    const uint16_t* at = p.q + size_t(walk.sq.row0 + tok) * p.q_row_stride + size_t(walk.at.head * p.group + row - tok * p.group) * p.head_dim + (i % lines) * 64u;
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+                }
+            }
         }
     } else if (warp < uint32_t(C::CONV_WARP0)) {
         // ---- softmax: a row a thread ----
@@ -305,6 +316,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const uint32_t q_tile = base + C::OFF_Q + g * C::TILE;
         float* const scale_s = reinterpret_cast<float*>(gen + C::OFF_SCALE) + g * TC_TILE_ROWS;
         const uint32_t D = p.head_dim;
+        const AttnDivisor group_div = attn_divisor(p.group);
         uint32_t s_ph = 0, pv_ph = 0;
         bool ok = true;
         while (ok && walk.next(p)) {
@@ -315,14 +327,18 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             if (n) {
                 // Q: this warp's 32 rows, sixteen bytes a lane
                 constexpr uint32_t CH = DP / 8;
-#pragma unroll 4
+                const uint16_t* const q_head = p.q + size_t(walk.sq.row0) * p.q_row_stride + size_t(walk.at.head) * p.group * D;
+                uint4 qv[CH];                                                // (all loads in flight: one latency)
+#pragma unroll
                 for (uint32_t i = 0; i < CH; ++i) {
-                    const uint32_t idx = i * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH, row = row0 + r;
-                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (r < rows && ch * 8u < D) {
-                        const uint32_t tok = row / p.group;
-                        v = *reinterpret_cast<const uint4*>(p.q + size_t(walk.sq.row0 + tok) * p.q_row_stride + size_t(walk.at.head * p.group + row - tok * p.group) * D + ch * 8u);
-                    }
+                    const uint32_t idx = i * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH, row = row0 + r, tok = attn_div(row, group_div);
+                    qv[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (r < rows && ch * 8u < D) qv[i] = *reinterpret_cast<const uint4*>(q_head + size_t(tok) * p.q_row_stride + (row - tok * p.group) * D + ch * 8u);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < CH; ++i) {
+                    const uint32_t idx = i * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH;
+                    uint4 v = qv[i];
                     if constexpr (FP8) {
                         uint32_t w[4] = {v.x, v.y, v.z, v.w}, top = 0;
 #pragma unroll
@@ -343,7 +359,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 mbar_arrive(Q_FULL + 8 * g);
                 if constexpr (FP8) c *= scale_s[row_in];
             }
-            const uint32_t row = row0 + row_in, tok = row / p.group, head = walk.at.head * p.group + row - tok * p.group;
+            const uint32_t row = row0 + row_in, tok = attn_div(row, group_div), head = walk.at.head * p.group + row - tok * p.group;
             const uint32_t keys = row_in < rows ? attn_row_keys(walk.sq, tok) : 0u, all_see = attn_row_keys(walk.sq, row0 / p.group);
             for (uint32_t j = 0; ok && j < n; ++j) {
                 ok = mbar_wait(S_FULL + 8 * g, s_ph, abort_flag, STATUS_WAIT_EXPIRED_EPILOGUE);
@@ -450,14 +466,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 if (p.lse && row_in < rows) p.lse[size_t(walk.sq.row0 + tok) * p.q_heads + head] = attn_lse(m, l);
                 __syncwarp();
                 constexpr uint32_t CH = DP / 8;
-#pragma unroll 4
+                uint16_t* const o_head = p.out + size_t(walk.sq.row0) * p.out_row_stride + size_t(walk.at.head) * p.group * D;
+#pragma unroll 8
                 for (uint32_t i = 0; i < CH; ++i) {
-                    const uint32_t idx = i * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH, rw = row0 + r;
+                    const uint32_t idx = i * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH, rw = row0 + r, t = attn_div(rw, group_div);
                     const uint4 v = lds128(q_tile + (ch >> 3) * C::PANEL + sw128_off(r, ch & 7u));
-                    if (r < rows && ch * 8u < D) {
-                        const uint32_t t = rw / p.group;
-                        *reinterpret_cast<uint4*>(p.out + size_t(walk.sq.row0 + t) * p.out_row_stride + size_t(walk.at.head * p.group + rw - t * p.group) * D + ch * 8u) = v;
-                    }
+                    if (r < rows && ch * 8u < D) *reinterpret_cast<uint4*>(o_head + size_t(t) * p.out_row_stride + (rw - t * p.group) * D + ch * 8u) = v;
                 }
                 __syncwarp();
                 uint32_t again = walk.sq.q_len > 1 ? __ballot_sync(0xFFFFFFFFu, odd && row_in < rows) : 0u;

@@ -13,12 +13,16 @@ SOURCE = """
 using namespace atlas;
 extern "C" {
 uint64_t floor_sum_(uint64_t n, uint64_t m, uint64_t a, uint64_t b) { return floor_sum(n, m, a, b); }
-uint32_t tiles(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k, uint32_t b) { return AttnSeq(q, kv, g, r, k).tiles(b); }
-uint32_t blocks(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k) { return AttnSeq(q, kv, g, r, k).blocks; }
-uint64_t total(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k, uint32_t h) { return AttnSeq(q, kv, g, r, k).total(h); }
-void locate(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k, uint32_t h, uint64_t x, uint32_t* out) {
-    const AttnPlace p = attn_locate(AttnSeq(q, kv, g, r, k), h, x);
-    out[0] = p.block; out[1] = p.head; out[2] = p.tile; out[3] = p.tiles;
+uint32_t tiles(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k, uint32_t e, uint32_t b) { return AttnSeq(q, kv, g, r, k, e).tiles(b); }
+uint32_t blocks(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k, uint32_t e) { return AttnSeq(q, kv, g, r, k, e).blocks; }
+uint64_t total(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k, uint32_t e, uint32_t h) { return AttnSeq(q, kv, g, r, k, e).total(h); }
+int locate(uint32_t q, uint32_t kv, uint32_t g, uint32_t r, uint32_t k, uint32_t e, uint32_t h, uint64_t x, uint32_t* out) {
+    const AttnSeq s(q, kv, g, r, k, e);
+    AttnPlace p = attn_locate(s, h, x);
+    out[0] = p.block; out[1] = p.head; out[2] = p.place; out[3] = p.tiles;
+    const int more = attn_next(s, h, p);
+    out[4] = p.block; out[5] = p.head; out[6] = p.place; out[7] = p.tiles;
+    return more;
 }
 uint64_t range_begin(uint64_t t, uint32_t n, uint32_t c) { return attn_range_begin(t, n, c); }
 uint32_t range_of(uint64_t t, uint32_t n, uint64_t x) { return attn_range_of(t, n, x); }
@@ -36,8 +40,8 @@ def plan(tmp_path_factory):
     L = C.CDLL(str(d / "plan.so"))
     u32, u64 = C.c_uint32, C.c_uint64
     L.floor_sum_.argtypes, L.floor_sum_.restype = [u64] * 4, u64
-    L.total.argtypes, L.total.restype = [u32] * 6, u64
-    L.locate.argtypes = [u32] * 6 + [u64, C.POINTER(u32)]
+    L.total.argtypes, L.total.restype = [u32] * 7, u64
+    L.locate.argtypes = [u32] * 7 + [u64, C.POINTER(u32)]
     L.range_begin.argtypes, L.range_begin.restype = [u64, u32, u32], u64
     L.range_of.argtypes, L.range_of.restype = [u64, u32, u64], u32
     L.ranges.argtypes, L.ranges.restype = [u64, u32, u32], u32
@@ -62,26 +66,28 @@ def _counted(q, kv, g, rows, keys):
     return out
 
 
-@pytest.mark.parametrize("rows,keys", [(16, 64), (16, 128), (128, 128), (256, 128)])
-def test_blocks_and_places(plan, rows, keys):
+@pytest.mark.parametrize("rows,keys,extra", [(16, 64, 1), (16, 128, 0), (128, 128, 2), (256, 128, 3)])
+def test_blocks_and_places(plan, rows, keys, extra):
     rng = random.Random(rows + keys)
-    out = (C.c_uint32 * 4)()
+    out = (C.c_uint32 * 8)()
     for _ in range(150):
         g, h = rng.choice((1, 2, 3, 4, 5, 7, 8, 16, 40)), rng.choice((1, 2, 5))
         q = rng.choice((1, 1, 2, rng.randint(1, 40), rng.randint(1, 700)))
         kv = rng.choice((q, q + rng.randint(0, 400), rng.randint(0, q), q + 64, q + 127))
-        tiles = _counted(q, kv, g, rows, keys)
-        assert plan.blocks(q, kv, g, rows, keys) == len(tiles)
-        assert [plan.tiles(q, kv, g, rows, keys, b) for b in range(len(tiles))] == tiles
-        assert plan.total(q, kv, g, rows, keys, h) == h * sum(tiles)
-        x = 0
-        for b, t in enumerate(tiles):
-            for head in range(h):
-                for tile in {0, t // 2, t - 1}:
-                    plan.locate(q, kv, g, rows, keys, h, x + tile, out)
-                    assert tuple(out) == (b, head, tile, t)
-                x += t
-    assert plan.blocks(0, 77, 4, rows, keys) == 0 and plan.total(0, 77, 4, rows, keys, 8) == 0
+        tiles, how = _counted(q, kv, g, rows, keys), (q, kv, g, rows, keys, extra)
+        assert plan.blocks(*how) == len(tiles)
+        assert [plan.tiles(*how, b) for b in range(len(tiles))] == tiles
+        assert plan.total(*how, h) == h * (sum(tiles) + extra * len(tiles))
+        x, items = 0, [(b, head, t) for b, t in enumerate(tiles) for head in range(h)]
+        for i, (b, head, t) in enumerate(items):
+            for place in {0, (t + extra) // 2, t + extra - 1}:
+                more = plan.locate(*how, h, x + place, out)
+                assert tuple(out)[:4] == (b, head, place, t)
+                assert bool(more) == (i + 1 < len(items))
+                if more:
+                    assert tuple(out)[4:] == (items[i + 1][0], items[i + 1][1], 0, items[i + 1][2])
+            x += t + extra
+    assert plan.blocks(0, 77, 4, rows, keys, extra) == 0 and plan.total(0, 77, 4, rows, keys, extra, 8) == 0
 
 
 def test_ranges_cover_the_line(plan):
