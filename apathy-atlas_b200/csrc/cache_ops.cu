@@ -85,7 +85,7 @@ int check_attention(const atlas_b200_attention_desc& d) {
         return ATLAS_B200_ERR_LIMIT;
     if (!d.q || !d.out || !d.k_cache || !d.v_cache || !d.block_table || !d.cu_q || !d.kv_len) return ATLAS_B200_ERR_NULL;
     if (!aligned(d.q, 4) || d.q_row_stride % 2 || !aligned(d.out, 2) || !aligned(d.k_cache, 16) || !aligned(d.v_cache, 16) || !aligned(d.block_table, 4) ||
-        !aligned(d.cu_q, 4) || !aligned(d.kv_len, 4) || !aligned(d.lse, 4) || !aligned(d.ws, 16))
+        !aligned(d.cu_q, 4) || !aligned(d.kv_len, 4) || !aligned(d.lse, 4) || !aligned(d.ws, 32))
         return ATLAS_B200_ERR_ALIGN;
     return ATLAS_B200_OK;
 }
@@ -180,17 +180,6 @@ template <int DP, bool FP8> int launch_tc(AttnParams p, const TcPlan& plan, cuda
     static std::atomic<bool> done[kMaxDevices] = {};
     const int rc = allow_smem(attn::attn_tc_kernel<DP, FP8>, C::SMEM, done);
     if (rc) return rc;
-    if (C::SOFT_REGS > C::LAUNCH_REGS) {
-        // the split of registers draws on what the block was launched with: a kernel built with fewer would wait for them forever
-        static std::atomic<int> built{0};
-        if (built.load(std::memory_order_relaxed) == 0) {
-            cudaFuncAttributes a{};
-            const cudaError_t e = cudaFuncGetAttributes(&a, attn::attn_tc_kernel<DP, FP8>);
-            if (e != cudaSuccess) return cuda_status(e);
-            built.store(a.numRegs, std::memory_order_relaxed);
-        }
-        if (built.load(std::memory_order_relaxed) < C::LAUNCH_REGS) return ATLAS_B200_ERR_LIMIT;
-    }
     CUtensorMap map_k, map_v;
     const uint64_t size = FP8 ? 1 : 2;
     const uint64_t dims[3] = {p.head_dim, p.kv_heads, uint64_t(p.n_pages) * p.block_size};

@@ -177,6 +177,9 @@ __device__ __forceinline__ int32_t attn_cache_row(const AttnParams& p, const Att
 
 __device__ __forceinline__ float attn_e4m3(uint8_t b) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3))); }
 
+// Logarithm of a row's sum of exponentials from its M and L.
+__device__ __forceinline__ float attn_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) * ATTN_LN2; }
+
 // One row again from its own keys alone, by one warp.  The kernels multiply masked places with zeros, and zero times an infinity or a
 // NaN in the values of a later token is a NaN; a row that came out not finite is computed here instead, which leaves other tokens'
 // values unread.  The cost (a chain over the row's keys) is paid by such rows only.
@@ -209,12 +212,10 @@ static __device__ __noinline__ void attn_row_again(const AttnParams& p, bool fp8
         m = top;
     }
     const float f = l == 0.0f ? 0.0f : p.v_scale / l;
+    if (p.lse && lane == 0) p.lse[size_t(token) * p.q_heads + head] = attn_lse(m, l);
     for (uint32_t i = 0; i < 8; ++i)
         if (lane + 32u * i < D) p.out[size_t(token) * p.out_row_stride + size_t(head) * D + lane + 32u * i] = f32_to_bf16_bits(l == 0.0f ? 0.0f : o[i] * f);
 }
-
-// Logarithm of a row's sum of exponentials from its M and L.
-__device__ __forceinline__ float attn_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) * ATTN_LN2; }
 
 // ------------------------------------------------------------------------------------------------------------------
 // Joins the pieces of items that were cut.  CTA (c, y) looks at the cut between ranges c and c + 1; the first cut of an item joins it, each
@@ -273,7 +274,7 @@ __global__ void __launch_bounds__(ATTN_JOIN_THREADS) attn_join_kernel(const __gr
             }
         }
         if (p.lse && lane == 0) p.lse[size_t(token) * p.q_heads + head] = attn_lse(m, l);
-        if (__any_sync(0xFFFFFFFFu, odd) && sq.q_len > 1)
+        if (__any_sync(0xFFFFFFFFu, odd))
             attn_row_again(p, FP8, f.seq, token, head, attn_row_keys(sq, in_seq));
     }
 }

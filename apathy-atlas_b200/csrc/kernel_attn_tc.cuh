@@ -1,20 +1,29 @@
 // Paged attention for many rows (chunks of a prompt, and few-token chunks with many heads to a KV head): tcgen05.
 //
-// A block is two tiles of 128 rows (DP 256: one), each with scores S = Q K^T [128 x 128] and an output O [128 x DP] in tensor memory:
-//     S_g (128 columns each) | O_g (DP columns each)      P_g, BF16, over the first half of S_g's columns
-// One thread owns a row: 128 scores come to its registers (tcgen05.ld), maximum and sum need no exchange with other threads, P goes back
-// to tensor memory as the A operand of O += P V.  The two tiles take turns: while one's scores are in its softmax, the tensor cores work on
-// the other's P V and next Q K^T.  Q, K, V are 128-byte-swizzled tiles in shared memory: Q and K K-major, V as it lies in the cache
-// ([key][channel]), the MN-major form of the B operand.  K and V come page by page by TMA, in boxes of the largest power of two that
-// divides page and tile (8 rows at least); zero fill stands in for pages that do not exist and for channels behind head_dim.
+// A block is two tiles of 128 rows (DP 256: one).  A step is 64 keys: scores S = Q K^T [128 x 64], and O += P V with O [128 x DP], all in tensor
+// memory, for each row tile g:
+//     S_g even | S_g odd (64 columns each)  ...  O_g (DP columns each)      P_g, BF16, over the first half of its S's columns
+// The scores of step u + 2 follow the product with P of step u, whose columns they take; those of step u + 1 are there already.  So the
+// softmax of a row tile goes from step to step without waiting for the tensor cores, and they work on one tile's step while the other's
+// is in its softmax.  (With S of 128 keys in one piece a tile's softmax, product and next scores were one chain: 3900 cycles for 128
+// keys of both tiles, of which the tensor cores worked 2090.  A product of 64 columns reads 6 KB of shared memory for 32 cycles of
+// arithmetic, so it takes 48: 2560 cycles is what is left of the chain.)
 //
-// O is multiplied with 2^(M_old - M_new) only where a row's maximum has grown by more than 2^8 (RESCALE) since O's last factor: until then
-// the weights are 2^(s - M) with the old M, up to 2^8 and in the same FP32 sums, which is the same quotient.  That takes the
-// correction off the path of nearly every tile.
+// One thread owns a row: its scores come to its registers (tcgen05.ld), maximum and sum need no exchange with other threads, P goes back
+// to tensor memory as the A operand.  Q, K, V are 128-byte-swizzled tiles in shared memory: Q and K K-major, V as it lies in the cache
+// ([key][channel]), the MN-major form of the B operand.  K and V come 128 keys at a time, page by page by TMA, in boxes of the largest
+// power of two that divides page and tile (8 rows at least); zero fill stands in for pages that do not exist and for channels behind
+// head_dim.
 //
-// Warps: 0 TMA, 1 MMA (converged, one lane issues), 2 tensor memory; 4-7 and 8-11 softmax, epilogue and Q of a tile each; E4M3 caches:
-// 12-15 turn raw tiles into FP16 ones (one instruction for two values, exact, NaN kept; Q as FP16 with a power of two per row, see the
-// mma.sync form).  Every wait is bounded as elsewhere in the library.
+// O is multiplied with 2^(M_old - M_new) only where a row's maximum has grown by more than 2^8 (TC_RESCALE) since O's last factor: until
+// then the weights are 2^(s - M) with the old M, up to 2^8 and in the same FP32 sums, which is the same quotient.  That takes the
+// correction off the path of nearly every step.  (Exponentials by a polynomial on the FMA pipe for a quarter to a half of the scores,
+// the special-function unit being the busiest of the softmax: no faster.)
+//
+// Warps: 0 TMA, 1 MMA (converged, one lane issues), 2 tensor memory, 2 and 3 bring the next items' Q to L2; 4-7 and 8-11 softmax, epilogue and Q
+// of a row tile each, the next item's Q before this one's output; E4M3 caches: 12-15 turn raw tiles into FP16 ones (one instruction for
+// two values, exact, NaN kept; Q as FP16 with a power of two per row, see the mma.sync form).  Every wait is bounded as elsewhere in the
+// library.
 #pragma once
 
 #include "kernel_attn.cuh"
@@ -25,7 +34,7 @@ namespace attn {
 
 using namespace atlas::tc;
 
-constexpr uint32_t TC_KEYS = 128, TC_TILE_ROWS = 128;
+constexpr uint32_t TC_KEYS = 128, TC_STEP = 64, TC_TILE_ROWS = 128;
 constexpr float TC_RESCALE = 8.0f;
 
 template <int DP, bool FP8> struct TcCfg {
@@ -34,26 +43,21 @@ template <int DP, bool FP8> struct TcCfg {
     static constexpr int PANELS = DP / 64;                                   // 128-byte panels of a row
     static constexpr int PANEL = 128 * 128;
     static constexpr int TILE = PANELS * PANEL;                              // Q of a row tile; K or V of a key tile
-    static constexpr int STAGES = DP <= 64 ? 4 : DP <= 128 ? 2 : 1;
+    // K and V tiles share a ring, in the order the products take them: K 0, V 0, K 1, V 1, ...  A tile takes some 3000 cycles from request to
+    // arrival where every SM asks for one a thousand cycles; with two stages of either side, each released with the last product of an
+    // iteration, the MMA warp waited 870 cycles an iteration of 2090.
+    static constexpr int SLOTS = DP <= 64 ? 8 : DP <= 128 ? (FP8 ? 4 : 5) : 2;
     static constexpr int RAW = FP8 ? 128 * DP : 0, RAW_STAGES = FP8 ? (DP <= 128 ? 2 : 1) : 0;
-    static constexpr int OFF_Q = 0, OFF_K = NQ * TILE, OFF_V = OFF_K + STAGES * TILE, OFF_RAW = OFF_V + STAGES * TILE;
+    static constexpr int OFF_Q = 0, OFF_KV = NQ * TILE, OFF_RAW = OFF_KV + SLOTS * TILE;
     static constexpr int OFF_SCALE = OFF_RAW + RAW_STAGES * RAW;             // float[ROWS]: E4M3: what takes a row's power of two back
     static constexpr int OFF_BAR = OFF_SCALE + (FP8 ? ROWS * 4 : 0);
-    static constexpr int N_BAR = 4 * STAGES + 1 + 4 * NQ + 2 * RAW_STAGES;
+    static constexpr int N_BAR = 2 * SLOTS + 1 + 7 * NQ + 2 * RAW_STAGES;
     static constexpr int OFF_MISC = OFF_BAR + N_BAR * 8;                     // tensor memory, -, abort; attn_find's words
     static constexpr int SMEM = OFF_MISC + 16 + 20 * 8 + 1024;
     static constexpr int SOFT_WARPS = 4 * NQ, WARPS = 4 + SOFT_WARPS + (FP8 ? 4 : 0), THREADS = 32 * WARPS;
     static constexpr int CONV_WARP0 = 4 + SOFT_WARPS;
-    // registers a thread: at launch, and the split (warpgroups of 4 warps; the sum of the split is at most the launch's)
-    static constexpr int LAUNCH_REGS = THREADS <= 256 ? 248 : THREADS <= 384 ? 168 : 128;
-    static constexpr int SOFT_REGS = THREADS <= 256 ? 248 : THREADS <= 384 ? (FP8 ? 248 : 200) : 168;
-    static constexpr int AUX_REGS = THREADS <= 256 ? 248 : THREADS <= 384 ? (FP8 ? 128 : 104) : 88;
-    static_assert(32 * (SOFT_WARPS * SOFT_REGS + (WARPS - SOFT_WARPS) * AUX_REGS) <= THREADS * LAUNCH_REGS, "registers");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
-
-template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
     asm volatile(
@@ -63,17 +67,32 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
           "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-          "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-          "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+// 32 bytes of a row in one store (whole sectors)
+__device__ __forceinline__ void stg256(void* to, const uint32_t* r) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"l"(to), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Two FP32 values in one register pair and one issue slot.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void of_pair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 // V as it lies in the cache: rows of keys, channels contiguous.  MN-major, 128-byte swizzle: 64 channels x 8 keys an atom of 1024 bytes,
 // the next 8 keys 1024 bytes on (stride offset), the next 64 channels a panel on (leading offset).
@@ -98,24 +117,25 @@ template <int DP, bool FP8>
 __global__ void __launch_bounds__(TcCfg<DP, FP8>::THREADS, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnParams p, const uint32_t box_rows) {
     using C = TcCfg<DP, FP8>;
-    constexpr int NQ = C::NQ, ST = C::STAGES;
+    constexpr int NQ = C::NQ, SLOTS = C::SLOTS;
     extern __shared__ uint8_t attn_smem_raw[];
     const uint32_t base = (smem_u32(attn_smem_raw) + 1023u) & ~1023u;
     uint8_t* const gen = attn_smem_raw + (base - smem_u32(attn_smem_raw));
     const uint32_t bar = base + C::OFF_BAR;
-    const uint32_t K_FULL = bar, K_EMPTY = bar + 8 * ST, V_FULL = bar + 16 * ST, V_EMPTY = bar + 24 * ST, V_TAIL = bar + 32 * ST, Q_FULL = V_TAIL + 8,
-                   S_FULL = Q_FULL + 8 * NQ, P_FULL = S_FULL + 8 * NQ, PV_DONE = P_FULL + 8 * NQ, RAW_FULL = PV_DONE + 8 * NQ, RAW_EMPTY = RAW_FULL + 8 * C::RAW_STAGES;
+    const uint32_t FULL = bar, EMPTY = bar + 8 * SLOTS, V_TAIL = bar + 16 * SLOTS, Q_FULL = V_TAIL + 8,
+                   S_FULL = Q_FULL + 8 * NQ, P_FULL = S_FULL + 16 * NQ, PV_DONE = P_FULL + 16 * NQ, RAW_FULL = PV_DONE + 16 * NQ, RAW_EMPTY = RAW_FULL + 8 * C::RAW_STAGES;
     volatile uint32_t* const misc = reinterpret_cast<volatile uint32_t*>(gen + C::OFF_MISC);
     volatile uint32_t* const abort_flag = misc + 2;
     uint64_t* const sh = reinterpret_cast<uint64_t*>(gen + C::OFF_MISC + 16);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
 
     if (tid == 0) {
-        for (int i = 0; i < ST; ++i) {
-            mbar_init(K_FULL + 8 * i, FP8 ? 128 : 1); mbar_init(K_EMPTY + 8 * i, 1); mbar_init(V_FULL + 8 * i, FP8 ? 128 : 1); mbar_init(V_EMPTY + 8 * i, 1);
-        }
+        for (int i = 0; i < SLOTS; ++i) { mbar_init(FULL + 8 * i, FP8 ? 128 : 1); mbar_init(EMPTY + 8 * i, 1); }
         mbar_init(V_TAIL, 1);
-        for (int g = 0; g < NQ; ++g) { mbar_init(Q_FULL + 8 * g, 128); mbar_init(S_FULL + 8 * g, 1); mbar_init(P_FULL + 8 * g, 128); mbar_init(PV_DONE + 8 * g, 1); }
+        for (int g = 0; g < NQ; ++g) mbar_init(Q_FULL + 8 * g, 128);
+        // Scores, weights and products of even and of odd steps have barriers of their own: whoever waits for one of step u knows that step
+        // u - 2 is over, so a phase cannot be mistaken for the one before last.
+        for (int i = 0; i < 2 * NQ; ++i) { mbar_init(S_FULL + 8 * i, 1); mbar_init(P_FULL + 8 * i, 128); mbar_init(PV_DONE + 8 * i, 1); }
         for (int i = 0; i < C::RAW_STAGES; ++i) { mbar_init(RAW_FULL + 8 * i, 1); mbar_init(RAW_EMPTY + 8 * i, 128); }
         misc[2] = 0;
         fence_barrier_init();
@@ -137,83 +157,76 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         return x < x_end ? x : ~0ull;
     });
     AttnWalk walk(p, found, x, x_end, C::ROWS, TC_KEYS);
-    // rows of a row tile of the item, the keys its last row sees, and its tiles within the piece
+    // rows of a row tile of the item, and the steps that it takes of the piece
     auto tile_rows = [&](uint32_t g) {
         const uint32_t all = walk.sq.q_len * p.group, r0 = walk.at.block * C::ROWS + g * TC_TILE_ROWS;
         return all > r0 ? min(all - r0, TC_TILE_ROWS) : 0u;
     };
-    auto tiles_of = [&](uint32_t g) {
+    auto steps_of = [&](uint32_t g) {
         const uint32_t rows = tile_rows(g);
         if (rows == 0) return 0u;
         const uint32_t keys = attn_row_keys(walk.sq, (walk.at.block * C::ROWS + g * TC_TILE_ROWS + rows - 1) / p.group);
-        const uint32_t t = min(max((keys + TC_KEYS - 1) / TC_KEYS, 1u), walk.t1);
-        return t > walk.t0 ? t - walk.t0 : 0u;
+        const uint32_t t = min(max((keys + TC_STEP - 1) / TC_STEP, 1u), 2u * walk.t1);
+        return t > 2u * walk.t0 ? t - 2u * walk.t0 : 0u;
     };
-    // tiles of the piece that any row tile wants (the last tile that has rows wants the most)
-    auto tiles_wanted = [&] { return NQ == 2 ? max(tiles_of(0), tiles_of(NQ - 1)) : tiles_of(0); };
+    // key tiles of the piece that any row tile wants (the last row tile that has rows wants the most)
+    auto tiles_wanted = [&] { return ((NQ == 2 ? max(steps_of(0), steps_of(NQ - 1)) : steps_of(0)) + 1u) / 2u; };
 
     if (warp < 4) {
-        if constexpr (C::AUX_REGS < C::LAUNCH_REGS) regs_down<C::AUX_REGS>();
         if (warp == 0) {
             // ---- TMA: K and V of a tile, one lane a box ----
             const uint32_t per_tile = TC_KEYS / box_rows;
             const AttnDivisor div = attn_divisor(p.block_size);
-            uint32_t ks = 0, kph = 0, vs = 0, vph = 0, tail_ph = 0, rs = 0, rph = 0;
+            uint32_t slot = 0, ph = 0, tail_ph = 0, rs = 0, rph = 0;
             bool ok = true;
             while (ok && walk.next(p)) {
                 const int32_t* table = p.block_table + size_t(walk.seq) * p.table_stride;
                 const uint32_t n = tiles_wanted(), kv_len = walk.sq.kv_len;
                 const uint32_t none = p.n_pages * p.block_size;              // a row behind the last page: TMA fills with zeros
-                auto find = [&](uint32_t j) -> uint32_t {                    // cache row of this lane's box of tile j
+                auto page_of = [&](uint32_t j) -> uint32_t {                 // this lane's box of tile j: its page, as the table has it
                     const uint32_t pos = (walk.t0 + j) * TC_KEYS + lane * box_rows;
-                    if (j >= n || lane >= per_tile || pos >= kv_len) return none;
-                    const uint32_t page = attn_div(pos, div), id = uint32_t(table[page]);
-                    if (id >= p.n_pages) { record_status(STATUS_PAGE_OUT_OF_RANGE); return none; }
-                    return id * p.block_size + (pos - page * p.block_size);
+                    return j < n && lane < per_tile && pos < kv_len ? uint32_t(table[attn_div(pos, div)]) : 0u;
                 };
-                uint32_t row_next = find(0);
+                uint32_t id_next = page_of(0);
                 for (uint32_t j = 0; ok && j < n; ++j) {
-                    const uint32_t row = row_next, pos0 = (walk.t0 + j) * TC_KEYS;
-                    row_next = find(j + 1);
+                    const uint32_t id = id_next, pos0 = (walk.t0 + j) * TC_KEYS, pos = pos0 + lane * box_rows;
+                    id_next = page_of(j + 1);
+                    uint32_t row = id * p.block_size + (pos - attn_div(pos, div) * p.block_size);
+                    if (id >= p.n_pages) {
+                        record_status(STATUS_PAGE_OUT_OF_RANGE);
+                        row = none;
+                    }
                     const uint32_t left = kv_len > pos0 ? kv_len - pos0 : 0u, boxes = min((left + box_rows - 1) / box_rows, per_tile);
                     if constexpr (!FP8) {
-                        ok = mbar_wait_warp(K_EMPTY + 8 * ks, kph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER, 20);
-                        if (!ok) break;
-                        const uint32_t kd = base + C::OFF_K + ks * C::TILE;
-                        if (lane == 0) mbar_arrive_expect_tx(K_FULL + 8 * ks, boxes * box_rows * 128u * C::PANELS);
-                        __syncwarp();
-                        if (lane < boxes)
 #pragma unroll
-                            for (int pn = 0; pn < C::PANELS; ++pn)
-                                tma_load_3d(kd + pn * C::PANEL + lane * box_rows * 128u, &map_k, pn * 64, int32_t(walk.at.head), int32_t(row), K_FULL + 8 * ks);
-                        __syncwarp();
-                        if (++ks == uint32_t(ST)) { ks = 0; kph ^= 1u; }
-                        ok = mbar_wait_warp(V_EMPTY + 8 * vs, vph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER, 20);
-                        if (!ok) break;
-                        const uint32_t vd = base + C::OFF_V + vs * C::TILE;
-                        const bool tail = left < TC_KEYS;
-                        const uint32_t full = tail ? V_TAIL : V_FULL + 8 * vs;
-                        if (lane == 0) mbar_arrive_expect_tx(full, boxes * box_rows * 128u * C::PANELS);
-                        __syncwarp();
-                        if (lane < boxes)
-#pragma unroll
-                            for (int pn = 0; pn < C::PANELS; ++pn)
-                                tma_load_3d(vd + pn * C::PANEL + lane * box_rows * 128u, &map_v, pn * 64, int32_t(walk.at.head), int32_t(row), full);
-                        __syncwarp();
-                        if (tail) {
-                            // behind the sequence's end a page holds anything, and zero times a NaN is one: zeros before the product
-                            ok = mbar_wait_warp(V_TAIL, tail_ph, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER);
-                            tail_ph ^= 1u;
+                        for (int side = 0; side < 2; ++side) {
+                            ok = ok && mbar_wait_warp(EMPTY + 8 * slot, ph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER, 20);
                             if (!ok) break;
-                            for (uint32_t i = lane; i < (TC_KEYS - left) * 8u; i += 32)
+                            const uint32_t dst = base + C::OFF_KV + slot * C::TILE;
+                            const bool tail = side == 1 && left < TC_KEYS;
+                            const uint32_t full = tail ? V_TAIL : FULL + 8 * slot;
+                            if (lane == 0) mbar_arrive_expect_tx(full, boxes * box_rows * 128u * C::PANELS);
+                            __syncwarp();
+                            if (lane < boxes)
 #pragma unroll
-                                for (int pn = 0; pn < C::PANELS; ++pn) sts128(vd + pn * C::PANEL + left * 128u + i * 16u, 0u, 0u, 0u, 0u);
-                            fence_proxy_async();
+                                for (int pn = 0; pn < C::PANELS; ++pn)
+                                    tma_load_3d(dst + pn * C::PANEL + lane * box_rows * 128u, side ? &map_v : &map_k, pn * 64, int32_t(walk.at.head), int32_t(row), full);
                             __syncwarp();
-                            if (lane == 0) mbar_arrive(V_FULL + 8 * vs);
-                            __syncwarp();
+                            if (tail) {
+                                // behind the sequence's end a page holds anything, and zero times a NaN is one: zeros before the product
+                                ok = mbar_wait_warp(V_TAIL, tail_ph, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER);
+                                tail_ph ^= 1u;
+                                if (!ok) break;
+                                for (uint32_t i = lane; i < (TC_KEYS - left) * 8u; i += 32)
+#pragma unroll
+                                    for (int pn = 0; pn < C::PANELS; ++pn) sts128(dst + pn * C::PANEL + left * 128u + i * 16u, 0u, 0u, 0u, 0u);
+                                fence_proxy_async();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(FULL + 8 * slot);
+                                __syncwarp();
+                            }
+                            if (++slot == uint32_t(SLOTS)) { slot = 0; ph ^= 1u; }
                         }
-                        if (++vs == uint32_t(ST)) { vs = 0; vph ^= 1u; }
                     } else {
 #pragma unroll 1
                         for (int side = 0; side < 2; ++side) {
@@ -233,67 +246,81 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
         } else if (warp == 1) {
             // ---- MMA ----
-            constexpr uint32_t idesc_s = attn_idesc(TC_KEYS, FP8, false), idesc_o = attn_idesc(DP, FP8, true);
-            uint32_t ks = 0, kph = 0, vs = 0, vph = 0, q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
+            constexpr uint32_t idesc_s = attn_idesc(TC_STEP, FP8, false), idesc_o = attn_idesc(DP, FP8, true);
+            uint32_t slot = 0, ph = 0, q_ph[2] = {0, 0}, p_ph[2][2] = {{0, 0}, {0, 0}};
             bool ok = true;
-            auto scores = [&](uint32_t g, uint32_t stage) {
+            auto advance = [&] { if (++slot == uint32_t(SLOTS)) { slot = 0; ph ^= 1u; } };
+            auto scores = [&](uint32_t g, uint32_t h, uint32_t stage) {      // of half h of the key tile in `stage`
                 if (elect_one()) {
-                    const uint64_t q = make_kmajor_sw128_desc(base + C::OFF_Q + g * C::TILE), k = make_kmajor_sw128_desc(base + C::OFF_K + stage * C::TILE);
+                    const uint64_t q = make_kmajor_sw128_desc(base + C::OFF_Q + g * C::TILE), k = make_kmajor_sw128_desc(base + C::OFF_KV + stage * C::TILE + h * (TC_STEP * 128u));
 #pragma unroll
                     for (int s = 0; s < DP / 16; ++s)
-                        umma_bf16_ss<false>(tmem + g * 128u, q + (s >> 2) * (C::PANEL >> 4) + (s & 3) * 2, k + (s >> 2) * (C::PANEL >> 4) + (s & 3) * 2, idesc_s, s ? 1u : 0u);
-                    umma_commit<false>(S_FULL + 8 * g);
+                        umma_bf16_ss<false>(tmem + g * 128u + h * TC_STEP, q + (s >> 2) * (C::PANEL >> 4) + (s & 3) * 2, k + (s >> 2) * (C::PANEL >> 4) + (s & 3) * 2, idesc_s, s ? 1u : 0u);
+                    umma_commit<false>(S_FULL + 8 * (2 * g + h));
                 }
                 __syncwarp();
             };
             while (ok && walk.next(p)) {
-                const uint32_t n_g[2] = {tiles_of(0), NQ == 2 ? tiles_of(NQ - 1) : 0u}, n = max(n_g[0], n_g[1]);
+                const uint32_t n_g[2] = {steps_of(0), NQ == 2 ? steps_of(NQ - 1) : 0u}, n = max(n_g[0], n_g[1]);
                 if (n == 0) continue;
-                ok = mbar_wait_warp(K_FULL + 8 * ks, kph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
+                ok = mbar_wait_warp(FULL + 8 * slot, ph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
                 if (!ok) break;
 #pragma unroll
-                for (uint32_t g = 0; g < uint32_t(NQ); ++g) {
-                    if (n_g[g] == 0) continue;
-                    ok = ok && mbar_wait_warp(Q_FULL + 8 * g, q_ph[g], abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
-                    if (!ok) break;
-                    q_ph[g] ^= 1u;
-                    tcgen05_fence_after();
-                    scores(g, ks);
-                }
-                if (!ok) break;
-                if (elect_one()) umma_commit<false>(K_EMPTY + 8 * ks);
-                __syncwarp();
-                if (++ks == uint32_t(ST)) { ks = 0; kph ^= 1u; }
-                for (uint32_t j = 0; ok && j < n; ++j) {
-                    ok = mbar_wait_warp(V_FULL + 8 * vs, vph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
-                    if (ok && j + 1 < n) ok = mbar_wait_warp(K_FULL + 8 * ks, kph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
-                    if (!ok) break;
-                    const uint32_t vd = base + C::OFF_V + vs * C::TILE;
+                for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
                     for (uint32_t g = 0; g < uint32_t(NQ); ++g) {
-                        if (j >= n_g[g]) continue;
-                        ok = ok && mbar_wait_warp(P_FULL + 8 * g, p_ph[g], abort_flag, STATUS_WAIT_EXPIRED_MMA);
-                        if (!ok) break;
-                        p_ph[g] ^= 1u;
-                        tcgen05_fence_after();
-                        if (elect_one()) {
-                            const uint64_t v = make_mnmajor_sw128_desc(vd, C::PANEL);
-#pragma unroll
-                            for (int s = 0; s < int(TC_KEYS) / 16; ++s)
-                                umma_bf16_ts<false>(tmem + NQ * 128u + g * uint32_t(DP), tmem + g * 128u + s * 8u, v + s * (2048 >> 4), idesc_o, (j | s) ? 1u : 0u);
-                            umma_commit<false>(PV_DONE + 8 * g);
+                        if (h >= n_g[g]) continue;
+                        if (h == 0) {
+                            ok = ok && mbar_wait_warp(Q_FULL + 8 * g, q_ph[g], abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
+                            q_ph[g] ^= 1u;
                         }
-                        __syncwarp();
-                        if (j + 1 < n_g[g]) scores(g, ks);
+                        if (!ok) break;
+                        tcgen05_fence_after();
+                        scores(g, h, slot);
                     }
+                if (!ok) break;
+                if (elect_one()) umma_commit<false>(EMPTY + 8 * slot);
+                __syncwarp();
+                advance();
+                for (uint32_t u0 = 0; ok && u0 < n; u0 += 2) {
+                    ok = mbar_wait_warp(FULL + 8 * slot, ph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
                     if (!ok) break;
-                    if (elect_one()) {
-                        umma_commit<false>(V_EMPTY + 8 * vs);
-                        if (j + 1 < n) umma_commit<false>(K_EMPTY + 8 * ks);
+                    const uint32_t v_slot = slot, vd = base + C::OFF_KV + slot * C::TILE;
+                    const uint32_t last_h = u0 + 1 < n ? 1u : 0u, last_g = NQ == 2 && u0 + last_h < n_g[1] ? 1u : 0u;   // the last to read V
+                    bool k_there = false;
+                    advance();
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (uint32_t g = 0; g < uint32_t(NQ); ++g) {
+                            const uint32_t u = u0 + h;
+                            if (!ok || u >= n_g[g]) continue;
+                            ok = mbar_wait_warp(P_FULL + 8 * (2 * g + h), p_ph[g][h], abort_flag, STATUS_WAIT_EXPIRED_MMA);
+                            if (!ok) continue;
+                            p_ph[g][h] ^= 1u;
+                            tcgen05_fence_after();
+                            if (elect_one()) {
+                                const uint64_t v = make_mnmajor_sw128_desc(vd + h * (TC_STEP * 128u), C::PANEL);
+#pragma unroll
+                                for (int s = 0; s < int(TC_STEP) / 16; ++s)
+                                    umma_bf16_ts<false>(tmem + NQ * 128u + g * uint32_t(DP), tmem + g * 128u + h * TC_STEP + s * 8u, v + s * (2048 >> 4), idesc_o, (u | s) ? 1u : 0u);
+                                umma_commit<false>(PV_DONE + 8 * (2 * g + h));
+                                if (h == last_h && g == last_g) umma_commit<false>(EMPTY + 8 * v_slot);
+                            }
+                            __syncwarp();
+                            if (u + 2 < n_g[g]) {
+                                if (!k_there) ok = mbar_wait_warp(FULL + 8 * slot, ph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
+                                if (!ok) continue;
+                                k_there = true;
+                                scores(g, h, slot);
+                            }
+                        }
                     }
-                    __syncwarp();
-                    if (++vs == uint32_t(ST)) { vs = 0; vph ^= 1u; }
-                    if (j + 1 < n && ++ks == uint32_t(ST)) { ks = 0; kph ^= 1u; }
+                    if (ok && u0 + 2 < n) {
+                        if (elect_one()) umma_commit<false>(EMPTY + 8 * slot);
+                        __syncwarp();
+                        advance();
+                    }
                 }
             }
         } else {
@@ -310,34 +337,32 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         }
     } else if (warp < uint32_t(C::CONV_WARP0)) {
         // ---- softmax: a row a thread ----
-        if constexpr (C::SOFT_REGS > C::LAUNCH_REGS) regs_up<C::SOFT_REGS>();
         const uint32_t g = (warp - 4) >> 2, quad = warp & 3u, row_in = quad * 32u + lane;
         const uint32_t t_s = tmem + g * 128u + ((quad * 32u) << 16), t_o = tmem + NQ * 128u + g * uint32_t(DP) + ((quad * 32u) << 16);
         const uint32_t q_tile = base + C::OFF_Q + g * C::TILE;
         float* const scale_s = reinterpret_cast<float*>(gen + C::OFF_SCALE) + g * TC_TILE_ROWS;
         const uint32_t D = p.head_dim;
         const AttnDivisor group_div = attn_divisor(p.group);
-        uint32_t s_ph = 0, pv_ph = 0;
-        bool ok = true;
-        while (ok && walk.next(p)) {
-            const uint32_t n = tiles_of(g), rows = tile_rows(g);
-            if (rows == 0) continue;
-            const uint32_t row0 = walk.at.block * C::ROWS + g * TC_TILE_ROWS;
-            float c = p.scale * p.k_scale * ATTN_LOG2E, m = -INFINITY, l = 0.0f;
-            if (n) {
-                // Q: this warp's 32 rows, sixteen bytes a lane
-                constexpr uint32_t CH = DP / 8;
-                const uint16_t* const q_head = p.q + size_t(walk.sq.row0) * p.q_row_stride + size_t(walk.at.head) * p.group * D;
-                uint4 qv[CH];                                                // (all loads in flight: one latency)
+        uint32_t s_ph[2] = {0, 0};                                           // of the next step's barriers, and of the ones after
+        // Q of the item that the walk is at: this warp's 32 rows, sixteen bytes a lane, all loads in flight.  (The item before has had its
+        // last scores computed.)
+        auto load_q = [&] {
+            const uint32_t rows = tile_rows(g), row0 = walk.at.block * C::ROWS + g * TC_TILE_ROWS;
+            if (rows == 0 || steps_of(g) == 0) return;
+            constexpr uint32_t CH = DP / 8, LOADS = CH < 16 ? CH : 16;
+            const uint16_t* const q_head = p.q + size_t(walk.sq.row0) * p.q_row_stride + size_t(walk.at.head) * p.group * D;
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < CH; i0 += LOADS) {
+                uint4 qv[LOADS];
 #pragma unroll
-                for (uint32_t i = 0; i < CH; ++i) {
-                    const uint32_t idx = i * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH, row = row0 + r, tok = attn_div(row, group_div);
+                for (uint32_t i = 0; i < LOADS; ++i) {
+                    const uint32_t idx = (i0 + i) * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH, row = row0 + r, tok = attn_div(row, group_div);
                     qv[i] = make_uint4(0u, 0u, 0u, 0u);
                     if (r < rows && ch * 8u < D) qv[i] = *reinterpret_cast<const uint4*>(q_head + size_t(tok) * p.q_row_stride + (row - tok * p.group) * D + ch * 8u);
                 }
 #pragma unroll
-                for (uint32_t i = 0; i < CH; ++i) {
-                    const uint32_t idx = i * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH;
+                for (uint32_t i = 0; i < LOADS; ++i) {
+                    const uint32_t idx = (i0 + i) * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH;
                     uint4 v = qv[i];
                     if constexpr (FP8) {
                         uint32_t w[4] = {v.x, v.y, v.z, v.w}, top = 0;
@@ -354,42 +379,59 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                     sts128(q_tile + (ch >> 3) * C::PANEL + sw128_off(r, ch & 7u), v.x, v.y, v.z, v.w);
                 }
-                fence_proxy_async();
-                __syncwarp();
-                mbar_arrive(Q_FULL + 8 * g);
-                if constexpr (FP8) c *= scale_s[row_in];
             }
+            fence_proxy_async();
+            __syncwarp();
+            mbar_arrive(Q_FULL + 8 * g);
+        };
+        bool ok = true, more = walk.next(p);
+        if (more) load_q();
+        while (ok && more) {
+            // this item, as the walk goes on to the next one before its output is written
+            const uint32_t n = steps_of(g), rows = tile_rows(g), row0 = walk.at.block * C::ROWS + g * TC_TILE_ROWS, seq = walk.seq, t0 = walk.t0, seq_row0 = walk.sq.row0;
+            const bool whole = walk.whole();
             const uint32_t row = row0 + row_in, tok = attn_div(row, group_div), head = walk.at.head * p.group + row - tok * p.group;
             const uint32_t keys = row_in < rows ? attn_row_keys(walk.sq, tok) : 0u, all_see = attn_row_keys(walk.sq, row0 / p.group);
-            for (uint32_t j = 0; ok && j < n; ++j) {
-                ok = mbar_wait(S_FULL + 8 * g, s_ph, abort_flag, STATUS_WAIT_EXPIRED_EPILOGUE);
-                ok = __all_sync(0xFFFFFFFFu, ok);
+            float c = p.scale * p.k_scale * ATTN_LOG2E, m = -INFINITY, l = 0.0f;
+            if constexpr (FP8) {
+                if (n) c *= scale_s[row_in];
+                __syncwarp();                                                // read before the next item's are written
+            }
+            const uint64_t c2 = pair_of(c, c);
+#pragma unroll 1
+            for (uint32_t u = 0; ok && u < n; ++u) {
+                const uint32_t h = u & 1u, t_h = t_s + h * TC_STEP;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(S_FULL + 8 * (2 * g + h), s_ph[0], abort_flag, STATUS_WAIT_EXPIRED_EPILOGUE));
                 if (!ok) break;
-                s_ph ^= 1u;
+                {                                                            // (the two barriers take turns, and so do their phases)
+                    const uint32_t t = s_ph[0] ^ 1u;
+                    s_ph[0] = s_ph[1];
+                    s_ph[1] = t;
+                }
                 tcgen05_fence_after();
-                uint32_t s[128];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) tmem_ld32(t_s + 32 * k, s + 32 * k);
+                uint32_t s[TC_STEP];
+                tmem_ld32(t_h, s);
+                tmem_ld32(t_h + 32, s + 32);
                 tmem_ld_wait();
-                const uint32_t pos0 = (walk.t0 + j) * TC_KEYS;
-                if (pos0 + TC_KEYS > all_see) {
+                const uint32_t pos0 = t0 * TC_KEYS + u * TC_STEP;
+                if (pos0 + TC_STEP > all_see) {
                     const uint32_t mine = keys > pos0 ? keys - pos0 : 0u;
 #pragma unroll
-                    for (uint32_t k = 0; k < 128; ++k)
+                    for (uint32_t k = 0; k < TC_STEP; ++k)
                         if (k >= mine) s[k] = 0xFF800000u;                   // -inf
                 }
                 float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 128; k += 8)
+                for (uint32_t k = 0; k < TC_STEP; k += 8)
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) top4[u] = fmaxf(fmaxf(top4[u], __uint_as_float(s[k + 2 * u])), __uint_as_float(s[k + 2 * u + 1]));
+                    for (int v = 0; v < 4; ++v) top4[v] = fmaxf(fmaxf(top4[v], __uint_as_float(s[k + 2 * v])), __uint_as_float(s[k + 2 * v + 1]));
                 const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * c;
-                const bool grow = top > m + (j ? TC_RESCALE : 0.0f);
-                if (j == 0) {
+                const bool grow = top > m + TC_RESCALE;
+                if (u == 0) {
                     m = top;
                 } else if (__any_sync(0xFFFFFFFFu, grow)) {
-                    // O is this thread's row until the next P is handed over, once the product before has been added
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(PV_DONE + 8 * g, pv_ph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_EPILOGUE));
+                    // O is this thread's row until this step's P is handed over, once the product before has been added
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(PV_DONE + 8 * (2 * g + (h ^ 1u)), s_ph[0] ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_EPILOGUE));
                     if (!ok) break;
                     tcgen05_fence_after();
                     const float keep = grow ? ex2(m - top) : 1.0f;
@@ -401,93 +443,100 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         tmem_ld16(t_o + k, v);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int u = 0; u < 16; ++u) v[u] = __float_as_uint(__uint_as_float(v[u]) * keep);
+                        for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
                         tmem_st16(t_o + k, v);
                     }
                 }
                 const float off = m == -INFINITY ? 0.0f : -m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t off2 = pair_of(off, off);
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
-                for (int k = 0; k < 128; k += 32) {
+                for (uint32_t k = 0; k < TC_STEP / 32; ++k) {
                     uint32_t w[16];
 #pragma unroll
-                    for (int u = 0; u < 16; ++u) {
-                        const float a = ex2(fmaf(__uint_as_float(s[k + 2 * u]), c, off)), b = ex2(fmaf(__uint_as_float(s[k + 2 * u + 1]), c, off));
-                        sum[u & 3] += a + b;
-                        w[u] = pack_pair<FP8>(a, b);
+                    for (int v = 0; v < 16; ++v) {
+                        const uint64_t x2 = fma2(pair_of(__uint_as_float(s[32 * k + 2 * v]), __uint_as_float(s[32 * k + 2 * v + 1])), c2, off2);
+                        float e0, e1;
+                        of_pair(x2, e0, e1);
+                        e0 = ex2(e0);
+                        e1 = ex2(e1);
+                        sum[v & 1] = add2(sum[v & 1], pair_of(e0, e1));
+                        w[v] = pack_pair<FP8>(e0, e1);
                     }
-                    tmem_st16(t_s + (k >> 1), w);
+                    tmem_st16(t_h + 16 * k, w);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                {
+                    float a0, a1;
+                    of_pair(add2(sum[0], sum[1]), a0, a1);
+                    l += a0 + a1;
+                }
                 tmem_st_wait();
                 tcgen05_fence_before();
-                mbar_arrive(P_FULL + 8 * g);
-                pv_ph ^= 1u;
+                mbar_arrive(P_FULL + 8 * (2 * g + h));
             }
             if (!ok) break;
-            // ---- the piece is done ----
-            const bool whole = walk.whole();
+            const uint32_t last_ph = s_ph[1] ^ 1u;
+            if (n & 1u) { const uint32_t t = s_ph[0]; s_ph[0] = s_ph[1]; s_ph[1] = t; }    // the next item begins with the even barrier
+            // ---- the piece is done: the next item's Q, then this one's output ----
+            more = walk.next(p);
+            if (more) load_q();
+            if (rows == 0) continue;
             if (n) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(PV_DONE + 8 * g, pv_ph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_EPILOGUE));
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(PV_DONE + 8 * (2 * g + ((n - 1u) & 1u)), last_ph, abort_flag, STATUS_WAIT_EXPIRED_EPILOGUE));
                 if (!ok) break;
                 tcgen05_fence_after();
             }
             if (!whole) {
-                float* part = p.parts + attn_part_floats(C::ROWS, DP) * (2 * size_t(blockIdx.x) + (walk.t0 == 0 ? 1 : 0));
+                float* part = p.parts + attn_part_floats(C::ROWS, DP) * (2 * size_t(blockIdx.x) + (t0 == 0 ? 1 : 0));
                 const uint32_t r = g * TC_TILE_ROWS + row_in;
 #pragma unroll 1
-                for (int k = 0; k < DP; k += 16) {
-                    uint32_t v[16] = {};
-                    if (n) { tmem_ld16(t_o + k, v); tmem_ld_wait(); }
+                for (int k = 0; k < DP; k += 32) {
+                    uint32_t v[32] = {};
+                    if (n) { tmem_ld32(t_o + k, v); tmem_ld_wait(); }
                     if (row_in < rows)
 #pragma unroll
-                        for (int u = 0; u < 16; u += 4)
-                            *reinterpret_cast<uint4*>(part + size_t(r) * DP + k + u) = make_uint4(v[u], v[u + 1], v[u + 2], v[u + 3]);
+                        for (int e = 0; e < 32; e += 8) stg256(part + size_t(r) * DP + k + e, v + e);
                 }
                 if (row_in < rows) { part[size_t(C::ROWS) * DP + r] = m; part[size_t(C::ROWS) * DP + C::ROWS + r] = l; }
             } else {
-                // through this warp's rows of the Q tile (all of its scores have been computed), then whole rows out
                 const float inv = l == 0.0f ? 0.0f : p.v_scale / l;
+                uint16_t* const o_row = p.out + size_t(seq_row0 + tok) * p.out_row_stride + size_t(head) * D;
+                const bool wide = (reinterpret_cast<uintptr_t>(o_row) & 31u) == 0u;
                 bool odd = false;
 #pragma unroll 1
-                for (int k = 0; k < DP; k += 16) {
-                    uint32_t v[16] = {}, w[8];
-                    if (n) { tmem_ld16(t_o + k, v); tmem_ld_wait(); }
+                for (uint32_t k = 0; k < D; k += 32) {                       // (head_dim is a multiple of 32)
+                    uint32_t v[32] = {}, w[16];
+                    if (n) { tmem_ld32(t_o + k, v); tmem_ld_wait(); }
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        const float a = l == 0.0f ? 0.0f : __uint_as_float(v[2 * u]) * inv, b = l == 0.0f ? 0.0f : __uint_as_float(v[2 * u + 1]) * inv;
+                    for (int e = 0; e < 16; ++e) {
+                        const float a = l == 0.0f ? 0.0f : __uint_as_float(v[2 * e]) * inv, b = l == 0.0f ? 0.0f : __uint_as_float(v[2 * e + 1]) * inv;
                         odd |= !isfinite(a) || !isfinite(b);
-                        w[u] = pack_bf16x2(a, b);
+                        w[e] = pack_bf16x2(a, b);
                     }
-                    const uint32_t to = q_tile + (k >> 6) * C::PANEL, ch = (k >> 3) & 7u;
-                    sts128(to + sw128_off(row_in, ch), w[0], w[1], w[2], w[3]);
-                    sts128(to + sw128_off(row_in, ch + 1), w[4], w[5], w[6], w[7]);
+                    if (row_in < rows) {
+                        if (wide) {
+                            stg256(o_row + k, w);
+                            stg256(o_row + k + 16, w + 8);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(o_row + k + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+                        }
+                    }
                 }
-                if (p.lse && row_in < rows) p.lse[size_t(walk.sq.row0 + tok) * p.q_heads + head] = attn_lse(m, l);
-                __syncwarp();
-                constexpr uint32_t CH = DP / 8;
-                uint16_t* const o_head = p.out + size_t(walk.sq.row0) * p.out_row_stride + size_t(walk.at.head) * p.group * D;
-#pragma unroll 8
-                for (uint32_t i = 0; i < CH; ++i) {
-                    const uint32_t idx = i * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH, rw = row0 + r, t = attn_div(rw, group_div);
-                    const uint4 v = lds128(q_tile + (ch >> 3) * C::PANEL + sw128_off(r, ch & 7u));
-                    if (r < rows && ch * 8u < D) *reinterpret_cast<uint4*>(o_head + size_t(t) * p.out_row_stride + (rw - t * p.group) * D + ch * 8u) = v;
-                }
-                __syncwarp();
-                uint32_t again = walk.sq.q_len > 1 ? __ballot_sync(0xFFFFFFFFu, odd && row_in < rows) : 0u;
+                if (p.lse && row_in < rows) p.lse[size_t(seq_row0 + tok) * p.q_heads + head] = attn_lse(m, l);
+                uint32_t again = __ballot_sync(0xFFFFFFFFu, odd && row_in < rows);
                 while (again) {
                     const uint32_t k = __ffs(again) - 1u;
                     again &= again - 1u;
-                    attn_row_again(p, FP8, walk.seq, walk.sq.row0 + __shfl_sync(0xFFFFFFFFu, tok, k), __shfl_sync(0xFFFFFFFFu, head, k), __shfl_sync(0xFFFFFFFFu, keys, k));
+                    attn_row_again(p, FP8, seq, seq_row0 + __shfl_sync(0xFFFFFFFFu, tok, k), __shfl_sync(0xFFFFFFFFu, head, k), __shfl_sync(0xFFFFFFFFu, keys, k));
                 }
             }
             tcgen05_fence_before();                                          // O has been read before the next item's P is handed over
         }
     } else if constexpr (FP8) {
         // ---- raw tiles to FP16 ones ----
-        if constexpr (C::AUX_REGS < C::LAUNCH_REGS) regs_down<C::AUX_REGS>();
         const uint32_t t = tid - 32u * C::CONV_WARP0;
-        uint32_t rs = 0, rph = 0, st[2] = {0, 0}, ph[2] = {0, 0};
+        uint32_t rs = 0, rph = 0, slot = 0, ph = 0;
         bool ok = true;
         while (ok && walk.next(p)) {
             const uint32_t n = tiles_wanted(), kv_len = walk.sq.kv_len;
@@ -496,9 +545,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
                 for (int side = 0; side < 2; ++side) {
                     ok = ok && mbar_wait(RAW_FULL + 8 * rs, rph, abort_flag, STATUS_WAIT_EXPIRED_DEQUANT) &&
-                         mbar_wait((side ? V_EMPTY : K_EMPTY) + 8 * st[side], ph[side] ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_DEQUANT);
+                         mbar_wait(EMPTY + 8 * slot, ph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_DEQUANT);
                     if (!ok) break;
-                    const uint32_t raw = base + C::OFF_RAW + rs * C::RAW, to = base + (side ? C::OFF_V : C::OFF_K) + st[side] * C::TILE;
+                    const uint32_t raw = base + C::OFF_RAW + rs * C::RAW, to = base + C::OFF_KV + slot * C::TILE;
                     constexpr uint32_t CH = DP / 16;                         // 16-byte pieces of a raw row
 #pragma unroll 4
                     for (uint32_t i = 0; i < CH; ++i) {
@@ -519,10 +568,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         sts128(panel + sw128_off(r, c0 + 1u), h[4], h[5], h[6], h[7]);
                     }
                     fence_proxy_async();
-                    mbar_arrive((side ? V_FULL : K_FULL) + 8 * st[side]);
+                    mbar_arrive(FULL + 8 * slot);
                     mbar_arrive(RAW_EMPTY + 8 * rs);
                     if (++rs == uint32_t(C::RAW_STAGES)) { rs = 0; rph ^= 1u; }
-                    if (++st[side] == uint32_t(ST)) { st[side] = 0; ph[side] ^= 1u; }
+                    if (++slot == uint32_t(SLOTS)) { slot = 0; ph ^= 1u; }
                 }
             }
         }

@@ -497,7 +497,7 @@ ATLAS_B200_API int32_t atlas_b200_registry_select_victim(const atlas_b200_regist
  *   kv_len       [n_seqs] i32: cached tokens, the new ones among them
  *   n_tokens     rows of q and out;  max_q_len, max_kv_len: no sequence has more (launch shapes go by them; more is computed all the
  *                same, only slower)
- *   ws           scratch of atlas_b200_paged_attention_ws_bytes(desc) bytes, 16-byte aligned, holding nothing between calls: calls
+ *   ws           scratch of atlas_b200_paged_attention_ws_bytes(desc) bytes, 32-byte aligned, holding nothing between calls: calls
  *                that may overlap on the GPU need one each.  NULL: no sequence's cache is split over several SMs, which is slow where
  *                there are few sequences.
  * head_dim a multiple of 32 up to 256, any group and block_size; scales positive and finite (-1).  n_pages * block_size and
