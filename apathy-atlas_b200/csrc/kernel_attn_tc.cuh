@@ -20,7 +20,7 @@
 // correction off the path of nearly every step.  (Exponentials by a polynomial on the FMA pipe for a quarter to a half of the scores,
 // the special-function unit being the busiest of the softmax: no faster.)
 //
-// Warps: 0 TMA, 1 MMA (converged, one lane issues), 2 tensor memory, 2 and 3 bring the next items' Q to L2; 4-7 and 8-11 softmax, epilogue and Q
+// Warps: 0 TMA, 1 and 3 MMA of a row tile each (converged, one lane issues), 2 tensor memory and the next items' Q to L2; 4-7 and 8-11 softmax, epilogue and Q
 // of a row tile each, the next item's Q before this one's output; E4M3 caches: 12-15 turn raw tiles into FP16 ones (one instruction for
 // two values, exact, NaN kept; Q as FP16 with a power of two per row, see the mma.sync form).  Every wait is bounded as elsewhere in the
 // library.
@@ -130,7 +130,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
 
     if (tid == 0) {
-        for (int i = 0; i < SLOTS; ++i) { mbar_init(FULL + 8 * i, FP8 ? 128 : 1); mbar_init(EMPTY + 8 * i, 1); }
+        for (int i = 0; i < SLOTS; ++i) { mbar_init(FULL + 8 * i, FP8 ? 128 : 1); mbar_init(EMPTY + 8 * i, NQ); }
         mbar_init(V_TAIL, 1);
         for (int g = 0; g < NQ; ++g) mbar_init(Q_FULL + 8 * g, 128);
         // Scores, weights and products of even and of odd steps have barriers of their own: whoever waits for one of step u knows that step
@@ -244,91 +244,89 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                 }
             }
-        } else if (warp == 1) {
-            // ---- MMA ----
+        } else if (warp == 1 || (NQ == 2 && warp == 3)) {
+            // ---- MMA of row tile 0 or 1: either warp waits for its own softmax only, and while it does the tensor cores have the other's work.
+            // (One warp for both, in turn: 2090 cycles a step, of which 700 went by between its waits and the next product.)
             constexpr uint32_t idesc_s = attn_idesc(TC_STEP, FP8, false), idesc_o = attn_idesc(DP, FP8, true);
-            uint32_t slot = 0, ph = 0, q_ph[2] = {0, 0}, p_ph[2][2] = {{0, 0}, {0, 0}};
+            const uint32_t g = warp >> 1, t_s = tmem + g * 128u, t_o = tmem + NQ * 128u + g * uint32_t(DP);
+            uint32_t slot = 0, ph = 0, q_ph = 0, p_ph[2] = {0, 0};
             bool ok = true;
             auto advance = [&] { if (++slot == uint32_t(SLOTS)) { slot = 0; ph ^= 1u; } };
-            auto scores = [&](uint32_t g, uint32_t h, uint32_t stage) {      // of half h of the key tile in `stage`
+            auto tile_there = [&] { return mbar_wait_warp(FULL + 8 * slot, ph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20); };
+            // (also for a tile that this row tile has no use for: it has been waited for, so the arrival is this round's)
+            auto release = [&](uint32_t which) {
+                if (elect_one()) umma_commit<false>(EMPTY + 8 * which);
+                __syncwarp();
+            };
+            auto scores = [&](uint32_t h) {                                  // of half h of the key tile in `slot`
                 if (elect_one()) {
-                    const uint64_t q = make_kmajor_sw128_desc(base + C::OFF_Q + g * C::TILE), k = make_kmajor_sw128_desc(base + C::OFF_KV + stage * C::TILE + h * (TC_STEP * 128u));
+                    const uint64_t q = make_kmajor_sw128_desc(base + C::OFF_Q + g * C::TILE), k = make_kmajor_sw128_desc(base + C::OFF_KV + slot * C::TILE + h * (TC_STEP * 128u));
 #pragma unroll
                     for (int s = 0; s < DP / 16; ++s)
-                        umma_bf16_ss<false>(tmem + g * 128u + h * TC_STEP, q + (s >> 2) * (C::PANEL >> 4) + (s & 3) * 2, k + (s >> 2) * (C::PANEL >> 4) + (s & 3) * 2, idesc_s, s ? 1u : 0u);
+                        umma_bf16_ss<false>(t_s + h * TC_STEP, q + (s >> 2) * (C::PANEL >> 4) + (s & 3) * 2, k + (s >> 2) * (C::PANEL >> 4) + (s & 3) * 2, idesc_s, s ? 1u : 0u);
                     umma_commit<false>(S_FULL + 8 * (2 * g + h));
                 }
                 __syncwarp();
             };
             while (ok && walk.next(p)) {
-                const uint32_t n_g[2] = {steps_of(0), NQ == 2 ? steps_of(NQ - 1) : 0u}, n = max(n_g[0], n_g[1]);
+                const uint32_t mine = steps_of(g), n = 2u * tiles_wanted();
                 if (n == 0) continue;
-                ok = mbar_wait_warp(FULL + 8 * slot, ph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
+                ok = tile_there();
+                if (ok && mine) ok = mbar_wait_warp(Q_FULL + 8 * g, q_ph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
                 if (!ok) break;
-#pragma unroll
-                for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-                    for (uint32_t g = 0; g < uint32_t(NQ); ++g) {
-                        if (h >= n_g[g]) continue;
-                        if (h == 0) {
-                            ok = ok && mbar_wait_warp(Q_FULL + 8 * g, q_ph[g], abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
-                            q_ph[g] ^= 1u;
-                        }
-                        if (!ok) break;
-                        tcgen05_fence_after();
-                        scores(g, h, slot);
-                    }
-                if (!ok) break;
-                if (elect_one()) umma_commit<false>(EMPTY + 8 * slot);
-                __syncwarp();
+                if (mine) {
+                    q_ph ^= 1u;
+                    tcgen05_fence_after();
+                    scores(0);
+                    if (mine > 1) scores(1);
+                }
+                release(slot);
                 advance();
                 for (uint32_t u0 = 0; ok && u0 < n; u0 += 2) {
-                    ok = mbar_wait_warp(FULL + 8 * slot, ph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
+                    ok = tile_there();
                     if (!ok) break;
                     const uint32_t v_slot = slot, vd = base + C::OFF_KV + slot * C::TILE;
-                    const uint32_t last_h = u0 + 1 < n ? 1u : 0u, last_g = NQ == 2 && u0 + last_h < n_g[1] ? 1u : 0u;   // the last to read V
                     bool k_there = false;
                     advance();
+                    if (u0 >= mine) release(v_slot);
 #pragma unroll
                     for (uint32_t h = 0; h < 2; ++h) {
+                        const uint32_t u = u0 + h;
+                        if (!ok || u >= mine) continue;
+                        ok = mbar_wait_warp(P_FULL + 8 * (2 * g + h), p_ph[h], abort_flag, STATUS_WAIT_EXPIRED_MMA);
+                        if (!ok) continue;
+                        p_ph[h] ^= 1u;
+                        tcgen05_fence_after();
+                        if (elect_one()) {
+                            const uint64_t v = make_mnmajor_sw128_desc(vd + h * (TC_STEP * 128u), C::PANEL);
 #pragma unroll
-                        for (uint32_t g = 0; g < uint32_t(NQ); ++g) {
-                            const uint32_t u = u0 + h;
-                            if (!ok || u >= n_g[g]) continue;
-                            ok = mbar_wait_warp(P_FULL + 8 * (2 * g + h), p_ph[g][h], abort_flag, STATUS_WAIT_EXPIRED_MMA);
+                            for (int s = 0; s < int(TC_STEP) / 16; ++s)
+                                umma_bf16_ts<false>(t_o, t_s + h * TC_STEP + s * 8u, v + s * (2048 >> 4), idesc_o, (u | s) ? 1u : 0u);
+                            umma_commit<false>(PV_DONE + 8 * (2 * g + h));
+                            if (h == 1 || u + 1 == mine) umma_commit<false>(EMPTY + 8 * v_slot);
+                        }
+                        __syncwarp();
+                        if (u + 2 < mine) {
+                            if (!k_there) ok = tile_there();
                             if (!ok) continue;
-                            p_ph[g][h] ^= 1u;
-                            tcgen05_fence_after();
-                            if (elect_one()) {
-                                const uint64_t v = make_mnmajor_sw128_desc(vd + h * (TC_STEP * 128u), C::PANEL);
-#pragma unroll
-                                for (int s = 0; s < int(TC_STEP) / 16; ++s)
-                                    umma_bf16_ts<false>(tmem + NQ * 128u + g * uint32_t(DP), tmem + g * 128u + h * TC_STEP + s * 8u, v + s * (2048 >> 4), idesc_o, (u | s) ? 1u : 0u);
-                                umma_commit<false>(PV_DONE + 8 * (2 * g + h));
-                                if (h == last_h && g == last_g) umma_commit<false>(EMPTY + 8 * v_slot);
-                            }
-                            __syncwarp();
-                            if (u + 2 < n_g[g]) {
-                                if (!k_there) ok = mbar_wait_warp(FULL + 8 * slot, ph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
-                                if (!ok) continue;
-                                k_there = true;
-                                scores(g, h, slot);
-                            }
+                            k_there = true;
+                            scores(h);
                         }
                     }
                     if (ok && u0 + 2 < n) {
-                        if (elect_one()) umma_commit<false>(EMPTY + 8 * slot);
-                        __syncwarp();
+                        if (!k_there) ok = tile_there();
+                        if (!ok) break;
+                        release(slot);
                         advance();
                     }
                 }
             }
         } else {
             // ---- Q of the items ahead to L2, so that its rows' latency is that of L2 when their turn comes ----
-            const uint32_t t = (warp - 2) * 32u + lane;
+            const uint32_t t = NQ == 2 ? lane : (warp - 2) * 32u + lane, all = NQ == 2 ? 32u : 64u;
             while (walk.next(p)) {
                 const uint32_t row0 = walk.at.block * C::ROWS, rows = tile_rows(0) + (NQ == 2 ? tile_rows(NQ - 1) : 0u), lines = (p.head_dim * 2u + 127u) / 128u;
-                for (uint32_t i = t; i < rows * lines; i += 64u) {
+                for (uint32_t i = t; i < rows * lines; i += all) {
                     const uint32_t row = row0 + i / lines, tok = row / p.group;
                     const uint16_t* at = p.q + size_t(walk.sq.row0 + tok) * p.q_row_stride + size_t(walk.at.head * p.group + row - tok * p.group) * p.head_dim + (i % lines) * 64u;
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
