@@ -67,6 +67,10 @@ int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, c
 // ---------------------------------------------------------------------------------------------
 thread_local uint32_t t_attn_shape[4] = {0, 0, 0, 0};
 
+// room for a cut of every range: more than any GPU this library runs on has SMs, twice
+constexpr size_t ATTN_CUT_BYTES = 512 * sizeof(AttnCut);
+constexpr uint32_t ATTN_MAX_CTAS = 512;
+
 uint32_t attn_dim(uint32_t head_dim) { return head_dim <= 64 ? 64u : head_dim <= 128 ? 128u : 256u; }
 
 int check_attention(const atlas_b200_attention_desc& d) {
@@ -98,7 +102,8 @@ AttnParams attention_params(const atlas_b200_attention_desc& d) {
     p.k_cache = static_cast<const uint8_t*>(d.k_cache);
     p.v_cache = static_cast<const uint8_t*>(d.v_cache);
     p.block_table = d.block_table; p.cu_q = d.cu_q; p.kv_len = d.kv_len;
-    p.parts = static_cast<float*>(d.ws);
+    p.cuts = static_cast<AttnCut*>(d.ws);
+    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(d.ws) + ATTN_CUT_BYTES);
     p.n_seqs = d.n_seqs; p.n_tokens = d.n_tokens; p.n_pages = d.n_pages; p.table_stride = d.table_stride;
     p.q_heads = d.q_heads; p.kv_heads = d.kv_heads; p.head_dim = d.head_dim; p.block_size = d.block_size; p.group = d.q_heads / d.kv_heads;
     p.q_row_stride = d.q_row_stride; p.out_row_stride = d.out_row_stride;
@@ -120,7 +125,7 @@ struct MmaPlan {
 };
 MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms) {
     const uint32_t dim = attn_dim(d.head_dim);
-    const uint32_t resident = sms * (dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u) >= 512u ? 1u : 2u);
+    const uint32_t resident = std::min(sms, ATTN_MAX_CTAS / 2) * (dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u) >= 512u ? 1u : 2u);
     const uint64_t group = d.q_heads / d.kv_heads;
     const uint64_t rows = std::min<uint64_t>(d.max_q_len, d.n_tokens) * group;
     const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * std::max<uint64_t>((rows + attn::MMA_ROWS - 1) / attn::MMA_ROWS, 1);
@@ -130,7 +135,7 @@ MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms) {
     r.least = r.by_item ? 1u : 4u;
     const uint64_t places = r.by_item ? items : (items * (tiles + MMA_EXTRA) + r.least - 1) / r.least;
     r.ctas = uint32_t(std::min<uint64_t>(resident, std::max<uint64_t>(places, 1)));
-    r.ws_bytes = r.by_item ? 0 : size_t(resident) * 2 * attn_part_floats(attn::MMA_ROWS, dim) * sizeof(float);
+    r.ws_bytes = r.by_item ? 0 : ATTN_CUT_BYTES + size_t(resident) * 2 * attn_part_floats(attn::MMA_ROWS, dim) * sizeof(float);
     return r;
 }
 
@@ -142,7 +147,7 @@ template <int DP, bool FP8> int launch_mma(AttnParams p, const MmaPlan& plan, cu
     p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.extra = MMA_EXTRA;
     const int rc2 = launch_dependent(attn::attn_mma_kernel<DP, FP8>, plan.ctas, attn::MMA_THREADS, C::SMEM, st, p, attn_divisor(p.block_size));
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
-    return launch_dependent(attn_join_kernel<attn::MMA_ROWS, attn::MMA_TILE, DP, FP8>, plan.ctas - 1, ATTN_JOIN_THREADS, 0, st, p);
+    return launch_dependent(attn_join_kernel<attn::MMA_ROWS, DP, FP8>, dim3(plan.ctas - 1, attn::MMA_ROWS / ATTN_JOIN_ROWS), ATTN_JOIN_THREADS, 0, st, p);
 }
 
 // The tcgen05 form.  It reads pages in boxes of the largest power of two that divides page and tile, at least a swizzle atom's eight rows,
@@ -161,6 +166,7 @@ bool takes_tc(const atlas_b200_attention_desc& d) {
     return rows > 32 && tc_box_rows(d.block_size) >= 8 && aligned(d.q, 16) && aligned(d.out, 16) && d.q_row_stride % 8 == 0 && d.out_row_stride % 8 == 0;
 }
 TcPlan plan_tc(const atlas_b200_attention_desc& d, uint32_t sms) {
+    sms = std::min(sms, ATTN_MAX_CTAS);
     const uint32_t dim = attn_dim(d.head_dim), block_rows = dim <= 128 ? 256u : 128u;
     const uint64_t rows = uint64_t(std::min(d.max_q_len, d.n_tokens)) * (d.q_heads / d.kv_heads);
     const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * ((rows + block_rows - 1) / block_rows);
@@ -171,7 +177,7 @@ TcPlan plan_tc(const atlas_b200_attention_desc& d, uint32_t sms) {
     r.least = r.by_item ? 1u : 2u;
     const uint64_t places = r.by_item ? items : (items * (tiles + TC_EXTRA) + r.least - 1) / r.least;
     r.ctas = uint32_t(std::min<uint64_t>(sms, std::max<uint64_t>(places, 1)));
-    r.ws_bytes = r.by_item ? 0 : size_t(sms) * 2 * attn_part_floats(block_rows, dim) * sizeof(float);
+    r.ws_bytes = r.by_item ? 0 : ATTN_CUT_BYTES + size_t(sms) * 2 * attn_part_floats(block_rows, dim) * sizeof(float);
     return r;
 }
 
@@ -192,7 +198,7 @@ template <int DP, bool FP8> int launch_tc(AttnParams p, const TcPlan& plan, cuda
     p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.extra = TC_EXTRA;
     const int rc2 = launch_dependent(attn::attn_tc_kernel<DP, FP8>, plan.ctas, C::THREADS, C::SMEM, st, map_k, map_v, p, plan.box_rows);
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
-    return launch_dependent(attn_join_kernel<C::ROWS, int(attn::TC_KEYS), DP, FP8>, dim3(plan.ctas - 1, C::ROWS / ATTN_JOIN_ROWS), ATTN_JOIN_THREADS, 0, st, p);
+    return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, C::ROWS / ATTN_JOIN_ROWS), ATTN_JOIN_THREADS, 0, st, p);
 }
 
 int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {

@@ -85,6 +85,10 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
         return x < x_end ? x : ~0ull;
     });
     AttnWalk walk(p, f, x, x_end, MMA_ROWS, MMA_TILE);
+    if (tid == 0 && !p.by_item) {
+        if (x < x_end) walk.note_cut(p, f, x);
+        else p.cuts[blockIdx.x].pieces = 0;                                  // more CTAs than ranges
+    }
     while (walk.next(p)) {
         const AttnSeqAt sq = walk.sq;
         const AttnPlace at = walk.at;

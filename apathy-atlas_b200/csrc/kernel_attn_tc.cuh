@@ -157,6 +157,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         return x < x_end ? x : ~0ull;
     });
     AttnWalk walk(p, found, x, x_end, C::ROWS, TC_KEYS);
+    if (tid == 64 && !p.by_item) {
+        if (x < x_end) walk.note_cut(p, found, x);
+        else p.cuts[blockIdx.x].pieces = 0;                                  // more CTAs than ranges
+    }
     // rows of a row tile of the item, and the steps that it takes of the piece
     auto tile_rows = [&](uint32_t g) {
         const uint32_t all = walk.sq.q_len * p.group, r0 = walk.at.block * C::ROWS + g * TC_TILE_ROWS;
