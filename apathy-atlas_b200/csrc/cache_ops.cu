@@ -120,17 +120,18 @@ constexpr uint32_t MMA_EXTRA = MMA_EXTRA_, TC_EXTRA = TC_EXTRA_;
 
 // The mma.sync form: how many CTAs, and whether each takes whole items.
 struct MmaPlan {
-    uint32_t ctas, by_item, least;
+    uint32_t ctas, by_item, least, tile;
     size_t ws_bytes;
 };
 MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms) {
     const uint32_t dim = attn_dim(d.head_dim);
-    const uint32_t resident = std::min(sms, ATTN_MAX_CTAS / 2) * (dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u) >= 512u ? 1u : 2u);
+    const uint32_t row_bytes = dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u), resident = std::min(sms, ATTN_MAX_CTAS / 2) * (row_bytes >= 512u ? 1u : 2u);
     const uint64_t group = d.q_heads / d.kv_heads;
     const uint64_t rows = std::min<uint64_t>(d.max_q_len, d.n_tokens) * group;
     const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * std::max<uint64_t>((rows + attn::MMA_ROWS - 1) / attn::MMA_ROWS, 1);
-    const uint64_t tiles = std::max<uint64_t>((uint64_t(d.max_kv_len) + attn::MMA_TILE - 1) / attn::MMA_TILE, 1);
     MmaPlan r{};
+    r.tile = uint32_t(attn::MMA_WARPS) * (row_bytes <= 128u ? 32u : 16u);
+    const uint64_t tiles = std::max<uint64_t>((uint64_t(d.max_kv_len) + r.tile - 1) / r.tile, 1);
     r.by_item = tiles <= 4;
     r.least = r.by_item ? 1u : 4u;
     const uint64_t places = r.by_item ? items : (items * (tiles + MMA_EXTRA) + r.least - 1) / r.least;
@@ -223,7 +224,7 @@ int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
     if (!d.ws && !plan.by_item) { plan.by_item = 1; plan.least = 1; }        // (no scratch: nothing is cut)
     const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3;
     const AttnParams p = attention_params(d);
-    t_attn_shape[0] = attn::MMA_ROWS; t_attn_shape[1] = plan.ctas; t_attn_shape[2] = plan.by_item; t_attn_shape[3] = attn::MMA_TILE;
+    t_attn_shape[0] = attn::MMA_ROWS; t_attn_shape[1] = plan.ctas; t_attn_shape[2] = plan.by_item; t_attn_shape[3] = plan.tile;
     if (dim == 64) return fp8 ? launch_mma<64, true>(p, plan, st) : launch_mma<64, false>(p, plan, st);
     if (dim == 128) return fp8 ? launch_mma<128, true>(p, plan, st) : launch_mma<128, false>(p, plan, st);
     return fp8 ? launch_mma<256, true>(p, plan, st) : launch_mma<256, false>(p, plan, st);

@@ -2,7 +2,7 @@
 //
 // What bounds it is the cache: per KV head and token 2 head_dim values are read for 4 head_dim operations a row, and a KV head has
 // `group` rows a token.  So a block is 16 rows (the M of mma.sync.m16n8k16, most of them empty in a decode step, which costs nothing),
-// every warp has sixteen tokens' K and V of its own in flight through a private ring in shared memory (cp.async, 16 bytes a lane: a row
+// every warp has units of sixteen tokens' K and V (32 where rows are short) of its own in flight through a private ring in shared memory (cp.async, 16 bytes a lane: a row
 // of the cache is wherever its page is, so any page size will do and places behind a sequence's end are filled with zeros), and no warp
 // waits for another until the range's item ends: then the warps' maxima, sums and outputs are joined in shared memory.
 //
@@ -17,11 +17,13 @@
 namespace atlas {
 namespace attn {
 
-constexpr int MMA_WARPS = 4, MMA_THREADS = 32 * MMA_WARPS, MMA_ROWS = 16, MMA_UNIT = 16, MMA_TILE = MMA_UNIT * MMA_WARPS;
+constexpr int MMA_WARPS = 4, MMA_THREADS = 32 * MMA_WARPS, MMA_ROWS = 16;
 
 template <int DP, bool FP8> struct MmaCfg {
     static constexpr int ROW_BYTES = DP * (FP8 ? 1 : 2);
-    static constexpr int SIDE = MMA_UNIT * ROW_BYTES;                        // K or V of a unit
+    // Tokens of a unit.  A unit is a chain (copy, scores, maximum, weights, product) of some 1500 cycles whatever its bytes.
+    static constexpr int UNIT = ROW_BYTES <= 128 ? 32 : 16, TILE = UNIT * MMA_WARPS;
+    static constexpr int SIDE = UNIT * ROW_BYTES;                            // K or V of a unit
     // two CTAs on an SM (one where a row is 512 bytes), the ring as deep as that leaves room for
     static constexpr int CTAS = ROW_BYTES >= 512 ? 1 : 2;
     static constexpr int STAGES = (ROW_BYTES >= 512 ? 196608 : 98304) / MMA_WARPS / (2 * SIDE) > 8 ? 8 : (ROW_BYTES >= 512 ? 196608 : 98304) / MMA_WARPS / (2 * SIDE);
@@ -79,12 +81,12 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
     pdl_release();
 
     uint64_t x = 0, x_end = 0;
-    const AttnFound f = attn_find<MMA_THREADS>(p, MMA_ROWS, MMA_TILE, sh, [&](uint64_t total) {
+    const AttnFound f = attn_find<MMA_THREADS>(p, MMA_ROWS, C::TILE, sh, [&](uint64_t total) {
         const uint32_t n = attn_ranges(total, p.ctas, p.least_tiles);
         if (blockIdx.x < n) { x = attn_range_begin(total, n, blockIdx.x); x_end = attn_range_begin(total, n, blockIdx.x + 1); }
         return x < x_end ? x : ~0ull;
     });
-    AttnWalk walk(p, f, x, x_end, MMA_ROWS, MMA_TILE);
+    AttnWalk walk(p, f, x, x_end, MMA_ROWS, C::TILE);
     if (tid == 0 && !p.by_item) {
         if (x < x_end) walk.note_cut(p, f, x);
         else p.cuts[blockIdx.x].pieces = 0;                                  // more CTAs than ranges
@@ -108,12 +110,12 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
         const uint32_t last_tok = (at.block * MMA_ROWS + rows - 1) / p.group, first_tok = at.block * MMA_ROWS / p.group;
         const uint32_t all_see = attn_row_keys(sq, first_tok), n_keys = attn_row_keys(sq, last_tok);
 
-        // the cache rows of a unit: lane l < 16 finds that of token l
+        // the cache rows of a unit: lane l finds that of token l
         const int32_t* table = p.block_table + size_t(seq) * p.table_stride;
-        const uint32_t units = t1 - t0, pos_w = t0 * MMA_TILE + warp * MMA_UNIT;
+        const uint32_t units = t1 - t0, pos_w = t0 * C::TILE + warp * C::UNIT;
         auto find_row = [&](uint32_t u) -> int32_t {
-            const uint32_t pos = pos_w + u * MMA_TILE + (lane & 15u);
-            return u < units && lane < 16u && pos < n_keys ? attn_cache_row(p, div, table, pos) : -1;
+            const uint32_t pos = pos_w + u * C::TILE + lane;
+            return u < units && lane < uint32_t(C::UNIT) && pos < n_keys ? attn_cache_row(p, div, table, pos) : -1;
         };
         constexpr uint32_t CH = C::ROW_BYTES / 16;                      // 16-byte chunks of a row
         const size_t head_at = size_t(at.head) * D * size, row_bytes = size_t(p.kv_heads) * D * size;
@@ -121,7 +123,7 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
             if (u < units) {
                 const uint32_t dst = ring + (u % C::STAGES) * (2 * C::SIDE);
 #pragma unroll
-                for (uint32_t i = 0; i < uint32_t(MMA_UNIT) * CH / 32; ++i) {
+                for (uint32_t i = 0; i < uint32_t(C::UNIT) * CH / 32; ++i) {
                     const uint32_t idx = i * 32u + lane, t = idx / CH, c = idx % CH;
                     const int32_t r = __shfl_sync(0xFFFFFFFFu, row, t);
                     const bool there = r >= 0 && c * 16u < D * size;
@@ -183,98 +185,110 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
             row_next = find_row(u + C::STAGES);
             asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
             __syncwarp();
-            const uint32_t pos0 = pos_w + u * MMA_TILE;
+            const uint32_t pos0 = pos_w + u * C::TILE;
             if (pos0 < n_keys) {                                             // (the same for the whole warp)
                 const uint32_t ks = ring + (u % C::STAGES) * (2 * C::SIDE), vs = ks + C::SIDE;
-                float s[2][4] = {};
+                float s[C::UNIT / 8][4] = {};
                 if constexpr (!FP8) {
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) {
-                        uint32_t b[4];
-                        ldsm4(b, ks + unit_off<C::ROW_BYTES>(((lane >> 4) << 3) + (lane & 7u), 2u * k + ((lane >> 3) & 1u)));
-                        mma16816<false>(s[0], qa[k], b[0], b[1]);
-                        mma16816<false>(s[1], qa[k], b[2], b[3]);
-                    }
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int n = 0; n < C::UNIT / 8; n += 2) {
+                            uint32_t b[4];
+                            ldsm4(b, ks + unit_off<C::ROW_BYTES>(8u * n + ((lane >> 4) << 3) + (lane & 7u), 2u * k + ((lane >> 3) & 1u)));
+                            mma16816<false>(s[n], qa[k], b[0], b[1]);
+                            mma16816<false>(s[n + 1], qa[k], b[2], b[3]);
+                        }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < DP / 64; ++j)
+                    for (int j = 0; j < DP / 64; ++j) {
+                        uint32_t w[C::UNIT / 8][4];
 #pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            uint32_t w[4];
-                            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                        for (int n = 0; n < C::UNIT / 8; ++n)
+                            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[n][0]), "=r"(w[n][1]), "=r"(w[n][2]), "=r"(w[n][3])
                                          : "r"(ks + unit_off<C::ROW_BYTES>(8u * n + g, 4u * j + q4)));
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) mma16816<true>(s[n], qa[4 * j + k], e4m3x2_to_f16x2(w[k]), e4m3x2_to_f16x2(w[k] >> 16));
-                        }
+                        for (int k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int n = 0; n < C::UNIT / 8; ++n) mma16816<true>(s[n], qa[4 * j + k], e4m3x2_to_f16x2(w[n][k]), e4m3x2_to_f16x2(w[n][k] >> 16));
+                    }
                 }
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < C::UNIT / 8; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[n][e] *= c_row[e >> 1];
-                if (pos0 + MMA_UNIT > all_see) {
+                if (pos0 + C::UNIT > all_see) {
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int n = 0; n < C::UNIT / 8; ++n)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if (pos0 + 8u * n + 2u * q4 + (e & 1) >= keys[e >> 1]) s[n][e] = -INFINITY;
                 }
-                uint32_t pa[4];
+                uint32_t pa[C::UNIT / 16][4];
                 float keep[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float top = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+                    float top = m[i];
+#pragma unroll
+                    for (int n = 0; n < C::UNIT / 8; ++n) top = fmaxf(fmaxf(top, s[n][2 * i]), s[n][2 * i + 1]);
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                    top = fmaxf(top, m[i]);
                     const float base = top == -INFINITY ? 0.0f : top;
                     keep[i] = exp2f(m[i] - base);
                     m[i] = top;
-                    const float p0 = exp2f(s[0][2 * i] - base), p1 = exp2f(s[0][2 * i + 1] - base), p2 = exp2f(s[1][2 * i] - base), p3 = exp2f(s[1][2 * i + 1] - base);
-                    l[i] = l[i] * keep[i] + ((p0 + p1) + (p2 + p3));
-                    pa[i] = pack2<FP8>(p0, p1);
-                    pa[2 + i] = pack2<FP8>(p2, p3);
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < C::UNIT / 8; ++n) {
+                        const float p0 = exp2f(s[n][2 * i] - base), p1 = exp2f(s[n][2 * i + 1] - base);
+                        sum += p0 + p1;
+                        pa[n >> 1][2 * (n & 1) + i] = pack2<FP8>(p0, p1);
+                    }
+                    l[i] = l[i] * keep[i] + sum;
                 }
                 if (__any_sync(0xFFFFFFFFu, keep[0] != 1.0f || keep[1] != 1.0f)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) { o[n][0] *= keep[0]; o[n][1] *= keep[0]; o[n][2] *= keep[1]; o[n][3] *= keep[1]; }
                 }
-                if constexpr (!FP8) {
 #pragma unroll
-                    for (int n = 0; n < NT; n += 2) {
-                        uint32_t b[4];
-                        ldsm4_trans(b, vs + unit_off<C::ROW_BYTES>((((lane >> 3) & 1u) << 3) + (lane & 7u), n + (lane >> 4)));
-                        mma16816<false>(o[n], pa, b[0], b[1]);
-                        mma16816<false>(o[n + 1], pa, b[2], b[3]);
-                    }
-                } else {
-                    // lane g has the channels W g .. W g + W - 1 (of each 128) of tokens 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9; n tile i is
-                    // channel i of every lane's
-                    constexpr int W = DP < 128 ? 8 : 16;
+                for (int kk = 0; kk < C::UNIT / 16; ++kk) {                  // sixteen tokens a product
+                    if constexpr (!FP8) {
 #pragma unroll
-                    for (int h = 0; h < (DP + 127) / 128; ++h) {
-                        uint32_t v[4][W / 4];
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            const uint32_t tok = 2u * q4 + (t & 1) + 8u * (t >> 1);
-                            if constexpr (W == 16) {
-                                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[t][0]), "=r"(v[t][1]), "=r"(v[t][2]), "=r"(v[t][3])
-                                             : "r"(vs + unit_off<C::ROW_BYTES>(tok, 8u * h + g)));
-                            } else {
-                                asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[t][0]), "=r"(v[t][1])
-                                             : "r"(vs + unit_off<C::ROW_BYTES>(tok, g >> 1) + 8u * (g & 1u)));
-                            }
+                        for (int n = 0; n < NT; n += 2) {
+                            uint32_t b[4];
+                            ldsm4_trans(b, vs + unit_off<C::ROW_BYTES>(16u * kk + (((lane >> 3) & 1u) << 3) + (lane & 7u), n + (lane >> 4)));
+                            mma16816<false>(o[n], pa[kk], b[0], b[1]);
+                            mma16816<false>(o[n + 1], pa[kk], b[2], b[3]);
                         }
+                    } else {
+                        // lane g has the channels W g .. W g + W - 1 (of each 128) of tokens 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9; n tile i is
+                        // channel i of every lane's
+                        constexpr int W = DP < 128 ? 8 : 16;
 #pragma unroll
-                        for (int w = 0; w < W / 4; ++w)
+                        for (int h = 0; h < (DP + 127) / 128; ++h) {
+                            uint32_t v[4][W / 4];
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {                    // channels 4 w + 2 e and the next one
-                                uint32_t t[4];
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) t[k] = e4m3x2_to_f16x2(v[k][w] >> (16 * e));
-                                const int n = h * W + 4 * w + 2 * e;
-                                mma16816<true>(o[n], pa, prmt(t[0], t[1], 0x5410u), prmt(t[2], t[3], 0x5410u));
-                                mma16816<true>(o[n + 1], pa, prmt(t[0], t[1], 0x7632u), prmt(t[2], t[3], 0x7632u));
+                            for (int t = 0; t < 4; ++t) {
+                                const uint32_t tok = 16u * kk + 2u * q4 + (t & 1) + 8u * (t >> 1);
+                                if constexpr (W == 16) {
+                                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[t][0]), "=r"(v[t][1]), "=r"(v[t][2]), "=r"(v[t][3])
+                                                 : "r"(vs + unit_off<C::ROW_BYTES>(tok, 8u * h + g)));
+                                } else {
+                                    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[t][0]), "=r"(v[t][1])
+                                                 : "r"(vs + unit_off<C::ROW_BYTES>(tok, g >> 1) + 8u * (g & 1u)));
+                                }
                             }
+#pragma unroll
+                            for (int w = 0; w < W / 4; ++w)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {                // channels 4 w + 2 e and the next one
+                                    uint32_t t[4];
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) t[k] = e4m3x2_to_f16x2(v[k][w] >> (16 * e));
+                                    const int n = h * W + 4 * w + 2 * e;
+                                    mma16816<true>(o[n], pa[kk], prmt(t[0], t[1], 0x5410u), prmt(t[2], t[3], 0x5410u));
+                                    mma16816<true>(o[n + 1], pa[kk], prmt(t[0], t[1], 0x7632u), prmt(t[2], t[3], 0x7632u));
+                                }
+                        }
                     }
                 }
             }
