@@ -237,14 +237,19 @@ static __device__ __noinline__ void attn_row_again(const AttnParams& p, bool fp8
 // ------------------------------------------------------------------------------------------------------------------
 // Joins the pieces of items that were cut.  CTA (c, y) looks at the cut between ranges c and c + 1; the first cut of an item joins it, each
 // y some of its rows.  A piece's slot: 2 c for the item that range c begins inside, 2 c + 1 for one that begins in range c and goes on.
+// Up to ATTN_JOIN_FEW pieces a warp takes a row; beyond (few sequences over a long cache: as many pieces as CTAs) the warps share a row's
+// pieces and add their sums in the order of the warps.
 // (With the item's place worked out here, from the lengths, the join took as long as a sixth of the attention of 512 tokens over 32768:
 // 50 us of 280.)
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int ATTN_JOIN_THREADS = 128, ATTN_JOIN_ROWS = 8;
+constexpr int ATTN_JOIN_WARPS = 4, ATTN_JOIN_THREADS = 32 * ATTN_JOIN_WARPS;
+constexpr uint32_t ATTN_JOIN_FEW = 8;
+constexpr int attn_join_ctas(int block_rows) { return block_rows <= 16 ? 8 : block_rows / 8; }   // grid y
 
 template <int ROWS, int DP, bool FP8>
 __global__ void __launch_bounds__(ATTN_JOIN_THREADS) attn_join_kernel(const __grid_constant__ AttnParams p) {
     constexpr int V = DP / 32;                                               // channels of a lane, side by side
+    __shared__ float o_s[ATTN_JOIN_WARPS][DP];
     pdl_wait();
     pdl_release();
     const uint32_t c = blockIdx.x + 1;
@@ -255,25 +260,49 @@ __global__ void __launch_bounds__(ATTN_JOIN_THREADS) attn_join_kernel(const __gr
     const size_t part = attn_part_floats(ROWS, DP);
     const float* const first = p.parts + part * (2 * size_t(c - 1) + 1);     // piece 0; piece i > 0 lies in slot 2 (c - 1 + i)
     auto piece = [&](uint32_t i) { return i == 0 ? first : p.parts + part * (2 * size_t(c - 1 + i)); };
-    const uint32_t lane = threadIdx.x & 31u;
-    for (uint32_t r = blockIdx.y * (ATTN_JOIN_THREADS / 32) + (threadIdx.x >> 5); r < rows; r += gridDim.y * (ATTN_JOIN_THREADS / 32)) {
-        float m = -INFINITY;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const bool few = cut.pieces <= ATTN_JOIN_FEW;
+    const uint32_t begin = few ? 0u : warp, step = few ? 1u : uint32_t(ATTN_JOIN_WARPS);
+    for (uint32_t r = few ? blockIdx.y * ATTN_JOIN_WARPS + warp : blockIdx.y; r < rows; r += gridDim.y * (few ? ATTN_JOIN_WARPS : 1)) {
+        float m = -INFINITY, l = 0.0f;
         for (uint32_t i = lane; i < cut.pieces; i += 32) m = fmaxf(m, piece(i)[size_t(ROWS) * DP + r]);
         for (uint32_t x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
         const float base = m == -INFINITY ? 0.0f : m;
-        float o[V] = {}, l = 0.0f;
-#pragma unroll 4
-        for (uint32_t i = 0; i < cut.pieces; ++i) {
-            const float* s = piece(i);
-            const float w = exp2f(s[size_t(ROWS) * DP + r] - base);
-            l += w * s[size_t(ROWS) * DP + ROWS + r];
-            float v[V];
-            if constexpr (V == 2) *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(s + size_t(r) * DP + lane * V);
-            else
+        float o[V] = {};
+        for (uint32_t i0 = 0; i0 < cut.pieces; i0 += 32) {                   // lane l: the weight of piece i0 + l
+            float w_mine = 0.0f;
+            if (i0 + lane < cut.pieces) {
+                const float* s = piece(i0 + lane) + size_t(ROWS) * DP;
+                w_mine = exp2f(s[r] - base);
+                l += w_mine * s[ROWS + r];
+            }
+            const uint32_t n = min(cut.pieces - i0, 32u);
+#pragma unroll 8
+            for (uint32_t i = begin; i < n; i += step) {
+                const float w = __shfl_sync(0xFFFFFFFFu, w_mine, i);
+                const float* s = piece(i0 + i) + size_t(r) * DP + lane * V;
+                float v[V];
+                if constexpr (V == 2) *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(s);
+                else
 #pragma unroll
-                for (int k = 0; k < V; k += 4) *reinterpret_cast<float4*>(v + k) = *reinterpret_cast<const float4*>(s + size_t(r) * DP + lane * V + k);
+                    for (int k = 0; k < V; k += 4) *reinterpret_cast<float4*>(v + k) = *reinterpret_cast<const float4*>(s + k);
 #pragma unroll
-            for (int k = 0; k < V; ++k) o[k] += w * v[k];
+                for (int k = 0; k < V; ++k) o[k] += w * v[k];
+            }
+        }
+        for (uint32_t x = 16; x; x >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
+        if (!few) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) o_s[warp][lane * V + k] = o[k];
+            __syncthreads();
+            if (warp == 0)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    o[k] = o_s[0][lane * V + k];
+                    for (int w = 1; w < ATTN_JOIN_WARPS; ++w) o[k] += o_s[w][lane * V + k];
+                }
+            __syncthreads();
+            if (warp != 0) continue;
         }
         const uint32_t row = cut.block * ROWS + r, in_seq = row / p.group, token = sq.row0 + in_seq, head = cut.head * p.group + row % p.group;
         const float inv = l == 0.0f ? 0.0f : p.v_scale / l;
