@@ -77,6 +77,13 @@ struct AttnCut {
     uint32_t seq, block, head;
 };
 
+// 2^x by the special-function unit; off by 2^-22 of the value at most, 0 below 2^-126
+__device__ __forceinline__ float attn_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // How many keys new token i of a sequence sees.
 __device__ __forceinline__ uint32_t attn_row_keys(const AttnSeqAt& s, uint32_t i) {
     const uint64_t n = uint64_t(s.kv_len) + i + 1;

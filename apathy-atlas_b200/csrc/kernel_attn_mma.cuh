@@ -213,10 +213,6 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
                             for (int n = 0; n < C::UNIT / 8; ++n) mma16816<true>(s[n], qa[4 * j + k], e4m3x2_to_f16x2(w[n][k]), e4m3x2_to_f16x2(w[n][k] >> 16));
                     }
                 }
-#pragma unroll
-                for (int n = 0; n < C::UNIT / 8; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[n][e] *= c_row[e >> 1];
                 if (pos0 + C::UNIT > all_see) {
 #pragma unroll
                     for (int n = 0; n < C::UNIT / 8; ++n)
@@ -228,18 +224,19 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
                 float keep[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float top = m[i];
+                    float top = -INFINITY;
 #pragma unroll
                     for (int n = 0; n < C::UNIT / 8; ++n) top = fmaxf(fmaxf(top, s[n][2 * i]), s[n][2 * i + 1]);
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                    top = fmaxf(top * c_row[i], m[i]);                       // (the factor is positive)
                     const float base = top == -INFINITY ? 0.0f : top;
-                    keep[i] = exp2f(m[i] - base);
+                    keep[i] = attn_exp2(m[i] - base);
                     m[i] = top;
                     float sum = 0.0f;
 #pragma unroll
                     for (int n = 0; n < C::UNIT / 8; ++n) {
-                        const float p0 = exp2f(s[n][2 * i] - base), p1 = exp2f(s[n][2 * i + 1] - base);
+                        const float p0 = attn_exp2(fmaf(s[n][2 * i], c_row[i], -base)), p1 = attn_exp2(fmaf(s[n][2 * i + 1], c_row[i], -base));
                         sum += p0 + p1;
                         pa[n >> 1][2 * (n & 1) + i] = pack2<FP8>(p0, p1);
                     }
@@ -280,13 +277,11 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
 #pragma unroll
                             for (int w = 0; w < W / 4; ++w)
 #pragma unroll
-                                for (int e = 0; e < 2; ++e) {                // channels 4 w + 2 e and the next one
-                                    uint32_t t[4];
-#pragma unroll
-                                    for (int k = 0; k < 4; ++k) t[k] = e4m3x2_to_f16x2(v[k][w] >> (16 * e));
+                                for (int e = 0; e < 2; ++e) {                // channels 4 w + 2 e and the next one: two tokens' bytes side by side, then converted
+                                    const uint32_t sel = e ? 0x7362u : 0x5140u, t0 = prmt(v[0][w], v[1][w], sel), t1 = prmt(v[2][w], v[3][w], sel);
                                     const int n = h * W + 4 * w + 2 * e;
-                                    mma16816<true>(o[n], pa[kk], prmt(t[0], t[1], 0x5410u), prmt(t[2], t[3], 0x5410u));
-                                    mma16816<true>(o[n + 1], pa[kk], prmt(t[0], t[1], 0x7632u), prmt(t[2], t[3], 0x7632u));
+                                    mma16816<true>(o[n], pa[kk], e4m3x2_to_f16x2(t0), e4m3x2_to_f16x2(t1));
+                                    mma16816<true>(o[n + 1], pa[kk], e4m3x2_to_f16x2(t0 >> 16), e4m3x2_to_f16x2(t1 >> 16));
                                 }
                         }
                     }

@@ -72,11 +72,6 @@ __device__ __forceinline__ void stg256(void* to, const uint32_t* r) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  ::"l"(to), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // Two FP32 values in one register pair and one issue slot.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
     uint64_t r;
@@ -436,7 +431,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     ok = __all_sync(0xFFFFFFFFu, mbar_wait(PV_DONE + 8 * (2 * g + (h ^ 1u)), s_ph[0] ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_EPILOGUE));
                     if (!ok) break;
                     tcgen05_fence_after();
-                    const float keep = grow ? ex2(m - top) : 1.0f;
+                    const float keep = grow ? attn_exp2(m - top) : 1.0f;
                     if (grow) m = top;
                     l *= keep;
 #pragma unroll 1
@@ -460,8 +455,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         const uint64_t x2 = fma2(pair_of(__uint_as_float(s[32 * k + 2 * v]), __uint_as_float(s[32 * k + 2 * v + 1])), c2, off2);
                         float e0, e1;
                         of_pair(x2, e0, e1);
-                        e0 = ex2(e0);
-                        e1 = ex2(e1);
+                        e0 = attn_exp2(e0);
+                        e1 = attn_exp2(e1);
                         sum[v & 1] = add2(sum[v & 1], pair_of(e0, e1));
                         w[v] = pack_pair<FP8>(e0, e1);
                     }
