@@ -148,7 +148,7 @@ template <int DP, bool FP8> int launch_mma(AttnParams p, const MmaPlan& plan, cu
     p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.extra = MMA_EXTRA;
     const int rc2 = launch_dependent(attn::attn_mma_kernel<DP, FP8>, plan.ctas, attn::MMA_THREADS, C::SMEM, st, p, attn_divisor(p.block_size));
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
-    return launch_dependent(attn_join_kernel<attn::MMA_ROWS, DP, FP8>, dim3(plan.ctas - 1, attn_join_ctas(attn::MMA_ROWS)), ATTN_JOIN_THREADS, 0, st, p);
+    return launch_dependent(attn_join_kernel<attn::MMA_ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, p);
 }
 
 // The tcgen05 form.  It reads pages in boxes of the largest power of two that divides page and tile, at least a swizzle atom's eight rows,
@@ -199,7 +199,7 @@ template <int DP, bool FP8> int launch_tc(AttnParams p, const TcPlan& plan, cuda
     p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.extra = TC_EXTRA;
     const int rc2 = launch_dependent(attn::attn_tc_kernel<DP, FP8>, plan.ctas, C::THREADS, C::SMEM, st, map_k, map_v, p, plan.box_rows);
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
-    return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, attn_join_ctas(C::ROWS)), ATTN_JOIN_THREADS, 0, st, p);
+    return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, p);
 }
 
 int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {

@@ -242,21 +242,50 @@ static __device__ __noinline__ void attn_row_again(const AttnParams& p, bool fp8
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Joins the pieces of items that were cut.  CTA (c, y) looks at the cut between ranges c and c + 1; the first cut of an item joins it, each
-// y some of its rows.  A piece's slot: 2 c for the item that range c begins inside, 2 c + 1 for one that begins in range c and goes on.
-// Up to ATTN_JOIN_FEW pieces a warp takes a row; beyond (few sequences over a long cache: as many pieces as CTAs) the warps share a row's
-// pieces and add their sums in the order of the warps.
-// (With the item's place worked out here, from the lengths, the join took as long as a sixth of the attention of 512 tokens over 32768:
-// 50 us of 280.)
+// Joins the pieces of items that were cut.  CTA (c, y) looks at the cut between ranges c and c + 1; the first cut of an item joins it.  A
+// piece's slot: 2 c for the item that range c begins inside, 2 c + 1 for one that begins in range c and goes on.
+//
+// What it costs is latency (where the item was cut, its lengths, M and L, then O), so a CTA has all its loads of a kind in flight: up to
+// ATTN_JOIN_FEW pieces it takes 32 rows, a warp works out their weights, then all warps go over the rows' channels; beyond (few sequences
+// over a long cache: as many pieces as CTAs) it takes a row at a time, whose pieces the warps share and add in the order of the warps.
+// (With the item's place worked out here, from the lengths, the join took 50 us of the 280 of 512 tokens over 32768; a row at a time to a
+// warp, 25.)
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int ATTN_JOIN_WARPS = 4, ATTN_JOIN_THREADS = 32 * ATTN_JOIN_WARPS;
-constexpr uint32_t ATTN_JOIN_FEW = 8;
-constexpr int attn_join_ctas(int block_rows) { return block_rows <= 16 ? 8 : block_rows / 8; }   // grid y
+constexpr int ATTN_JOIN_WARPS = 8, ATTN_JOIN_THREADS = 32 * ATTN_JOIN_WARPS;
+constexpr uint32_t ATTN_JOIN_FEW = 8, ATTN_JOIN_ROWS = 32;
+constexpr uint32_t ATTN_JOIN_Y = 8;                                          // grid y: 8 x 32 rows cover the largest block
+
+// N channels of a row from channel `ch` on; true if one is not finite
+template <int N>
+__device__ __forceinline__ bool attn_store(const AttnParams& p, uint32_t token, uint32_t head, uint32_t ch, const float (&o)[N], float l) {
+    const float inv = l == 0.0f ? 0.0f : p.v_scale / l;
+    uint16_t* const to = p.out + size_t(token) * p.out_row_stride + size_t(head) * p.head_dim + ch;
+    if (ch >= p.head_dim) return false;                                      // (head_dim is a multiple of 32, and N divides it)
+    bool odd = false;
+    uint32_t y[N / 2];
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+        const float a = l == 0.0f ? 0.0f : o[k] * inv, b = l == 0.0f ? 0.0f : o[k + 1] * inv;
+        odd |= !isfinite(a) || !isfinite(b);
+        y[k / 2] = pack_bf16x2(a, b);
+    }
+    if ((reinterpret_cast<uintptr_t>(to) & (2u * N - 1u)) == 0u) {
+        if constexpr (N == 2) *reinterpret_cast<uint32_t*>(to) = y[0];
+        if constexpr (N == 4) *reinterpret_cast<uint2*>(to) = make_uint2(y[0], y[1]);
+        if constexpr (N == 8) *reinterpret_cast<uint4*>(to) = make_uint4(y[0], y[1], y[2], y[3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) to[k] = uint16_t(y[k >> 1] >> (16 * (k & 1)));
+    }
+    return odd;
+}
 
 template <int ROWS, int DP, bool FP8>
-__global__ void __launch_bounds__(ATTN_JOIN_THREADS) attn_join_kernel(const __grid_constant__ AttnParams p) {
-    constexpr int V = DP / 32;                                               // channels of a lane, side by side
-    __shared__ float o_s[ATTN_JOIN_WARPS][DP];
+__global__ void __launch_bounds__(ATTN_JOIN_THREADS, 4) attn_join_kernel(const __grid_constant__ AttnParams p) {
+    __shared__ float o_s[ATTN_JOIN_WARPS][DP], w_s[ATTN_JOIN_FEW][ATTN_JOIN_ROWS], l_s[ATTN_JOIN_ROWS];
+    __shared__ uint32_t odd_s;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) odd_s = 0;
     pdl_wait();
     pdl_release();
     const uint32_t c = blockIdx.x + 1;
@@ -267,10 +296,63 @@ __global__ void __launch_bounds__(ATTN_JOIN_THREADS) attn_join_kernel(const __gr
     const size_t part = attn_part_floats(ROWS, DP);
     const float* const first = p.parts + part * (2 * size_t(c - 1) + 1);     // piece 0; piece i > 0 lies in slot 2 (c - 1 + i)
     auto piece = [&](uint32_t i) { return i == 0 ? first : p.parts + part * (2 * size_t(c - 1 + i)); };
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const bool few = cut.pieces <= ATTN_JOIN_FEW;
-    const uint32_t begin = few ? 0u : warp, step = few ? 1u : uint32_t(ATTN_JOIN_WARPS);
-    for (uint32_t r = few ? blockIdx.y * ATTN_JOIN_WARPS + warp : blockIdx.y; r < rows; r += gridDim.y * (few ? ATTN_JOIN_WARPS : 1)) {
+    auto place = [&](uint32_t r, uint32_t& in_seq, uint32_t& token, uint32_t& head) {
+        const uint32_t row = cut.block * ROWS + r;
+        in_seq = row / p.group;
+        token = sq.row0 + in_seq;
+        head = cut.head * p.group + row - in_seq * p.group;
+    };
+    uint32_t in_seq, token, head;
+    if (cut.pieces <= ATTN_JOIN_FEW) {
+        const uint32_t r0 = blockIdx.y * ATTN_JOIN_ROWS;
+        if (r0 >= rows) return;
+        const uint32_t n_rows = min(rows - r0, ATTN_JOIN_ROWS);
+        if (warp == 0) {
+            const uint32_t r = r0 + min(lane, n_rows - 1u);
+            float m[ATTN_JOIN_FEW], l_i[ATTN_JOIN_FEW], top = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < ATTN_JOIN_FEW; ++i) {
+                const float* s = piece(min(i, cut.pieces - 1u)) + size_t(ROWS) * DP + r;
+                m[i] = i < cut.pieces ? s[0] : -INFINITY;
+                l_i[i] = i < cut.pieces ? s[ROWS] : 0.0f;
+                top = fmaxf(top, m[i]);
+            }
+            const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (uint32_t i = 0; i < ATTN_JOIN_FEW; ++i) {
+                const float w = exp2f(m[i] - base);
+                l += w * l_i[i];
+                w_s[i][lane] = w;
+            }
+            l_s[lane] = l;
+            place(r, in_seq, token, head);
+            if (p.lse && lane < n_rows) p.lse[size_t(token) * p.q_heads + head] = attn_lse(top, l);
+        }
+        __syncthreads();
+        constexpr uint32_t LANES = DP / 4, AT_ONCE = ATTN_JOIN_THREADS / LANES;   // four channels a lane
+        const uint32_t ch = (threadIdx.x % LANES) * 4u;
+#pragma unroll 4
+        for (uint32_t k = threadIdx.x / LANES; k < n_rows; k += AT_ONCE) {
+            float o[4] = {};
+#pragma unroll 2
+            for (uint32_t i = 0; i < cut.pieces; ++i) {
+                const float4 v = *reinterpret_cast<const float4*>(piece(i) + size_t(r0 + k) * DP + ch);
+                const float w = w_s[i][k];
+                o[0] += w * v.x; o[1] += w * v.y; o[2] += w * v.z; o[3] += w * v.w;
+            }
+            place(r0 + k, in_seq, token, head);
+            if (attn_store<4>(p, token, head, ch, o, l_s[k])) atomicOr(&odd_s, 1u << k);
+        }
+        __syncthreads();
+        for (uint32_t k = warp; k < n_rows; k += ATTN_JOIN_WARPS)
+            if ((odd_s >> k) & 1u) {
+                place(r0 + k, in_seq, token, head);
+                attn_row_again(p, FP8, cut.seq, token, head, attn_row_keys(sq, in_seq));
+            }
+        return;
+    }
+    constexpr int V = DP / 32;                                               // channels of a lane, side by side
+    for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
         float m = -INFINITY, l = 0.0f;
         for (uint32_t i = lane; i < cut.pieces; i += 32) m = fmaxf(m, piece(i)[size_t(ROWS) * DP + r]);
         for (uint32_t x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
@@ -284,8 +366,8 @@ __global__ void __launch_bounds__(ATTN_JOIN_THREADS) attn_join_kernel(const __gr
                 l += w_mine * s[ROWS + r];
             }
             const uint32_t n = min(cut.pieces - i0, 32u);
-#pragma unroll 8
-            for (uint32_t i = begin; i < n; i += step) {
+#pragma unroll 4
+            for (uint32_t i = warp; i < n; i += ATTN_JOIN_WARPS) {
                 const float w = __shfl_sync(0xFFFFFFFFu, w_mine, i);
                 const float* s = piece(i0 + i) + size_t(r) * DP + lane * V;
                 float v[V];
@@ -298,43 +380,21 @@ __global__ void __launch_bounds__(ATTN_JOIN_THREADS) attn_join_kernel(const __gr
             }
         }
         for (uint32_t x = 16; x; x >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
-        if (!few) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) o_s[warp][lane * V + k] = o[k];
-            __syncthreads();
-            if (warp == 0)
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    o[k] = o_s[0][lane * V + k];
-                    for (int w = 1; w < ATTN_JOIN_WARPS; ++w) o[k] += o_s[w][lane * V + k];
-                }
-            __syncthreads();
-            if (warp != 0) continue;
-        }
-        const uint32_t row = cut.block * ROWS + r, in_seq = row / p.group, token = sq.row0 + in_seq, head = cut.head * p.group + row % p.group;
-        const float inv = l == 0.0f ? 0.0f : p.v_scale / l;
-        uint16_t* const to = p.out + size_t(token) * p.out_row_stride + size_t(head) * p.head_dim + lane * V;
-        bool odd = false;
-        if (lane * V < p.head_dim) {                                         // (head_dim is a multiple of V)
-            uint32_t y[V / 2];
+        for (int k = 0; k < V; ++k) o_s[warp][lane * V + k] = o[k];
+        __syncthreads();
+        if (warp == 0) {
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                o[k] = l == 0.0f ? 0.0f : o[k] * inv;
-                odd |= !isfinite(o[k]);
+                o[k] = o_s[0][lane * V + k];
+                for (int w = 1; w < ATTN_JOIN_WARPS; ++w) o[k] += o_s[w][lane * V + k];
             }
-#pragma unroll
-            for (int k = 0; k < V / 2; ++k) y[k] = pack_bf16x2(o[2 * k], o[2 * k + 1]);
-            if ((reinterpret_cast<uintptr_t>(to) & (2u * V - 1u)) == 0u) {
-                if constexpr (V == 2) *reinterpret_cast<uint32_t*>(to) = y[0];
-                if constexpr (V == 4) *reinterpret_cast<uint2*>(to) = make_uint2(y[0], y[1]);
-                if constexpr (V == 8) *reinterpret_cast<uint4*>(to) = make_uint4(y[0], y[1], y[2], y[3]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < V; ++k) to[k] = uint16_t(y[k >> 1] >> (16 * (k & 1)));
-            }
+            place(r, in_seq, token, head);
+            const bool odd = attn_store<V>(p, token, head, lane * V, o, l);
+            if (p.lse && lane == 0) p.lse[size_t(token) * p.q_heads + head] = attn_lse(m, l);
+            if (__any_sync(0xFFFFFFFFu, odd)) attn_row_again(p, FP8, cut.seq, token, head, attn_row_keys(sq, in_seq));
         }
-        if (p.lse && lane == 0) p.lse[size_t(token) * p.q_heads + head] = attn_lse(m, l);
-        if (__any_sync(0xFFFFFFFFu, odd)) attn_row_again(p, FP8, cut.seq, token, head, attn_row_keys(sq, in_seq));
+        __syncthreads();
     }
 }
 
