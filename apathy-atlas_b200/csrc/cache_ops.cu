@@ -125,7 +125,7 @@ struct MmaPlan {
 };
 MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms) {
     const uint32_t dim = attn_dim(d.head_dim);
-    const uint32_t row_bytes = dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u), resident = std::min(sms, ATTN_MAX_CTAS / 2) * (row_bytes >= 512u ? 1u : 2u);
+    const uint32_t row_bytes = dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u), resident = std::min(sms, ATTN_MAX_CTAS / 3) * (row_bytes >= 512u ? 1u : row_bytes > 128u ? 2u : 3u);
     const uint64_t group = d.q_heads / d.kv_heads;
     const uint64_t rows = std::min<uint64_t>(d.max_q_len, d.n_tokens) * group;
     const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * std::max<uint64_t>((rows + attn::MMA_ROWS - 1) / attn::MMA_ROWS, 1);

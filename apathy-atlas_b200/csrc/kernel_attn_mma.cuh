@@ -24,9 +24,11 @@ template <int DP, bool FP8> struct MmaCfg {
     // Tokens of a unit.  A unit is a chain (copy, scores, maximum, weights, product) of some 1500 cycles whatever its bytes.
     static constexpr int UNIT = ROW_BYTES <= 128 ? 32 : 16, TILE = UNIT * MMA_WARPS;
     static constexpr int SIDE = UNIT * ROW_BYTES;                            // K or V of a unit
-    // two CTAs on an SM (one where a row is 512 bytes), the ring as deep as that leaves room for
-    static constexpr int CTAS = ROW_BYTES >= 512 ? 1 : 2;
-    static constexpr int STAGES = (ROW_BYTES >= 512 ? 196608 : 98304) / MMA_WARPS / (2 * SIDE) > 8 ? 8 : (ROW_BYTES >= 512 ? 196608 : 98304) / MMA_WARPS / (2 * SIDE);
+    // CTAs on an SM, and the ring as deep as that leaves room for.  Short rows mean more arithmetic for a byte, so three: what a unit waits
+    // for is its own instructions.
+    static constexpr int CTAS = ROW_BYTES >= 512 ? 1 : ROW_BYTES > 128 ? 2 : 3;
+    static constexpr int RING_BYTES = ROW_BYTES >= 512 ? 196608 : ROW_BYTES > 128 ? 98304 : 65536;
+    static constexpr int STAGES = RING_BYTES / MMA_WARPS / (2 * SIDE) > 8 ? 8 : RING_BYTES / MMA_WARPS / (2 * SIDE);
     static constexpr int RING = MMA_WARPS * STAGES * 2 * SIDE;
     static constexpr int JOIN = MMA_WARPS * MMA_ROWS * (DP + 4) * 4;         // (overlaid)
     static constexpr int MAIN = RING > JOIN ? RING : JOIN;
