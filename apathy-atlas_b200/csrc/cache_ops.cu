@@ -68,8 +68,8 @@ int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, c
 thread_local uint32_t t_attn_shape[4] = {0, 0, 0, 0};
 
 // room for a cut of every range: more than any GPU this library runs on has SMs, twice
-constexpr size_t ATTN_CUT_BYTES = 512 * sizeof(AttnCut);
-constexpr uint32_t ATTN_MAX_CTAS = 512;
+constexpr size_t ATTN_CUT_BYTES = 1024 * sizeof(AttnCut);
+constexpr uint32_t ATTN_MAX_CTAS = 1024;
 
 uint32_t attn_dim(uint32_t head_dim) { return head_dim <= 64 ? 64u : head_dim <= 128 ? 128u : 256u; }
 
@@ -120,35 +120,40 @@ constexpr uint32_t MMA_EXTRA = MMA_EXTRA_, TC_EXTRA = TC_EXTRA_;
 
 // The mma.sync form: how many CTAs, and whether each takes whole items.
 struct MmaPlan {
-    uint32_t ctas, by_item, least, tile;
+    uint32_t ctas, by_item, least, tile, block_rows;
     size_t ws_bytes;
 };
 MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms) {
     const uint32_t dim = attn_dim(d.head_dim);
-    const uint32_t row_bytes = dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u), resident = std::min(sms, ATTN_MAX_CTAS / 3) * (row_bytes >= 512u ? 1u : row_bytes > 128u ? 2u : 3u);
+    const uint32_t row_bytes = dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u), resident = std::min(sms, ATTN_MAX_CTAS / 3) * uint32_t(attn::attn_mma_ctas(int(row_bytes), d.cache_dtype == ATLAS_B200_CACHE_E4M3));
     const uint64_t group = d.q_heads / d.kv_heads;
     const uint64_t rows = std::min<uint64_t>(d.max_q_len, d.n_tokens) * group;
-    const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * std::max<uint64_t>((rows + attn::MMA_ROWS - 1) / attn::MMA_ROWS, 1);
     MmaPlan r{};
+    r.block_rows = rows <= 8 ? 8u : 16u;
+    const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * std::max<uint64_t>((rows + r.block_rows - 1) / r.block_rows, 1);
     r.tile = uint32_t(attn::MMA_WARPS) * (row_bytes <= 128u ? 32u : 16u);
     const uint64_t tiles = std::max<uint64_t>((uint64_t(d.max_kv_len) + r.tile - 1) / r.tile, 1);
     r.by_item = tiles <= 4;
     r.least = r.by_item ? 1u : 4u;
     const uint64_t places = r.by_item ? items : (items * (tiles + MMA_EXTRA) + r.least - 1) / r.least;
     r.ctas = uint32_t(std::min<uint64_t>(resident, std::max<uint64_t>(places, 1)));
-    r.ws_bytes = r.by_item ? 0 : ATTN_CUT_BYTES + size_t(resident) * 2 * attn_part_floats(attn::MMA_ROWS, dim) * sizeof(float);
+    r.ws_bytes = r.by_item ? 0 : ATTN_CUT_BYTES + size_t(resident) * 2 * attn_part_floats(r.block_rows, dim) * sizeof(float);
     return r;
 }
 
-template <int DP, bool FP8> int launch_mma(AttnParams p, const MmaPlan& plan, cudaStream_t st) {
-    using C = attn::MmaCfg<DP, FP8>;
+template <int DP, bool FP8, int RT> int launch_mma_rows(AttnParams p, const MmaPlan& plan, cudaStream_t st) {
+    using C = attn::MmaCfg<DP, FP8, RT>;
     static std::atomic<bool> done[kMaxDevices] = {};
-    const int rc = allow_smem(attn::attn_mma_kernel<DP, FP8>, C::SMEM, done);
+    const int rc = allow_smem(attn::attn_mma_kernel<DP, FP8, RT>, C::SMEM, done);
     if (rc) return rc;
     p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.extra = MMA_EXTRA;
-    const int rc2 = launch_dependent(attn::attn_mma_kernel<DP, FP8>, plan.ctas, attn::MMA_THREADS, C::SMEM, st, p, attn_divisor(p.block_size));
+    const int rc2 = launch_dependent(attn::attn_mma_kernel<DP, FP8, RT>, plan.ctas, attn::MMA_THREADS, C::SMEM, st, p, attn_divisor(p.block_size));
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
-    return launch_dependent(attn_join_kernel<attn::MMA_ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, p);
+    return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, p);
+}
+
+template <int DP, bool FP8> int launch_mma(const AttnParams& p, const MmaPlan& plan, cudaStream_t st) {
+    return plan.block_rows == 8 ? launch_mma_rows<DP, FP8, 1>(p, plan, st) : launch_mma_rows<DP, FP8, 2>(p, plan, st);
 }
 
 // The tcgen05 form.  It reads pages in boxes of the largest power of two that divides page and tile, at least a swizzle atom's eight rows,
@@ -163,8 +168,11 @@ uint32_t tc_box_rows(uint32_t block_size) {
     return r;
 }
 bool takes_tc(const atlas_b200_attention_desc& d) {
-    const uint64_t rows = uint64_t(std::min(d.max_q_len, d.n_tokens)) * (d.q_heads / d.kv_heads);
-    return rows > 32 && tc_box_rows(d.block_size) >= 8 && aligned(d.q, 16) && aligned(d.out, 16) && d.q_row_stride % 8 == 0 && d.out_row_stride % 8 == 0;
+    // Rows of a KV head from which on the tensor cores' 256-row blocks pay, although most of such a block is empty.  16 sequences of 4000
+    // tokens, 8 KV heads of 128, this form / mma.sync: BF16, 12 rows 64 / 56 us, 24 rows 64 / 89, 40 rows 66 / 129; E4M3, whose tiles
+    // are converted by four warps, 24 rows 92 / 79.
+    const uint64_t rows = uint64_t(std::min(d.max_q_len, d.n_tokens)) * (d.q_heads / d.kv_heads), from = d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 32 : 16;
+    return rows > from && tc_box_rows(d.block_size) >= 8 && aligned(d.q, 16) && aligned(d.out, 16) && d.q_row_stride % 8 == 0 && d.out_row_stride % 8 == 0;
 }
 TcPlan plan_tc(const atlas_b200_attention_desc& d, uint32_t sms) {
     sms = std::min(sms, ATTN_MAX_CTAS);
@@ -224,7 +232,7 @@ int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
     if (!d.ws && !plan.by_item) { plan.by_item = 1; plan.least = 1; }        // (no scratch: nothing is cut)
     const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3;
     const AttnParams p = attention_params(d);
-    t_attn_shape[0] = attn::MMA_ROWS; t_attn_shape[1] = plan.ctas; t_attn_shape[2] = plan.by_item; t_attn_shape[3] = plan.tile;
+    t_attn_shape[0] = plan.block_rows; t_attn_shape[1] = plan.ctas; t_attn_shape[2] = plan.by_item; t_attn_shape[3] = plan.tile;
     if (dim == 64) return fp8 ? launch_mma<64, true>(p, plan, st) : launch_mma<64, false>(p, plan, st);
     if (dim == 128) return fp8 ? launch_mma<128, true>(p, plan, st) : launch_mma<128, false>(p, plan, st);
     return fp8 ? launch_mma<256, true>(p, plan, st) : launch_mma<256, false>(p, plan, st);

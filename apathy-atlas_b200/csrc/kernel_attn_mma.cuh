@@ -1,9 +1,14 @@
 // Paged attention for few rows: one token of every sequence (decode), a few drafts, and any shape the tcgen05 form does not take.
 //
 // What bounds it is the cache: per KV head and token 2 head_dim values are read for 4 head_dim operations a row, and a KV head has
-// `group` rows a token.  So a block is 16 rows (the M of mma.sync.m16n8k16, most of them empty in a decode step, which costs nothing),
-// every warp has units of sixteen tokens' K and V (32 where rows are short) of its own in flight through a private ring in shared memory (cp.async, 16 bytes a lane: a row
-// of the cache is wherever its page is, so any page size will do and places behind a sequence's end are filled with zeros), and no warp
+// `group` rows a token.  The products are the transposed ones, with tokens and channels as the sixteen rows of mma.sync.m16n8k16 and the block's
+// rows as its eight columns: S^T = K Q^T, O^T = V^T P^T.  So a block of up to eight rows (RT = 1) wastes nothing: half the matrix
+// instructions, exponentials and accumulators of the form with Q as the sixteen rows; RT = 2 has sixteen.  P^T comes out of S^T by one 8 x 8
+// transposition (movmatrix).
+//
+// Every warp has units of sixteen tokens' K and V (32 where rows are short) of its own in flight through a private ring in shared memory
+// (cp.async, 16 bytes a lane: a row of the cache is wherever its page is, so any page size will do and places behind a sequence's end are
+// filled with zeros; a bulk copy for each row takes 15 cycles whatever its length, which is 2.3 TB/s for rows of 128 bytes), and no warp
 // waits for another until the range's item ends: then the warps' maxima, sums and outputs are joined in shared memory.
 //
 // An E4M3 cache is multiplied as FP16, which holds every E4M3 value: conversion is one instruction for two values and keeps NaN.  Q is
@@ -17,22 +22,25 @@
 namespace atlas {
 namespace attn {
 
-constexpr int MMA_WARPS = 4, MMA_THREADS = 32 * MMA_WARPS, MMA_ROWS = 16;
+constexpr int attn_mma_ctas(int row_bytes, bool fp8) { return row_bytes >= 512 ? 1 : row_bytes > 128 && !fp8 ? 2 : 3; }
+constexpr int MMA_WARPS = 4, MMA_THREADS = 32 * MMA_WARPS;
 
-template <int DP, bool FP8> struct MmaCfg {
+template <int DP, bool FP8, int RT> struct MmaCfg {
+    static constexpr int ROWS = 8 * RT;
     static constexpr int ROW_BYTES = DP * (FP8 ? 1 : 2);
     // Tokens of a unit.  A unit is a chain (copy, scores, maximum, weights, product) of some 1500 cycles whatever its bytes.
     static constexpr int UNIT = ROW_BYTES <= 128 ? 32 : 16, TILE = UNIT * MMA_WARPS;
     static constexpr int SIDE = UNIT * ROW_BYTES;                            // K or V of a unit
-    // CTAs on an SM, and the ring as deep as that leaves room for.  Short rows mean more arithmetic for a byte, so three: what a unit waits
-    // for is its own instructions.
-    static constexpr int CTAS = ROW_BYTES >= 512 ? 1 : ROW_BYTES > 128 ? 2 : 3;
-    static constexpr int RING_BYTES = ROW_BYTES >= 512 ? 196608 : ROW_BYTES > 128 ? 98304 : 65536;
+    // CTAs on an SM, and the ring as deep as that leaves room for.  Short rows and conversions mean more arithmetic for a byte, so three:
+    // what a unit waits for is its own instructions (256 sequences of up to 4096 over E4M3: 278 us with two, 252 with three; with units of
+    // 16 tokens 299, and 290 with four CTAs).
+    static constexpr int CTAS = attn_mma_ctas(ROW_BYTES, FP8);
+    static constexpr int RING_BYTES = CTAS == 1 ? 196608 : CTAS == 2 ? 98304 : 65536;
     static constexpr int STAGES = RING_BYTES / MMA_WARPS / (2 * SIDE) > 8 ? 8 : RING_BYTES / MMA_WARPS / (2 * SIDE);
     static constexpr int RING = MMA_WARPS * STAGES * 2 * SIDE;
-    static constexpr int JOIN = MMA_WARPS * MMA_ROWS * (DP + 4) * 4;         // (overlaid)
+    static constexpr int JOIN = MMA_WARPS * ROWS * (DP + 4) * 4;         // (overlaid)
     static constexpr int MAIN = RING > JOIN ? RING : JOIN;
-    static constexpr int SMEM = MAIN + MMA_WARPS * MMA_ROWS * 8 + 16 * 8;
+    static constexpr int SMEM = MAIN + MMA_WARPS * ROWS * 8 + 16 * 8;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -40,6 +48,12 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
 }
 __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 8 x 8 matrix of 16-bit values, one row a group of four lanes, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
 template <bool HALF>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -69,10 +83,11 @@ template <int ROW_BYTES> __device__ __forceinline__ uint32_t unit_off(uint32_t t
     else return t * ROW_BYTES + ((c ^ ((t >> 1) & 3u)) << 4);
 }
 
-template <int DP, bool FP8>
-__global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_kernel(const __grid_constant__ AttnParams p, const AttnDivisor div) {
-    using C = MmaCfg<DP, FP8>;
-    constexpr int NT = DP / 8, KS = DP / 16;                                 // n tiles of the output, K steps of the scores
+template <int DP, bool FP8, int RT>
+__global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_mma_kernel(const __grid_constant__ AttnParams p, const AttnDivisor div) {
+    using C = MmaCfg<DP, FP8, RT>;
+    constexpr int MT = DP / 16, KS = DP / 16, UT = C::UNIT / 16;             // sixteen channels of the output; K steps of the scores; sixteen tokens of a unit
+    constexpr int MMA_ROWS = C::ROWS;
     extern __shared__ __align__(1024) uint8_t attn_smem[];
     uint64_t* sh = reinterpret_cast<uint64_t*>(attn_smem + C::MAIN + MMA_WARPS * MMA_ROWS * 8);
     float* ml = reinterpret_cast<float*>(attn_smem + C::MAIN);               // [warp][row] M, then [warp][row] L
@@ -99,16 +114,6 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
         const uint32_t seq = walk.seq, t0 = walk.t0, t1 = walk.t1;
         const uint32_t rows_left = sq.q_len * p.group - at.block * MMA_ROWS, rows = min(rows_left, uint32_t(MMA_ROWS));
 
-        // this lane's two rows: their tokens, heads and how many keys they see
-        uint32_t keys[2];
-        const uint16_t* q_row[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t r = g + 8u * i, row = at.block * MMA_ROWS + r, tok = row / p.group;
-            const bool there = r < rows;
-            keys[i] = there ? attn_row_keys(sq, tok) : 0u;
-            q_row[i] = there ? p.q + size_t(sq.row0 + tok) * p.q_row_stride + size_t(at.head * p.group + row % p.group) * D : nullptr;
-        }
         const uint32_t last_tok = (at.block * MMA_ROWS + rows - 1) / p.group, first_tok = at.block * MMA_ROWS / p.group;
         const uint32_t all_see = attn_row_keys(sq, first_tok), n_keys = attn_row_keys(sq, last_tok);
 
@@ -146,23 +151,25 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
         }
         int32_t row_next = find_row(C::STAGES - 1);
 
-        // Q as the A operand.  BF16: K step s covers channels 16 s + {2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9}; E4M3: step 4 j + w covers
-        // 64 j + 16 q4 + 4 w .. + 3, which are the bytes that a lane reads of K in one word.
-        uint32_t qa[KS][4];
-        float c_row[2] = {p.scale * ATTN_LOG2E, p.scale * ATTN_LOG2E};
+        // Q as the B operand, row g of a row tile.  BF16: K step s covers channels 16 s + {2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9}; E4M3: step 4 j + w
+        // covers 64 j + 16 q4 + 4 w .. + 3, which are the bytes that a lane reads of K in one word.
+        uint32_t qb[RT][KS][2], keys[RT][2];
+        float c_row[RT][2];                                                  // of this lane's scores: rows 2 q4 and 2 q4 + 1
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            uint32_t w[2 * KS];
+        for (int t = 0; t < RT; ++t) {
+            const uint32_t r = 8u * t + g, row = at.block * MMA_ROWS + r, tok = row / p.group;
+            const uint16_t* q_row = r < rows ? p.q + size_t(sq.row0 + tok) * p.q_row_stride + size_t(at.head * p.group + row % p.group) * D : nullptr;
             uint32_t top = 0;
 #pragma unroll
             for (int s = 0; s < KS; ++s)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t d = FP8 ? 64u * (s >> 2) + 16u * q4 + 4u * (s & 3) + 2u * h : 16u * s + 2u * q4 + 8u * h;
-                    const uint32_t v = q_row[i] && d < D ? *reinterpret_cast<const uint32_t*>(q_row[i] + d) : 0u;
-                    w[2 * s + h] = v;
+                    const uint32_t v = q_row && d < D ? *reinterpret_cast<const uint32_t*>(q_row + d) : 0u;
+                    qb[t][s][h] = v;
                     if constexpr (FP8) top = max(top, max(v & 0x7FFFu, (v >> 16) & 0x7FFFu));
                 }
+            float c = p.scale * ATTN_LOG2E;
             if constexpr (FP8) {
                 top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                 top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
@@ -170,17 +177,28 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
                 // holds either way; rows of zeros, infinities or NaN are left as they are.)
                 const int e = int(top >> 7), by = e == 0 || e == 255 ? 0 : min(max(141 - e, -120), 120);
                 const float up = __uint_as_float(uint32_t(127 + by) << 23);
-                c_row[i] *= p.k_scale * __uint_as_float(uint32_t(127 - by) << 23);
+                c *= p.k_scale * __uint_as_float(uint32_t(127 - by) << 23);
 #pragma unroll
-                for (int k = 0; k < 2 * KS; ++k) w[k] = pack2<true>(bf16_lo(w[k]) * up, bf16_hi(w[k]) * up);
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) qb[t][s][h] = pack2<true>(bf16_lo(qb[t][s][h]) * up, bf16_hi(qb[t][s][h]) * up);
             }
 #pragma unroll
-            for (int s = 0; s < KS; ++s) { qa[s][i] = w[2 * s]; qa[s][2 + i] = w[2 * s + 1]; }
+            for (uint32_t e = 0; e < 2; ++e) {
+                const uint32_t mine = 8u * t + 2u * q4 + e;
+                c_row[t][e] = FP8 ? __shfl_sync(0xFFFFFFFFu, c, 4u * (2u * q4 + e)) : c;
+                keys[t][e] = mine < rows ? attn_row_keys(sq, (at.block * MMA_ROWS + mine) / p.group) : 0u;
+            }
         }
 
-        float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        float o[MT][RT][4], m[RT][2], l[RT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+        for (int t = 0; t < RT; ++t) {
+            m[t][0] = m[t][1] = -INFINITY;
+            l[t][0] = l[t][1] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < MT; ++n) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.0f;
+        }
 
         for (uint32_t u = 0; u < units; ++u) {
             issue(u + C::STAGES - 1, row_next);
@@ -190,77 +208,94 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
             const uint32_t pos0 = pos_w + u * C::TILE;
             if (pos0 < n_keys) {                                             // (the same for the whole warp)
                 const uint32_t ks = ring + (u % C::STAGES) * (2 * C::SIDE), vs = ks + C::SIDE;
-                float s[C::UNIT / 8][4] = {};
+                float s[UT][RT][4] = {};                                     // tokens g and g + 8, rows 2 q4 and 2 q4 + 1
                 if constexpr (!FP8) {
 #pragma unroll
                     for (int k = 0; k < KS; ++k)
 #pragma unroll
-                        for (int n = 0; n < C::UNIT / 8; n += 2) {
-                            uint32_t b[4];
-                            ldsm4(b, ks + unit_off<C::ROW_BYTES>(8u * n + ((lane >> 4) << 3) + (lane & 7u), 2u * k + ((lane >> 3) & 1u)));
-                            mma16816<false>(s[n], qa[k], b[0], b[1]);
-                            mma16816<false>(s[n + 1], qa[k], b[2], b[3]);
+                        for (int n = 0; n < UT; ++n) {
+                            uint32_t a[4];
+                            ldsm4(a, ks + unit_off<C::ROW_BYTES>(16u * n + (lane & 15u), 2u * k + (lane >> 4)));
+#pragma unroll
+                            for (int t = 0; t < RT; ++t) mma16816<false>(s[n][t], a, qb[t][k][0], qb[t][k][1]);
                         }
                 } else {
 #pragma unroll
                     for (int j = 0; j < DP / 64; ++j) {
-                        uint32_t w[C::UNIT / 8][4];
+                        uint32_t w[2 * UT][4];
 #pragma unroll
-                        for (int n = 0; n < C::UNIT / 8; ++n)
+                        for (int n = 0; n < 2 * UT; ++n)
                             asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[n][0]), "=r"(w[n][1]), "=r"(w[n][2]), "=r"(w[n][3])
                                          : "r"(ks + unit_off<C::ROW_BYTES>(8u * n + g, 4u * j + q4)));
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
 #pragma unroll
-                            for (int n = 0; n < C::UNIT / 8; ++n) mma16816<true>(s[n], qa[4 * j + k], e4m3x2_to_f16x2(w[n][k]), e4m3x2_to_f16x2(w[n][k] >> 16));
+                            for (int n = 0; n < UT; ++n) {
+                                const uint32_t a[4] = {e4m3x2_to_f16x2(w[2 * n][k]), e4m3x2_to_f16x2(w[2 * n + 1][k]), e4m3x2_to_f16x2(w[2 * n][k] >> 16),
+                                                       e4m3x2_to_f16x2(w[2 * n + 1][k] >> 16)};
+#pragma unroll
+                                for (int t = 0; t < RT; ++t) mma16816<true>(s[n][t], a, qb[t][4 * j + k][0], qb[t][4 * j + k][1]);
+                            }
                     }
                 }
                 if (pos0 + C::UNIT > all_see) {
 #pragma unroll
-                    for (int n = 0; n < C::UNIT / 8; ++n)
+                    for (int n = 0; n < UT; ++n)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (pos0 + 8u * n + 2u * q4 + (e & 1) >= keys[e >> 1]) s[n][e] = -INFINITY;
+                        for (int t = 0; t < RT; ++t)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (pos0 + 16u * n + g + 8u * (e >> 1) >= keys[t][e & 1]) s[n][t][e] = -INFINITY;
                 }
-                uint32_t pa[C::UNIT / 16][4];
-                float keep[2];
+                uint32_t pb[UT][RT][2];
+                bool turn = false;
+                float keep[RT][2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float top = -INFINITY;
+                for (int t = 0; t < RT; ++t) {
+                    float base[2];
 #pragma unroll
-                    for (int n = 0; n < C::UNIT / 8; ++n) top = fmaxf(fmaxf(top, s[n][2 * i]), s[n][2 * i + 1]);
-                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                    top = fmaxf(top * c_row[i], m[i]);                       // (the factor is positive)
-                    const float base = top == -INFINITY ? 0.0f : top;
-                    keep[i] = attn_exp2(m[i] - base);
-                    m[i] = top;
-                    float sum = 0.0f;
+                    for (int e = 0; e < 2; ++e) {
+                        float top = -INFINITY;
 #pragma unroll
-                    for (int n = 0; n < C::UNIT / 8; ++n) {
-                        const float p0 = attn_exp2(fmaf(s[n][2 * i], c_row[i], -base)), p1 = attn_exp2(fmaf(s[n][2 * i + 1], c_row[i], -base));
-                        sum += p0 + p1;
-                        pa[n >> 1][2 * (n & 1) + i] = pack2<FP8>(p0, p1);
+                        for (int n = 0; n < UT; ++n) top = fmaxf(fmaxf(top, s[n][t][e]), s[n][t][2 + e]);
+#pragma unroll
+                        for (uint32_t x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+                        top = fmaxf(top * c_row[t][e], m[t][e]);             // (the factor is positive)
+                        base[e] = top == -INFINITY ? 0.0f : top;
+                        keep[t][e] = attn_exp2(m[t][e] - base[e]);
+                        turn |= keep[t][e] != 1.0f;
+                        m[t][e] = top;
+                        l[t][e] *= keep[t][e];
                     }
-                    l[i] = l[i] * keep[i] + sum;
-                }
-                if (__any_sync(0xFFFFFFFFu, keep[0] != 1.0f || keep[1] != 1.0f)) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) { o[n][0] *= keep[0]; o[n][1] *= keep[0]; o[n][2] *= keep[1]; o[n][3] *= keep[1]; }
+                    for (int n = 0; n < UT; ++n)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float p0 = attn_exp2(fmaf(s[n][t][2 * h], c_row[t][0], -base[0])), p1 = attn_exp2(fmaf(s[n][t][2 * h + 1], c_row[t][1], -base[1]));
+                            l[t][0] += p0;
+                            l[t][1] += p1;
+                            pb[n][t][h] = transposed(pack2<FP8>(p0, p1));
+                        }
+                }
+                if (__any_sync(0xFFFFFFFFu, turn)) {
+#pragma unroll
+                    for (int n = 0; n < MT; ++n)
+#pragma unroll
+                        for (int t = 0; t < RT; ++t) { o[n][t][0] *= keep[t][0]; o[n][t][1] *= keep[t][1]; o[n][t][2] *= keep[t][0]; o[n][t][3] *= keep[t][1]; }
                 }
 #pragma unroll
-                for (int kk = 0; kk < C::UNIT / 16; ++kk) {                  // sixteen tokens a product
+                for (int kk = 0; kk < UT; ++kk) {                            // sixteen tokens a product
                     if constexpr (!FP8) {
 #pragma unroll
-                        for (int n = 0; n < NT; n += 2) {
-                            uint32_t b[4];
-                            ldsm4_trans(b, vs + unit_off<C::ROW_BYTES>(16u * kk + (((lane >> 3) & 1u) << 3) + (lane & 7u), n + (lane >> 4)));
-                            mma16816<false>(o[n], pa[kk], b[0], b[1]);
-                            mma16816<false>(o[n + 1], pa[kk], b[2], b[3]);
+                        for (int n = 0; n < MT; ++n) {
+                            uint32_t a[4];
+                            ldsm4_trans(a, vs + unit_off<C::ROW_BYTES>(16u * kk + ((lane >> 4) << 3) + (lane & 7u), 2u * n + ((lane >> 3) & 1u)));
+#pragma unroll
+                            for (int t = 0; t < RT; ++t) mma16816<false>(o[n][t], a, pb[kk][t][0], pb[kk][t][1]);
                         }
                     } else {
-                        // lane g has the channels W g .. W g + W - 1 (of each 128) of tokens 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9; n tile i is
-                        // channel i of every lane's
+                        // lane g has the channels W g .. W g + W - 1 (of each 128) of tokens 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9; rows g and g + 8 of
+                        // product i are channels 2 i and 2 i + 1 of every lane's.  Two tokens' bytes side by side, then converted.
                         constexpr int W = DP < 128 ? 8 : 16;
 #pragma unroll
                         for (int h = 0; h < (DP + 127) / 128; ++h) {
@@ -279,11 +314,11 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
 #pragma unroll
                             for (int w = 0; w < W / 4; ++w)
 #pragma unroll
-                                for (int e = 0; e < 2; ++e) {                // channels 4 w + 2 e and the next one: two tokens' bytes side by side, then converted
+                                for (int e = 0; e < 2; ++e) {
                                     const uint32_t sel = e ? 0x7362u : 0x5140u, t0 = prmt(v[0][w], v[1][w], sel), t1 = prmt(v[2][w], v[3][w], sel);
-                                    const int n = h * W + 4 * w + 2 * e;
-                                    mma16816<true>(o[n], pa[kk], e4m3x2_to_f16x2(t0), e4m3x2_to_f16x2(t1));
-                                    mma16816<true>(o[n + 1], pa[kk], e4m3x2_to_f16x2(t0 >> 16), e4m3x2_to_f16x2(t1 >> 16));
+                                    const uint32_t a[4] = {e4m3x2_to_f16x2(t0), e4m3x2_to_f16x2(t0 >> 16), e4m3x2_to_f16x2(t1), e4m3x2_to_f16x2(t1 >> 16)};
+#pragma unroll
+                                    for (int t = 0; t < RT; ++t) mma16816<true>(o[h * (W / 2) + 2 * w + e][t], a, pb[kk][t][0], pb[kk][t][1]);
                                 }
                         }
                     }
@@ -297,22 +332,22 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8>::CTAS) attn_mma_k
         // ---- the warps' pieces together ----
         float* sum = reinterpret_cast<float*>(attn_smem);                    // [warp][row][DP + 4]
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
-            const uint32_t r = g + 8u * i;
-            if (r >= rows) continue;
-            if (q4 == 0) { ml[warp * MMA_ROWS + r] = m[i]; ml[(MMA_WARPS + warp) * MMA_ROWS + r] = l[i]; }
-            float* to = sum + (warp * MMA_ROWS + r) * (DP + 4);
+        for (int t = 0; t < RT; ++t)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    constexpr int W = DP < 128 ? 8 : 16;
-                    const uint32_t d = FP8 ? 128u * (n / W) + W * (2u * q4 + e) + n % W : 8u * n + 2u * q4 + e;
-                    to[d] = o[n][2 * i + e];
-                }
-        }
+                for (uint32_t x = 4; x < 32; x <<= 1) l[t][e] += __shfl_xor_sync(0xFFFFFFFFu, l[t][e], x);
+                const uint32_t r = 8u * t + 2u * q4 + e;
+                if (r >= rows) continue;
+                if (g == 0) { ml[warp * MMA_ROWS + r] = m[t][e]; ml[(MMA_WARPS + warp) * MMA_ROWS + r] = l[t][e]; }
+                float* to = sum + (warp * MMA_ROWS + r) * (DP + 4);
+                constexpr int W = DP < 128 ? 8 : 16;
+#pragma unroll
+                for (int n = 0; n < MT; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        to[FP8 ? 128u * (n / (W / 2)) + W * g + 2u * (n % (W / 2)) + h : 16u * n + g + 8u * h] = o[n][t][2 * h + e];
+            }
         __syncthreads();
         const bool whole = walk.whole();
         float* part = whole ? nullptr : p.parts + attn_part_floats(MMA_ROWS, DP) * (2 * size_t(blockIdx.x) + (t0 == 0 ? 1 : 0));

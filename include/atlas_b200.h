@@ -598,7 +598,7 @@ ATLAS_B200_API int atlas_b200_last_persistent_shape(uint32_t out[2]);
 /* More of it: out[0] = 1 if the call's MMAs left gaps for the shrink that ran beside it, out[1] = 1 if the kernel for the smallest
  * batches had its weights brought by TMA. */
 ATLAS_B200_API int atlas_b200_last_launch_details(uint32_t out[2]);
-/* The attention launched last on this thread: out[0] = rows of a block (16: the mma.sync form), out[1] = CTAs, out[2] = 1 if every CTA
+/* The attention launched last on this thread: out[0] = rows of a block (8, 16: the mma.sync form), out[1] = CTAs, out[2] = 1 if every CTA
  * took whole items, out[3] = keys of a tile. */
 ATLAS_B200_API int atlas_b200_last_attention_shape(uint32_t out[4]);
 /* Per-CTA cycle counters of the tcgen05 kernel, the counterpart of the reference's per-phase timers
