@@ -1513,21 +1513,20 @@ static int qkv_norm_rope_cache_write(void* q, const void* k_in, const void* v_in
     p.rms_eps = rms_eps; p.attention_factor = attention_factor; p.norm_offset_one = norm_offset_one ? 1u : 0u;
     p.k_inv_scale = k_inv_scale; p.v_inv_scale = v_inv_scale;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool exact = rotary_dim == 64 && (head_dim == 64 || head_dim == 128 || head_dim == 256);
-    if (fp8) {
-        if (head_dim <= 64) return exact ? launch_chained(qkv_norm_rope_cache_kernel<1, true, true>, tokens, KVE_WARPS * 32, st, p)
-                                  : launch_chained(qkv_norm_rope_cache_kernel<1, false, true>, tokens, KVE_WARPS * 32, st, p);
-        if (head_dim <= 128) return exact ? launch_chained(qkv_norm_rope_cache_kernel<2, true, true>, tokens, KVE_WARPS * 32, st, p)
-                                        : launch_chained(qkv_norm_rope_cache_kernel<2, false, true>, tokens, KVE_WARPS * 32, st, p);
-        return exact ? launch_chained(qkv_norm_rope_cache_kernel<4, true, true>, tokens, KVE_WARPS * 32, st, p)
-                   : launch_chained(qkv_norm_rope_cache_kernel<4, false, true>, tokens, KVE_WARPS * 32, st, p);
+    // which part of the head is rotated, where the instances know it: 64 channels, or all (see the kernel)
+    const bool known = head_dim == 64 || head_dim == 128 || head_dim == 256;
+    const uint32_t rot = !known ? 0u : rotary_dim == 64 ? 1u : rotary_dim == head_dim ? 2u : 0u;
+    auto launch = [&](auto kernel) { return launch_chained(kernel, tokens, KVE_WARPS * 32, st, p); };
+    if (head_dim <= 64) {
+        if (fp8) return rot ? launch(qkv_norm_rope_cache_kernel<1, 1, true>) : launch(qkv_norm_rope_cache_kernel<1, 0, true>);
+        return rot ? launch(qkv_norm_rope_cache_kernel<1, 1>) : launch(qkv_norm_rope_cache_kernel<1, 0>);
     }
-    if (head_dim <= 64) return exact ? launch_chained(qkv_norm_rope_cache_kernel<1, true>, tokens, KVE_WARPS * 32, st, p)
-                              : launch_chained(qkv_norm_rope_cache_kernel<1, false>, tokens, KVE_WARPS * 32, st, p);
-    if (head_dim <= 128) return exact ? launch_chained(qkv_norm_rope_cache_kernel<2, true>, tokens, KVE_WARPS * 32, st, p)
-                                    : launch_chained(qkv_norm_rope_cache_kernel<2, false>, tokens, KVE_WARPS * 32, st, p);
-    return exact ? launch_chained(qkv_norm_rope_cache_kernel<4, true>, tokens, KVE_WARPS * 32, st, p)
-               : launch_chained(qkv_norm_rope_cache_kernel<4, false>, tokens, KVE_WARPS * 32, st, p);
+    if (head_dim <= 128) {
+        if (fp8) return rot == 2 ? launch(qkv_norm_rope_cache_kernel<2, 2, true>) : rot ? launch(qkv_norm_rope_cache_kernel<2, 1, true>) : launch(qkv_norm_rope_cache_kernel<2, 0, true>);
+        return rot == 2 ? launch(qkv_norm_rope_cache_kernel<2, 2>) : rot ? launch(qkv_norm_rope_cache_kernel<2, 1>) : launch(qkv_norm_rope_cache_kernel<2, 0>);
+    }
+    if (fp8) return rot == 2 ? launch(qkv_norm_rope_cache_kernel<4, 2, true>) : rot ? launch(qkv_norm_rope_cache_kernel<4, 1, true>) : launch(qkv_norm_rope_cache_kernel<4, 0, true>);
+    return rot == 2 ? launch(qkv_norm_rope_cache_kernel<4, 2>) : rot ? launch(qkv_norm_rope_cache_kernel<4, 1>) : launch(qkv_norm_rope_cache_kernel<4, 0>);
 }
 
 int atlas_b200_qkv_norm_rope_cache_write(void* q, const void* k_in, const void* v_in, uint32_t q_row_stride, uint32_t kv_row_stride,

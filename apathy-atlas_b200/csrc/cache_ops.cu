@@ -244,7 +244,7 @@ int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 size_t pages_ws_bytes(const atlas_b200_cache_desc& d, uint32_t n) {
-    return round256(size_t(d.n_seqs) * 4) + round256(size_t(n) * 16) + round256(size_t(d.n_pages) * 4) + 256;
+    return round256(size_t(d.n_seqs) * 4) + round256(size_t(n) * 24) + round256(size_t(d.n_pages) * 4) + 256;
 }
 
 int check_pages(const atlas_b200_cache_desc& d, uint32_t n, bool copies, pages::PagesParams& p) {
@@ -262,8 +262,8 @@ int check_pages(const atlas_b200_cache_desc& d, uint32_t n, bool copies, pages::
     uint8_t* ws = static_cast<uint8_t*>(d.ws);
     p.claim = reinterpret_cast<int32_t*>(ws);
     p.entry = reinterpret_cast<int32_t*>(ws + round256(size_t(d.n_seqs) * 4));
-    p.list = reinterpret_cast<int32_t*>(ws + round256(size_t(d.n_seqs) * 4) + round256(size_t(n) * 16));
-    p.count = reinterpret_cast<int32_t*>(ws + round256(size_t(d.n_seqs) * 4) + round256(size_t(n) * 16) + round256(size_t(d.n_pages) * 4));
+    p.list = reinterpret_cast<int32_t*>(ws + round256(size_t(d.n_seqs) * 4) + round256(size_t(n) * 24));
+    p.count = reinterpret_cast<int32_t*>(ws + round256(size_t(d.n_seqs) * 4) + round256(size_t(n) * 24) + round256(size_t(d.n_pages) * 4));
     return ATLAS_B200_OK;
 }
 

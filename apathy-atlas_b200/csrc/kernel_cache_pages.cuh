@@ -29,7 +29,7 @@ struct PagesParams {
     uint64_t page_bytes;
     // scratch
     int32_t* claim;               // [n_seqs] lowest entry of the call that names the sequence
-    int32_t* entry;               // [n][4]
+    int32_t* entry;               // [n][6]
     int32_t* list;                // [n_pages] free pages found; or holes from the front and moved pages from the back
     int32_t* count;               // [4]
 };
@@ -96,9 +96,13 @@ __device__ __forceinline__ uint32_t pages_of(const PagesParams& p, uint64_t toke
 
 // ---- append ------------------------------------------------------------------------------------------------------
 // Entry i gives sequence seqs[i] room for n_new[i] more tokens; slots of all entries' tokens in a row into slot_mapping.
+// (Entries of the usual call are kept in shared memory: the second pass, a warp an entry, is a chain of the loads it makes.)
+constexpr uint32_t APPEND_FIELDS = 6, APPEND_IN_SMEM = PLAN_THREADS;
 __global__ void __launch_bounds__(PLAN_THREADS) append_kernel(PagesParams p, const int32_t* seqs, const int32_t* n_new, uint32_t n, uint32_t max_tokens,
                                                               long long* slot_mapping, int32_t* status) {
     __shared__ uint64_t sh[32];
+    __shared__ int32_t entry_s[APPEND_FIELDS * APPEND_IN_SMEM];
+    int32_t* const entry = n <= APPEND_IN_SMEM ? entry_s : p.entry;
     pdl_release();
     pdl_wait();
     seqs = pdl_after(seqs); n_new = pdl_after(n_new); p.refcount = pdl_after(p.refcount); p.block_table = pdl_after(p.block_table); p.seq_len = pdl_after(p.seq_len);
@@ -108,12 +112,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) append_kernel(PagesParams p, con
     for (uint32_t base = 0; base < n; base += PLAN_THREADS) {
         const uint32_t i = base + threadIdx.x;
         int32_t say = ATLAS_B200_ERR_DIMS;
-        uint32_t need = 0, add = 0;
+        uint32_t need = 0, add = 0, s = 0;
+        uint64_t len = 0;
         if (i < n) {
-            const uint32_t s = uint32_t(seqs[i]);
+            s = uint32_t(seqs[i]);
             add = n_new[i] > 0 ? uint32_t(n_new[i]) : 0u;
             if (s < p.n_seqs && __ldcg(p.claim + s) == int32_t(i) && n_new[i] >= 0 && p.seq_len[s] >= 0 && uint64_t(p.seq_len[s]) <= room) {
-                const uint64_t len = uint32_t(p.seq_len[s]);
+                len = uint32_t(p.seq_len[s]);
                 if (len + add > room) say = ATLAS_B200_ERR_LIMIT;
                 else { say = 0; need = pages_of(p, len + add) - pages_of(p, len); }
             }
@@ -124,40 +129,45 @@ __global__ void __launch_bounds__(PLAN_THREADS) append_kernel(PagesParams p, con
         if (say == 0 && tok + add > max_tokens) { say = ATLAS_B200_ERR_LIMIT; need = 0; }
         const uint64_t before = need_all + block_scan(need, sh, sum);
         if (i < n) {
-            p.entry[4 * i] = say;
-            p.entry[4 * i + 1] = int32_t(before > 0x7FFFFFFFull ? 0x7FFFFFFFull : before);
-            p.entry[4 * i + 2] = int32_t(need);
-            p.entry[4 * i + 3] = int32_t(tok > max_tokens ? max_tokens : tok);
+            int32_t* const e = entry + APPEND_FIELDS * i;
+            e[0] = say;
+            e[1] = int32_t(before > 0x7FFFFFFFull ? 0x7FFFFFFFull : before);
+            e[2] = int32_t(need);
+            e[3] = int32_t(tok > max_tokens ? max_tokens : tok);
+            e[4] = int32_t(s);
+            e[5] = int32_t(len);
         }
         need_all += sum;
         tokens_all += tok_sum;
     }
     __syncthreads();
     const uint32_t there = find_free(p, need_all < p.n_pages ? need_all : p.n_pages, sh);
-    const uint32_t lane = threadIdx.x & 31u;
-    for (uint32_t i = threadIdx.x >> 5; i < n; i += PLAN_THREADS / 32) {     // a warp an entry
-        int32_t say = p.entry[4 * i];
-        const uint32_t before = uint32_t(p.entry[4 * i + 1]), need = uint32_t(p.entry[4 * i + 2]), tok = uint32_t(p.entry[4 * i + 3]);
+    // Eight lanes an entry, or a warp where entries have many tokens: each is a chain of loads, and 192 entries of a few tokens took a third of
+    // the call with a warp each.
+    const uint32_t width = tokens_all > 16ull * n ? 32u : 8u, lane = threadIdx.x & (width - 1u);
+    for (uint32_t i = threadIdx.x / width; i < n; i += PLAN_THREADS / width) {
+        const int32_t* const e = entry + APPEND_FIELDS * i;
+        int32_t say = e[0];
+        const uint32_t before = uint32_t(e[1]), need = uint32_t(e[2]), tok = uint32_t(e[3]);
         if (say == 0 && need && uint64_t(before) + need > there) say = ATLAS_B200_ERR_LIMIT;
         const uint32_t add = n_new[i] > 0 ? uint32_t(n_new[i]) : 0u;
         if (say == 0) {
-            const uint32_t s = uint32_t(seqs[i]), len = uint32_t(p.seq_len[s]), have = pages_of(p, len);
+            const uint32_t s = uint32_t(e[4]), len = uint32_t(e[5]), have = pages_of(p, len);
             int32_t* row = p.block_table + size_t(s) * p.table_stride;
-            for (uint32_t k = lane; k < need; k += 32) {
+            for (uint32_t k = lane; k < need; k += width) {
                 const int32_t id = p.list[before + k];
                 row[have + k] = id;
                 p.refcount[id] = 1;
             }
-            for (uint32_t k = lane; k < add; k += 32) {
+            for (uint32_t k = lane; k < add; k += width) {
                 const uint32_t pos = len + k, page = pos / p.block_size;
                 const int32_t id = page < have ? row[page] : p.list[before + page - have];
                 slot_mapping[tok + k] = uint32_t(id) < p.n_pages ? (long long)(id) * p.block_size + (pos - page * p.block_size) : -1ll;
                 if (uint32_t(id) >= p.n_pages) record_status(STATUS_PAGE_OUT_OF_RANGE);
             }
-            __syncwarp();
             if (lane == 0) p.seq_len[s] = int32_t(len + add);
         } else {
-            for (uint32_t k = lane; k < add && tok + k < max_tokens; k += 32) slot_mapping[tok + k] = -1ll;
+            for (uint32_t k = lane; k < add && tok + k < max_tokens; k += width) slot_mapping[tok + k] = -1ll;
         }
         if (lane == 0 && status) status[i] = say;
     }
