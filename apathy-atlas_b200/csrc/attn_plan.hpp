@@ -21,16 +21,20 @@
 
 namespace atlas {
 
+// A quotient, in 32 bits where both numbers have no more: a GPU divides those in a tenth of the time, and the numbers of a plan, which
+// every CTA works out before it can ask for its first key, nearly always have.
+ATLAS_HD inline uint64_t attn_quotient(uint64_t a, uint64_t b) { return ((a | b) >> 32) == 0 ? uint64_t(uint32_t(a) / uint32_t(b)) : a / b; }
+
 // sum of floor((a i + b) / m) over i = 0 .. n - 1, by Euclid's algorithm on (a, m)
 ATLAS_HD inline uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
     uint64_t sum = 0;
     while (n > 0) {
-        if (a >= m) { sum += (a / m) * (n * (n - 1) / 2); a %= m; }
-        if (b >= m) { sum += (b / m) * n; b %= m; }
+        if (a >= m) { const uint64_t q = attn_quotient(a, m); sum += q * (n * (n - 1) / 2); a -= q * m; }
+        if (b >= m) { const uint64_t q = attn_quotient(b, m); sum += q * n; b -= q * m; }
         const uint64_t last = a * n + b;
         if (last < m) break;
-        n = last / m;
-        b = last % m;
+        n = attn_quotient(last, m);
+        b = last - n * m;
         const uint64_t t = m;
         m = a;
         a = t;
@@ -45,19 +49,20 @@ struct AttnSeq {
     uint32_t group, block_rows, tile_keys, extra;
     ATLAS_HD AttnSeq(uint32_t q, uint32_t kv, uint32_t g, uint32_t rows, uint32_t keys, uint32_t more)
         : q_len(q), kv_len(kv), group(g), block_rows(rows), tile_keys(keys), extra(more) {
-        blocks = uint32_t((uint64_t(q) * g + rows - 1) / rows);
+        blocks = uint32_t(attn_quotient(uint64_t(q) * g + rows - 1, rows));
         whole = kv ? (kv - 1) / keys + 1 : 1;
     }
     // the last row of block b is row (b + 1) rows - 1, token floor of it / group; it sees kv_len - q_len + that token + 1 keys
     ATLAS_HD uint32_t tiles(uint32_t b) const {
         if (kv_len < q_len || b + 1 >= blocks) return whole;
         const uint64_t keys_less_1 = uint64_t(kv_len - q_len) + tile_keys;
-        const uint64_t t = (uint64_t(block_rows) * b + block_rows - 1 + uint64_t(group) * keys_less_1) / (uint64_t(group) * tile_keys);
+        const uint64_t t = attn_quotient(uint64_t(block_rows) * b + block_rows - 1 + uint64_t(group) * keys_less_1, uint64_t(group) * tile_keys);
         return t < whole ? uint32_t(t) : whole;
     }
     // places of the blocks before b, of one KV head
     ATLAS_HD uint64_t before(uint32_t b) const {
         if (b == 0 || blocks == 0) return 0;
+        if (blocks == 1) return uint64_t(whole) + extra;
         const uint32_t n = b < blocks ? b : blocks - 1;                                   // by the formula
         uint64_t sum = kv_len < q_len ? uint64_t(whole) * n
                                       : floor_sum(n, uint64_t(group) * tile_keys, block_rows, block_rows - 1 + uint64_t(group) * (uint64_t(kv_len - q_len) + tile_keys));
@@ -69,6 +74,16 @@ struct AttnSeq {
 struct AttnPlace {
     uint32_t block, head, place, tiles;         // place within the item, which has extra + tiles of them
 };
+// where place x lies, known to be in a block
+ATLAS_HD inline AttnPlace attn_place_in_block(const AttnSeq& s, uint32_t kv_heads, uint64_t x, uint32_t block) {
+    AttnPlace p;
+    p.block = block;
+    p.tiles = s.tiles(block);
+    const uint64_t in_block = x - s.before(block) * kv_heads;
+    p.head = uint32_t(attn_quotient(in_block, s.extra + p.tiles));
+    p.place = uint32_t(in_block - uint64_t(p.head) * (s.extra + p.tiles));
+    return p;
+}
 // where place x of a sequence's part of the line lies, x < total(kv_heads)
 ATLAS_HD inline AttnPlace attn_locate(const AttnSeq& s, uint32_t kv_heads, uint64_t x) {
     uint32_t lo = 0, hi = s.blocks - 1;
@@ -77,13 +92,7 @@ ATLAS_HD inline AttnPlace attn_locate(const AttnSeq& s, uint32_t kv_heads, uint6
         if (s.before(mid) * kv_heads <= x) lo = mid;
         else hi = mid - 1;
     }
-    AttnPlace p;
-    p.block = lo;
-    p.tiles = s.tiles(lo);
-    const uint64_t in_block = x - s.before(lo) * kv_heads;
-    p.head = uint32_t(in_block / (s.extra + p.tiles));
-    p.place = uint32_t(in_block % (s.extra + p.tiles));
-    return p;
+    return attn_place_in_block(s, kv_heads, x, lo);
 }
 
 // The next item of a sequence's part of the line; false behind the last.
@@ -98,17 +107,17 @@ ATLAS_HD inline bool attn_next(const AttnSeq& s, uint32_t kv_heads, AttnPlace& p
 
 // Range c of `ranges` over a line of `total` places begins here; range_of: the one that place x belongs to.
 ATLAS_HD inline uint64_t attn_range_begin(uint64_t total, uint32_t ranges, uint32_t c) {
-    const uint64_t each = total / ranges, more = total % ranges;                          // the first `more` are one longer
+    const uint64_t each = attn_quotient(total, ranges), more = total - each * ranges;     // the first `more` are one longer
     return each * c + (c < more ? c : more);
 }
 ATLAS_HD inline uint32_t attn_range_of(uint64_t total, uint32_t ranges, uint64_t x) {
-    const uint64_t each = total / ranges, more = total % ranges;
+    const uint64_t each = attn_quotient(total, ranges), more = total - each * ranges;
     const uint64_t longer = more * (each + 1);
-    return x < longer ? uint32_t(x / (each + 1)) : uint32_t(more + (x - longer) / each);
+    return x < longer ? uint32_t(attn_quotient(x, each + 1)) : uint32_t(more + attn_quotient(x - longer, each));
 }
 // how many of the `ctas` CTAs take part where each is to have `least` places at least
 ATLAS_HD inline uint32_t attn_ranges(uint64_t total, uint32_t ctas, uint32_t least) {
-    const uint64_t n = (total + least - 1) / least;
+    const uint64_t n = attn_quotient(total + least - 1, least);
     return n < 1 ? 1u : n < ctas ? uint32_t(n) : ctas;
 }
 

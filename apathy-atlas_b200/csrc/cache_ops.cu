@@ -106,6 +106,8 @@ AttnParams attention_params(const atlas_b200_attention_desc& d) {
     p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(d.ws) + ATTN_CUT_BYTES);
     p.n_seqs = d.n_seqs; p.n_tokens = d.n_tokens; p.n_pages = d.n_pages; p.table_stride = d.table_stride;
     p.q_heads = d.q_heads; p.kv_heads = d.kv_heads; p.head_dim = d.head_dim; p.block_size = d.block_size; p.group = d.q_heads / d.kv_heads;
+    p.page_div = attn_divisor(d.block_size);
+    p.group_div = attn_divisor(p.group);
     p.q_row_stride = d.q_row_stride; p.out_row_stride = d.out_row_stride;
     p.scale = d.softmax_scale; p.k_scale = d.k_scale; p.v_scale = d.v_scale;
     return p;
@@ -125,11 +127,11 @@ struct MmaPlan {
 };
 MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms) {
     const uint32_t dim = attn_dim(d.head_dim);
-    const uint32_t row_bytes = dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u), resident = std::min(sms, ATTN_MAX_CTAS / 3) * uint32_t(attn::attn_mma_ctas(int(row_bytes), d.cache_dtype == ATLAS_B200_CACHE_E4M3));
     const uint64_t group = d.q_heads / d.kv_heads;
     const uint64_t rows = std::min<uint64_t>(d.max_q_len, d.n_tokens) * group;
     MmaPlan r{};
     r.block_rows = rows <= 8 ? 8u : 16u;
+    const uint32_t row_bytes = dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u), resident = std::min(sms, ATTN_MAX_CTAS / 3) * uint32_t(attn::attn_mma_ctas(int(row_bytes), d.cache_dtype == ATLAS_B200_CACHE_E4M3, r.block_rows == 8u ? 1 : 2));
     const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * std::max<uint64_t>((rows + r.block_rows - 1) / r.block_rows, 1);
     r.tile = uint32_t(attn::MMA_WARPS) * (row_bytes <= 128u ? 32u : 16u);
     const uint64_t tiles = std::max<uint64_t>((uint64_t(d.max_kv_len) + r.tile - 1) / r.tile, 1);
@@ -147,7 +149,7 @@ template <int DP, bool FP8, int RT> int launch_mma_rows(AttnParams p, const MmaP
     const int rc = allow_smem(attn::attn_mma_kernel<DP, FP8, RT>, C::SMEM, done);
     if (rc) return rc;
     p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.extra = MMA_EXTRA;
-    const int rc2 = launch_dependent(attn::attn_mma_kernel<DP, FP8, RT>, plan.ctas, attn::MMA_THREADS, C::SMEM, st, p, attn_divisor(p.block_size));
+    const int rc2 = launch_dependent(attn::attn_mma_kernel<DP, FP8, RT>, plan.ctas, attn::MMA_THREADS, C::SMEM, st, p);
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
     return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, p);
 }

@@ -23,6 +23,18 @@ namespace atlas {
 
 constexpr float ATTN_LOG2E = 1.4426950408889634f, ATTN_LN2 = 0.6931471805599453f;
 
+// page and place in it of a position: a product with a rounded-up reciprocal is exact for positions below 2^31 (checked at launch by
+// its construction: m = ceil(2^(31 + s) / d) with 2^s >= d)
+struct AttnDivisor {
+    uint32_t d, mul, shift;
+};
+__host__ __device__ inline AttnDivisor attn_divisor(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return AttnDivisor{d, uint32_t(((1ull << (31 + s)) + d - 1) / d), s};
+}
+__device__ __forceinline__ uint32_t attn_div(uint32_t x, const AttnDivisor& v) { return uint32_t((uint64_t(x) * v.mul) >> (31 + v.shift)); }
+
 struct AttnParams {
     const uint16_t* q;            // first column of row 0, rows q_row_stride elements apart
     uint16_t* out;
@@ -38,20 +50,9 @@ struct AttnParams {
     uint32_t ctas, least_tiles;   // ranges: at most `ctas`, of `least_tiles` tiles each at least
     uint32_t by_item;             // every CTA takes whole items: no pieces
     uint32_t extra;               // what an item costs besides its tiles, in tiles
+    AttnDivisor page_div, group_div;
     float scale, k_scale, v_scale;
 };
-
-// page and place in it of a position: a product with a rounded-up reciprocal is exact for positions below 2^31 (checked at launch by
-// its construction: m = ceil(2^(31 + s) / d) with 2^s >= d)
-struct AttnDivisor {
-    uint32_t d, mul, shift;
-};
-__host__ __device__ inline AttnDivisor attn_divisor(uint32_t d) {
-    uint32_t s = 0;
-    while ((1ull << s) < d) ++s;
-    return AttnDivisor{d, uint32_t(((1ull << (31 + s)) + d - 1) / d), s};
-}
-__device__ __forceinline__ uint32_t attn_div(uint32_t x, const AttnDivisor& v) { return uint32_t((uint64_t(x) * v.mul) >> (31 + v.shift)); }
 
 __host__ __device__ constexpr size_t attn_part_floats(uint32_t block_rows, uint32_t dim) { return size_t(block_rows) * dim + 2 * block_rows; }
 
@@ -90,10 +91,12 @@ __device__ __forceinline__ uint32_t attn_row_keys(const AttnSeqAt& s, uint32_t i
     return n <= s.q_len ? 0u : uint32_t(n - s.q_len);
 }
 
-// Length of the line, in places (tiles, or items where p.by_item), and the sequence that place `x` lies in.  By all THREADS threads of a
-// CTA; `sh`: THREADS / 32 + 3 words of 64 bits.
-struct AttnFound {
-    uint64_t total, seq_begin;    // seq_begin: the place where the sequence begins
+// Where a CTA's range of the line begins: worked out by one warp, while the others have nothing to do yet (all of them going through the
+// same divisions took twice as long), and left in shared memory.
+struct AttnStart {
+    uint64_t left;                // places of the range; 0: there is none
+    AttnPlace at;
+    AttnSeqAt sq;
     uint32_t seq;
 };
 __device__ __forceinline__ uint64_t attn_seq_places(const AttnParams& p, uint32_t s, uint32_t rows, uint32_t keys) {
@@ -101,43 +104,91 @@ __device__ __forceinline__ uint64_t attn_seq_places(const AttnParams& p, uint32_
     const AttnSeq a(q.q_len, q.kv_len, p.group, rows, keys, p.extra);
     return p.by_item ? uint64_t(a.blocks) * p.kv_heads : a.total(p.kv_heads);
 }
-template <int THREADS, typename F>
-__device__ __forceinline__ AttnFound attn_find(const AttnParams& p, uint32_t rows, uint32_t keys, uint64_t* sh, F place_of_total) {
-    constexpr int WARPS = THREADS / 32;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    const uint32_t each = (p.n_seqs + THREADS - 1) / THREADS, s0 = min(tid * each, p.n_seqs), s1 = min(s0 + each, p.n_seqs);
-    uint64_t mine = 0;
-    for (uint32_t s = s0; s < s1; ++s) mine += attn_seq_places(p, s, rows, keys);
-    uint64_t upto = mine;
+__device__ __forceinline__ uint64_t attn_warp_scan(uint64_t mine) {          // inclusive
+    const uint32_t lane = threadIdx.x & 31u;
 #pragma unroll
     for (uint32_t o = 1; o < 32; o <<= 1) {
-        const uint64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-        if (lane >= o) upto += v;
+        const uint64_t v = __shfl_up_sync(0xFFFFFFFFu, mine, o);
+        if (lane >= o) mine += v;
     }
-    if (lane == 31u) sh[warp] = upto;
-    __syncthreads();
-    uint64_t before = 0, total = 0;
-    for (int w = 0; w < WARPS; ++w) {
-        if (w < int(warp)) before += sh[w];
-        total += sh[w];
+    return mine;
+}
+// By one warp: the place `begin` of the sequence's part of the line, whose first place is seq_begin; and a note of the cut there.
+__device__ __forceinline__ void attn_begin_at(const AttnParams& p, uint32_t rows, uint32_t keys, uint64_t total, uint32_t n, uint64_t begin, uint64_t end, uint32_t seq,
+                                              uint64_t seq_begin, AttnStart* start) {
+    const uint32_t lane = threadIdx.x & 31u, c = blockIdx.x;
+    const AttnSeqAt sq = attn_seq(p, seq);
+    const AttnSeq plan(sq.q_len, sq.kv_len, p.group, rows, keys, p.extra);
+    const uint64_t x = begin - seq_begin;
+    AttnPlace at;
+    if (p.by_item) {
+        at.block = uint32_t(attn_quotient(x, p.kv_heads));
+        at.head = uint32_t(x - uint64_t(at.block) * p.kv_heads);
+        at.place = 0;
+        at.tiles = plan.tiles(at.block);
+    } else {
+        uint32_t lo = 0, hi = plan.blocks - 1;                               // the last block that begins at or before x: 32 looked at at once
+        while (lo < hi) {
+            const uint32_t step = (hi - lo + 31u) / 32u, mid = lo + (lane + 1u) * step;
+            const uint32_t past = __popc(__ballot_sync(0xFFFFFFFFu, mid <= hi && plan.before(mid) * p.kv_heads <= x));
+            lo += past * step;
+            hi = min(hi, lo + step - 1u);
+        }
+        at = attn_place_in_block(plan, p.kv_heads, x, lo);
     }
-    const uint64_t x = place_of_total(total);
-    const uint64_t end = before + upto, begin = end - mine;
-    if (mine && x >= begin && x < end) {                                                  // (one thread at most)
-        uint64_t at = begin;
-        for (uint32_t s = s0; s < s1; ++s) {
-            const uint64_t n = s1 - s0 == 1 ? mine : attn_seq_places(p, s, rows, keys);
-            if (x < at + n) { sh[WARPS] = s; sh[WARPS + 1] = at; break; }
-            at += n;
+    if (lane != 0) return;
+    start->left = end - begin;
+    start->at = at;
+    start->sq = sq;
+    start->seq = seq;
+    if (p.by_item) return;
+    const uint64_t first_tile = begin - at.place + p.extra;
+    AttnCut cut{0u, seq, at.block, at.head};
+    if (c > 0 && begin > first_tile && attn_range_begin(total, n, c - 1) <= first_tile) cut.pieces = attn_range_of(total, n, first_tile + at.tiles - 1) - c + 2u;
+    p.cuts[c] = cut;
+}
+// By all THREADS threads of a CTA; `sh`: THREADS / 32 words of 64 bits.  Ends with a barrier.
+constexpr uint32_t ATTN_WARP_SEQS = 256;
+template <int THREADS>
+__device__ __forceinline__ void attn_begin(const AttnParams& p, uint32_t rows, uint32_t keys, uint64_t* sh, AttnStart* start) {
+    constexpr uint32_t WARPS = THREADS / 32;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, c = blockIdx.x;
+    const bool few = p.n_seqs <= ATTN_WARP_SEQS;                             // one warp sums up the sequences too
+    if (!few || warp == 0) {
+        const uint32_t by = few ? 32u : uint32_t(THREADS), each = (p.n_seqs + by - 1) / by, s0 = min(tid * each, p.n_seqs), s1 = min(s0 + each, p.n_seqs);
+        uint64_t mine = 0;
+        for (uint32_t s = s0; s < s1; ++s) mine += attn_seq_places(p, s, rows, keys);
+        uint64_t upto = attn_warp_scan(mine), total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+        if (!few) {
+            if (lane == 31u) sh[warp] = upto;
+            __syncthreads();
+            total = 0;
+            for (uint32_t w = 0; w < WARPS; ++w) {
+                if (w < warp) upto += sh[w];
+                total += sh[w];
+            }
+        }
+        const uint32_t n = attn_ranges(total, p.ctas, p.least_tiles);
+        const uint64_t begin = c < n ? attn_range_begin(total, n, c) : 0, end = c < n ? attn_range_begin(total, n, c + 1) : 0;
+        if (begin == end) {
+            if (tid == 0) {
+                start->left = 0;
+                if (!p.by_item) p.cuts[c].pieces = 0;                        // more CTAs than ranges
+            }
+        } else {
+            const bool owns = mine && begin < upto && begin >= upto - mine;  // one lane of one warp
+            const uint32_t who = __ballot_sync(0xFFFFFFFFu, owns);
+            if (who) {
+                uint32_t seq = s0;
+                uint64_t at = upto - mine;
+                if (owns && s1 - s0 > 1)
+                    for (uint64_t k; seq + 1 < s1 && begin >= at + (k = attn_seq_places(p, seq, rows, keys)); ++seq) at += k;
+                const uint32_t lane_of = __ffs(who) - 1u;
+                attn_begin_at(p, rows, keys, total, n, begin, end, __shfl_sync(0xFFFFFFFFu, seq, lane_of), __shfl_sync(0xFFFFFFFFu, at, lane_of), start);
+            }
         }
     }
     __syncthreads();
-    AttnFound f;
-    f.total = total;
-    f.seq = uint32_t(sh[WARPS]);
-    f.seq_begin = sh[WARPS + 1];
-    __syncthreads();
-    return f;
 }
 
 // The items of one CTA's range, one after the other; every thread walks by itself.
@@ -146,24 +197,8 @@ struct AttnWalk {
     AttnPlace at;                 // of the item; its piece is tiles t0 .. t1 - 1
     uint32_t seq, t0, t1, rows, keys;
 
-    // (one thread of the CTA, whose range is not empty, at its first item)
-    __device__ __forceinline__ void note_cut(const AttnParams& p, const AttnFound& f, uint64_t begin) const {
-        if (p.by_item) return;
-        const uint32_t n = attn_ranges(f.total, p.ctas, p.least_tiles), c = blockIdx.x;
-        const uint64_t first_tile = begin - at.place + p.extra;
-        AttnCut cut{0u, seq, at.block, at.head};
-        if (c > 0 && begin > first_tile && attn_range_begin(f.total, n, c - 1) <= first_tile)
-            cut.pieces = attn_range_of(f.total, n, first_tile + at.tiles - 1) - c + 2u;
-        p.cuts[c] = cut;
-    }
-    __device__ __forceinline__ AttnWalk(const AttnParams& p, const AttnFound& f, uint64_t begin, uint64_t end, uint32_t block_rows, uint32_t tile_keys)
-        : seq(f.seq), rows(block_rows), keys(tile_keys), left_(end - begin), fresh_(true) {
-        if (!left_) return;
-        sq = attn_seq(p, seq);
-        const uint64_t x = begin - f.seq_begin;
-        if (p.by_item) { at.block = uint32_t(x / p.kv_heads); at.head = uint32_t(x % p.kv_heads); at.place = 0; at.tiles = plan(p).tiles(at.block); }
-        else at = attn_locate(plan(p), p.kv_heads, x);
-    }
+    __device__ __forceinline__ AttnWalk(const AttnStart& s, uint32_t block_rows, uint32_t tile_keys)
+        : sq(s.sq), at(s.at), seq(s.seq), t0(0), t1(0), rows(block_rows), keys(tile_keys), left_(s.left), fresh_(true) {}
     __device__ __forceinline__ AttnSeq plan(const AttnParams& p) const { return AttnSeq(sq.q_len, sq.kv_len, p.group, rows, keys, p.extra); }
     __device__ __forceinline__ bool next(const AttnParams& p) {
         if (!left_) return false;
@@ -193,8 +228,8 @@ private:
 };
 
 // Row `pos` of a sequence in the cache seen as [pages * block_size, kv_heads, head_dim]; -1 and a record where the table names no page.
-__device__ __forceinline__ int32_t attn_cache_row(const AttnParams& p, const AttnDivisor& div, const int32_t* table, uint32_t pos) {
-    const uint32_t page = attn_div(pos, div), id = uint32_t(table[page]);
+__device__ __forceinline__ int32_t attn_cache_row(const AttnParams& p, const int32_t* table, uint32_t pos) {
+    const uint32_t page = attn_div(pos, p.page_div), id = uint32_t(table[page]);
     if (id >= p.n_pages) { record_status(STATUS_PAGE_OUT_OF_RANGE); return -1; }
     return int32_t(id * p.block_size + (pos - page * p.block_size));
 }
@@ -209,14 +244,13 @@ __device__ __forceinline__ float attn_lse(float m, float l) { return l == 0.0f ?
 // values unread.  The cost (a chain over the row's keys) is paid by such rows only.
 static __device__ __noinline__ void attn_row_again(const AttnParams& p, bool fp8, uint32_t seq, uint32_t token, uint32_t head, uint32_t keys) {
     const uint32_t lane = threadIdx.x & 31u, D = p.head_dim;
-    const AttnDivisor div = attn_divisor(p.block_size);
     const int32_t* table = p.block_table + size_t(seq) * p.table_stride;
     const uint16_t* q = p.q + size_t(token) * p.q_row_stride + size_t(head) * D;
     float qv[8], o[8] = {}, m = -INFINITY, l = 0.0f;
     for (uint32_t i = 0; i < 8; ++i) qv[i] = lane + 32u * i < D ? __uint_as_float(uint32_t(q[lane + 32u * i]) << 16) : 0.0f;
     const float c = p.scale * p.k_scale * ATTN_LOG2E;
     for (uint32_t j = 0; j < keys; ++j) {
-        const int32_t row = attn_cache_row(p, div, table, j);
+        const int32_t row = attn_cache_row(p, table, j);
         const size_t at = (size_t(row < 0 ? 0 : row) * p.kv_heads + head / p.group) * D;
         float s = 0.0f, v[8];
         for (uint32_t i = 0; i < 8; ++i) {
@@ -298,7 +332,7 @@ __global__ void __launch_bounds__(ATTN_JOIN_THREADS, 4) attn_join_kernel(const _
     auto piece = [&](uint32_t i) { return i == 0 ? first : p.parts + part * (2 * size_t(c - 1 + i)); };
     auto place = [&](uint32_t r, uint32_t& in_seq, uint32_t& token, uint32_t& head) {
         const uint32_t row = cut.block * ROWS + r;
-        in_seq = row / p.group;
+        in_seq = attn_div(row, p.group_div);
         token = sq.row0 + in_seq;
         head = cut.head * p.group + row - in_seq * p.group;
     };

@@ -22,7 +22,8 @@
 namespace atlas {
 namespace attn {
 
-constexpr int attn_mma_ctas(int row_bytes, bool fp8) { return row_bytes >= 512 ? 1 : row_bytes > 128 && !fp8 ? 2 : 3; }
+// (heads of 256 over E4M3 in blocks of sixteen rows have 128 accumulators: two)
+constexpr int attn_mma_ctas(int row_bytes, bool fp8, int rt) { return row_bytes >= 512 ? 1 : row_bytes > 128 && (!fp8 || rt == 2) ? 2 : 3; }
 constexpr int MMA_WARPS = 4, MMA_THREADS = 32 * MMA_WARPS;
 
 template <int DP, bool FP8, int RT> struct MmaCfg {
@@ -34,13 +35,13 @@ template <int DP, bool FP8, int RT> struct MmaCfg {
     // CTAs on an SM, and the ring as deep as that leaves room for.  Short rows and conversions mean more arithmetic for a byte, so three:
     // what a unit waits for is its own instructions (256 sequences of up to 4096 over E4M3: 278 us with two, 252 with three; with units of
     // 16 tokens 299, and 290 with four CTAs).
-    static constexpr int CTAS = attn_mma_ctas(ROW_BYTES, FP8);
+    static constexpr int CTAS = attn_mma_ctas(ROW_BYTES, FP8, RT);
     static constexpr int RING_BYTES = CTAS == 1 ? 196608 : CTAS == 2 ? 98304 : 65536;
     static constexpr int STAGES = RING_BYTES / MMA_WARPS / (2 * SIDE) > 8 ? 8 : RING_BYTES / MMA_WARPS / (2 * SIDE);
     static constexpr int RING = MMA_WARPS * STAGES * 2 * SIDE;
     static constexpr int JOIN = MMA_WARPS * ROWS * (DP + 4) * 4;         // (overlaid)
     static constexpr int MAIN = RING > JOIN ? RING : JOIN;
-    static constexpr int SMEM = MAIN + MMA_WARPS * ROWS * 8 + 16 * 8;
+    static constexpr int SMEM = MAIN + MMA_WARPS * ROWS * 8 + MMA_WARPS * 8 + int(sizeof(AttnStart));
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -84,7 +85,7 @@ template <int ROW_BYTES> __device__ __forceinline__ uint32_t unit_off(uint32_t t
 }
 
 template <int DP, bool FP8, int RT>
-__global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_mma_kernel(const __grid_constant__ AttnParams p, const AttnDivisor div) {
+__global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_mma_kernel(const __grid_constant__ AttnParams p) {
     using C = MmaCfg<DP, FP8, RT>;
     constexpr int MT = DP / 16, KS = DP / 16, UT = C::UNIT / 16;             // sixteen channels of the output; K steps of the scores; sixteen tokens of a unit
     constexpr int MMA_ROWS = C::ROWS;
@@ -97,24 +98,16 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_m
     pdl_wait();
     pdl_release();
 
-    uint64_t x = 0, x_end = 0;
-    const AttnFound f = attn_find<MMA_THREADS>(p, MMA_ROWS, C::TILE, sh, [&](uint64_t total) {
-        const uint32_t n = attn_ranges(total, p.ctas, p.least_tiles);
-        if (blockIdx.x < n) { x = attn_range_begin(total, n, blockIdx.x); x_end = attn_range_begin(total, n, blockIdx.x + 1); }
-        return x < x_end ? x : ~0ull;
-    });
-    AttnWalk walk(p, f, x, x_end, MMA_ROWS, C::TILE);
-    if (tid == 0 && !p.by_item) {
-        if (x < x_end) walk.note_cut(p, f, x);
-        else p.cuts[blockIdx.x].pieces = 0;                                  // more CTAs than ranges
-    }
+    AttnStart* const start = reinterpret_cast<AttnStart*>(sh + MMA_WARPS);
+    attn_begin<MMA_THREADS>(p, MMA_ROWS, C::TILE, sh, start);
+    AttnWalk walk(*start, MMA_ROWS, C::TILE);
     while (walk.next(p)) {
         const AttnSeqAt sq = walk.sq;
         const AttnPlace at = walk.at;
         const uint32_t seq = walk.seq, t0 = walk.t0, t1 = walk.t1;
         const uint32_t rows_left = sq.q_len * p.group - at.block * MMA_ROWS, rows = min(rows_left, uint32_t(MMA_ROWS));
 
-        const uint32_t last_tok = (at.block * MMA_ROWS + rows - 1) / p.group, first_tok = at.block * MMA_ROWS / p.group;
+        const uint32_t last_tok = attn_div(at.block * MMA_ROWS + rows - 1, p.group_div), first_tok = attn_div(at.block * MMA_ROWS, p.group_div);
         const uint32_t all_see = attn_row_keys(sq, first_tok), n_keys = attn_row_keys(sq, last_tok);
 
         // the cache rows of a unit: lane l finds that of token l
@@ -122,7 +115,7 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_m
         const uint32_t units = t1 - t0, pos_w = t0 * C::TILE + warp * C::UNIT;
         auto find_row = [&](uint32_t u) -> int32_t {
             const uint32_t pos = pos_w + u * C::TILE + lane;
-            return u < units && lane < uint32_t(C::UNIT) && pos < n_keys ? attn_cache_row(p, div, table, pos) : -1;
+            return u < units && lane < uint32_t(C::UNIT) && pos < n_keys ? attn_cache_row(p, table, pos) : -1;
         };
         constexpr uint32_t CH = C::ROW_BYTES / 16;                      // 16-byte chunks of a row
         const size_t head_at = size_t(at.head) * D * size, row_bytes = size_t(p.kv_heads) * D * size;
@@ -157,8 +150,8 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_m
         float c_row[RT][2];                                                  // of this lane's scores: rows 2 q4 and 2 q4 + 1
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            const uint32_t r = 8u * t + g, row = at.block * MMA_ROWS + r, tok = row / p.group;
-            const uint16_t* q_row = r < rows ? p.q + size_t(sq.row0 + tok) * p.q_row_stride + size_t(at.head * p.group + row % p.group) * D : nullptr;
+            const uint32_t r = 8u * t + g, row = at.block * MMA_ROWS + r, tok = attn_div(row, p.group_div);
+            const uint16_t* q_row = r < rows ? p.q + size_t(sq.row0 + tok) * p.q_row_stride + size_t(at.head * p.group + row - tok * p.group) * D : nullptr;
             uint32_t top = 0;
 #pragma unroll
             for (int s = 0; s < KS; ++s)
@@ -187,7 +180,7 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_m
             for (uint32_t e = 0; e < 2; ++e) {
                 const uint32_t mine = 8u * t + 2u * q4 + e;
                 c_row[t][e] = FP8 ? __shfl_sync(0xFFFFFFFFu, c, 4u * (2u * q4 + e)) : c;
-                keys[t][e] = mine < rows ? attn_row_keys(sq, (at.block * MMA_ROWS + mine) / p.group) : 0u;
+                keys[t][e] = mine < rows ? attn_row_keys(sq, attn_div(at.block * MMA_ROWS + mine, p.group_div)) : 0u;
             }
         }
 
@@ -371,7 +364,7 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_m
                 if (lane == 0) { part[size_t(MMA_ROWS) * DP + r] = top; part[size_t(MMA_ROWS) * DP + MMA_ROWS + r] = total; }
                 continue;
             }
-            const uint32_t row = at.block * MMA_ROWS + r, tok = row / p.group, head = at.head * p.group + row % p.group;
+            const uint32_t row = at.block * MMA_ROWS + r, tok = attn_div(row, p.group_div), head = at.head * p.group + row - tok * p.group;
             const float inv = total == 0.0f ? 0.0f : p.v_scale / total;
             bool odd = false;
 #pragma unroll

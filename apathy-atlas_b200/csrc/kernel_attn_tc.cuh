@@ -53,7 +53,7 @@ template <int DP, bool FP8> struct TcCfg {
     static constexpr int OFF_BAR = OFF_SCALE + (FP8 ? ROWS * 4 : 0);
     static constexpr int N_BAR = 2 * SLOTS + 1 + 7 * NQ + 2 * RAW_STAGES;
     static constexpr int OFF_MISC = OFF_BAR + N_BAR * 8;                     // tensor memory, -, abort; attn_find's words
-    static constexpr int SMEM = OFF_MISC + 16 + 20 * 8 + 1024;
+    static constexpr int SMEM = OFF_MISC + 16 + 16 * 8 + int(sizeof(AttnStart)) + 1024;
     static constexpr int SOFT_WARPS = 4 * NQ, WARPS = 4 + SOFT_WARPS + (FP8 ? 4 : 0), THREADS = 32 * WARPS;
     static constexpr int CONV_WARP0 = 4 + SOFT_WARPS;
     static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -145,17 +145,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     pdl_wait();
     pdl_release();
 
-    uint64_t x = 0, x_end = 0;
-    const AttnFound found = attn_find<C::THREADS>(p, C::ROWS, TC_KEYS, sh, [&](uint64_t total) {
-        const uint32_t n = attn_ranges(total, p.ctas, p.least_tiles);
-        if (blockIdx.x < n) { x = attn_range_begin(total, n, blockIdx.x); x_end = attn_range_begin(total, n, blockIdx.x + 1); }
-        return x < x_end ? x : ~0ull;
-    });
-    AttnWalk walk(p, found, x, x_end, C::ROWS, TC_KEYS);
-    if (tid == 64 && !p.by_item) {
-        if (x < x_end) walk.note_cut(p, found, x);
-        else p.cuts[blockIdx.x].pieces = 0;                                  // more CTAs than ranges
-    }
+    AttnStart* const start = reinterpret_cast<AttnStart*>(sh + C::WARPS);
+    attn_begin<C::THREADS>(p, C::ROWS, TC_KEYS, sh, start);
+    AttnWalk walk(*start, C::ROWS, TC_KEYS);
     // rows of a row tile of the item, and the steps that it takes of the piece
     auto tile_rows = [&](uint32_t g) {
         const uint32_t all = walk.sq.q_len * p.group, r0 = walk.at.block * C::ROWS + g * TC_TILE_ROWS;
@@ -164,7 +156,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     auto steps_of = [&](uint32_t g) {
         const uint32_t rows = tile_rows(g);
         if (rows == 0) return 0u;
-        const uint32_t keys = attn_row_keys(walk.sq, (walk.at.block * C::ROWS + g * TC_TILE_ROWS + rows - 1) / p.group);
+        const uint32_t keys = attn_row_keys(walk.sq, attn_div(walk.at.block * C::ROWS + g * TC_TILE_ROWS + rows - 1, p.group_div));
         const uint32_t t = min(max((keys + TC_STEP - 1) / TC_STEP, 1u), 2u * walk.t1);
         return t > 2u * walk.t0 ? t - 2u * walk.t0 : 0u;
     };
@@ -175,7 +167,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         if (warp == 0) {
             // ---- TMA: K and V of a tile, one lane a box ----
             const uint32_t per_tile = TC_KEYS / box_rows;
-            const AttnDivisor div = attn_divisor(p.block_size);
+            const AttnDivisor div = p.page_div;
             uint32_t slot = 0, ph = 0, tail_ph = 0, rs = 0, rph = 0;
             bool ok = true;
             while (ok && walk.next(p)) {
@@ -326,7 +318,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             while (walk.next(p)) {
                 const uint32_t row0 = walk.at.block * C::ROWS, rows = tile_rows(0) + (NQ == 2 ? tile_rows(NQ - 1) : 0u), lines = (p.head_dim * 2u + 127u) / 128u;
                 for (uint32_t i = t; i < rows * lines; i += all) {
-                    const uint32_t row = row0 + i / lines, tok = row / p.group;
+                    const uint32_t row = row0 + i / lines, tok = attn_div(row, p.group_div);
                     const uint16_t* at = p.q + size_t(walk.sq.row0 + tok) * p.q_row_stride + size_t(walk.at.head * p.group + row - tok * p.group) * p.head_dim + (i % lines) * 64u;
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
                 }
@@ -339,14 +331,15 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const uint32_t q_tile = base + C::OFF_Q + g * C::TILE;
         float* const scale_s = reinterpret_cast<float*>(gen + C::OFF_SCALE) + g * TC_TILE_ROWS;
         const uint32_t D = p.head_dim;
-        const AttnDivisor group_div = attn_divisor(p.group);
+        const AttnDivisor group_div = p.group_div;
         uint32_t s_ph[2] = {0, 0};                                           // of the next step's barriers, and of the ones after
-        // Q of the item that the walk is at: this warp's 32 rows, sixteen bytes a lane, all loads in flight.  (The item before has had its
-        // last scores computed.)
+        // Q of the item that the walk is at: this warp's 32 rows, sixteen bytes a lane, eight loads in flight.  (The item before has had its
+        // last scores computed.  All sixteen in flight were a thousand instructions in a row, which a CTA has to fetch before its first
+        // scores: 6 to 26 thousand cycles.)
         auto load_q = [&] {
             const uint32_t rows = tile_rows(g), row0 = walk.at.block * C::ROWS + g * TC_TILE_ROWS;
             if (rows == 0 || steps_of(g) == 0) return;
-            constexpr uint32_t CH = DP / 8, LOADS = CH < 16 ? CH : 16;
+            constexpr uint32_t CH = DP / 8, LOADS = 8;
             const uint16_t* const q_head = p.q + size_t(walk.sq.row0) * p.q_row_stride + size_t(walk.at.head) * p.group * D;
 #pragma unroll 1
             for (uint32_t i0 = 0; i0 < CH; i0 += LOADS) {
@@ -388,7 +381,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const uint32_t n = steps_of(g), rows = tile_rows(g), row0 = walk.at.block * C::ROWS + g * TC_TILE_ROWS, seq = walk.seq, t0 = walk.t0, seq_row0 = walk.sq.row0;
             const bool whole = walk.whole();
             const uint32_t row = row0 + row_in, tok = attn_div(row, group_div), head = walk.at.head * p.group + row - tok * p.group;
-            const uint32_t keys = row_in < rows ? attn_row_keys(walk.sq, tok) : 0u, all_see = attn_row_keys(walk.sq, row0 / p.group);
+            const uint32_t keys = row_in < rows ? attn_row_keys(walk.sq, tok) : 0u, all_see = attn_row_keys(walk.sq, attn_div(row0, group_div));
             float c = p.scale * p.k_scale * ATTN_LOG2E, m = -INFINITY, l = 0.0f;
             if constexpr (FP8) {
                 if (n) c *= scale_s[row_in];
