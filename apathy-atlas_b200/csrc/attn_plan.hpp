@@ -21,8 +21,18 @@
 
 namespace atlas {
 
-// A quotient, in 32 bits where both numbers have no more: a GPU divides those in a tenth of the time, and the numbers of a plan, which
-// every CTA works out before it can ask for its first key, nearly always have.
+// Quotients by a number that the host knows: a product with the rounded-up reciprocal, exact for numbers below 2^31
+// (mul d = 2^(31 + shift) + e with e < d <= 2^shift, so x e < 2^(31 + shift)).
+struct AttnDivisor {
+    uint32_t d, mul, shift;
+};
+ATLAS_HD inline AttnDivisor attn_divisor(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return AttnDivisor{d, uint32_t(((1ull << (31 + s)) + d - 1) / d), s};
+}
+ATLAS_HD inline uint32_t attn_div(uint32_t x, const AttnDivisor& v) { return uint32_t((uint64_t(x) * v.mul) >> (31 + v.shift)); }
+// Others: in 32 bits where both numbers have no more, which a GPU divides in a tenth of the time.
 ATLAS_HD inline uint64_t attn_quotient(uint64_t a, uint64_t b) { return ((a | b) >> 32) == 0 ? uint64_t(uint32_t(a) / uint32_t(b)) : a / b; }
 
 // sum of floor((a i + b) / m) over i = 0 .. n - 1, by Euclid's algorithm on (a, m)
@@ -42,31 +52,54 @@ ATLAS_HD inline uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t 
     return sum;
 }
 
+// What is the same for all sequences of a call.  With R = 2^rows_log2 rows of a block and group * 2^keys_log2 = K: the tiles of block b are
+// floor((R b + c) / K), c from the sequence.  Where K = P R that is floor((b + floor(c / R)) / P), and the sum over blocks has a closed
+// form with one quotient by P, which the host knows; otherwise (an odd group of three or more over blocks of more rows than a tile has keys,
+// or numbers beyond 31 bits) it is floor_sum.  Every CTA works out where its range begins before it can ask for its first key: 9000
+// cycles by floor_sum.
+struct AttnShape {
+    uint32_t group, rows_log2, keys_log2, extra;
+    uint32_t closed;                            // P is a whole number, and what it divides stays below 2^31
+    AttnDivisor per;                            // P
+};
+// most_keys: no sequence has more
+ATLAS_HD inline AttnShape attn_shape(uint32_t group, uint32_t rows_log2, uint32_t keys_log2, uint32_t extra, uint64_t most_keys, uint64_t most_rows) {
+    const uint64_t k = uint64_t(group) << keys_log2, p = k >> rows_log2;
+    const bool closed = (p << rows_log2) == k && p > 0 && p < (1ull << 31) && ((((most_keys + (1ull << keys_log2)) * group + most_rows) >> rows_log2) + 2) < (1ull << 31);
+    return AttnShape{group, rows_log2, keys_log2, extra, closed ? 1u : 0u, attn_divisor(closed ? uint32_t(p) : 1u)};
+}
+
 // One sequence's blocks.  Without new tokens it has none; with fewer cached tokens than new ones (the first rows see nothing) all of
 // its blocks count as if they saw the whole cache.
 struct AttnSeq {
     uint32_t q_len, kv_len, blocks, whole;      // whole: tiles of the cached tokens, one at least
-    uint32_t group, block_rows, tile_keys, extra;
-    ATLAS_HD AttnSeq(uint32_t q, uint32_t kv, uint32_t g, uint32_t rows, uint32_t keys, uint32_t more)
-        : q_len(q), kv_len(kv), group(g), block_rows(rows), tile_keys(keys), extra(more) {
-        blocks = uint32_t(attn_quotient(uint64_t(q) * g + rows - 1, rows));
-        whole = kv ? (kv - 1) / keys + 1 : 1;
+    uint32_t first;                             // floor(c / R)
+    AttnShape sh;
+    ATLAS_HD AttnSeq(uint32_t q, uint32_t kv, const AttnShape& shape) : q_len(q), kv_len(kv), sh(shape) {
+        const uint32_t rows = 1u << sh.rows_log2;
+        blocks = uint32_t((uint64_t(q) * sh.group + rows - 1) >> sh.rows_log2);
+        whole = kv ? ((kv - 1) >> sh.keys_log2) + 1 : 1;
+        first = uint32_t(numerator() >> sh.rows_log2);
     }
-    // the last row of block b is row (b + 1) rows - 1, token floor of it / group; it sees kv_len - q_len + that token + 1 keys
+    // of block 0: its last row is row R - 1, token floor of that / group; it sees kv_len - q_len + that token + 1 keys
+    ATLAS_HD uint64_t numerator() const { return ((1u << sh.rows_log2) - 1u) + uint64_t(sh.group) * (uint64_t(kv_len - q_len) + (1u << sh.keys_log2)); }
     ATLAS_HD uint32_t tiles(uint32_t b) const {
         if (kv_len < q_len || b + 1 >= blocks) return whole;
-        const uint64_t keys_less_1 = uint64_t(kv_len - q_len) + tile_keys;
-        const uint64_t t = attn_quotient(uint64_t(block_rows) * b + block_rows - 1 + uint64_t(group) * keys_less_1, uint64_t(group) * tile_keys);
+        const uint64_t t = sh.closed ? attn_div(first + b, sh.per) : attn_quotient((uint64_t(b) << sh.rows_log2) + numerator(), uint64_t(sh.group) << sh.keys_log2);
         return t < whole ? uint32_t(t) : whole;
+    }
+    // sum of floor(i / P) over i = 0 .. x - 1
+    ATLAS_HD uint64_t upto(uint32_t x) const {
+        const uint64_t q = attn_div(x, sh.per);
+        return sh.per.d * (q * (q - 1) / 2) + q * (x - q * sh.per.d);
     }
     // places of the blocks before b, of one KV head
     ATLAS_HD uint64_t before(uint32_t b) const {
         if (b == 0 || blocks == 0) return 0;
-        if (blocks == 1) return uint64_t(whole) + extra;
         const uint32_t n = b < blocks ? b : blocks - 1;                                   // by the formula
-        uint64_t sum = kv_len < q_len ? uint64_t(whole) * n
-                                      : floor_sum(n, uint64_t(group) * tile_keys, block_rows, block_rows - 1 + uint64_t(group) * (uint64_t(kv_len - q_len) + tile_keys));
-        return (b < blocks ? sum : sum + whole) + uint64_t(b) * extra;
+        const uint64_t sum = n == 0 ? 0 : kv_len < q_len ? uint64_t(whole) * n : sh.closed ? upto(first + n) - upto(first)
+                                      : floor_sum(n, uint64_t(sh.group) << sh.keys_log2, 1u << sh.rows_log2, numerator());
+        return (b < blocks ? sum : sum + whole) + uint64_t(b) * sh.extra;
     }
     ATLAS_HD uint64_t total(uint32_t kv_heads) const { return before(blocks) * kv_heads; }
 };
@@ -74,14 +107,14 @@ struct AttnSeq {
 struct AttnPlace {
     uint32_t block, head, place, tiles;         // place within the item, which has extra + tiles of them
 };
-// where place x lies, known to be in a block
+// where place x of a sequence's part of the line lies, known to be in a block
 ATLAS_HD inline AttnPlace attn_place_in_block(const AttnSeq& s, uint32_t kv_heads, uint64_t x, uint32_t block) {
     AttnPlace p;
     p.block = block;
     p.tiles = s.tiles(block);
     const uint64_t in_block = x - s.before(block) * kv_heads;
-    p.head = uint32_t(attn_quotient(in_block, s.extra + p.tiles));
-    p.place = uint32_t(in_block - uint64_t(p.head) * (s.extra + p.tiles));
+    p.head = kv_heads == 1 ? 0u : uint32_t(attn_quotient(in_block, s.sh.extra + p.tiles));
+    p.place = uint32_t(in_block - uint64_t(p.head) * (s.sh.extra + p.tiles));
     return p;
 }
 // where place x of a sequence's part of the line lies, x < total(kv_heads)
@@ -105,20 +138,22 @@ ATLAS_HD inline bool attn_next(const AttnSeq& s, uint32_t kv_heads, AttnPlace& p
     return true;
 }
 
-// Range c of `ranges` over a line of `total` places begins here; range_of: the one that place x belongs to.
-ATLAS_HD inline uint64_t attn_range_begin(uint64_t total, uint32_t ranges, uint32_t c) {
-    const uint64_t each = attn_quotient(total, ranges), more = total - each * ranges;     // the first `more` are one longer
-    return each * c + (c < more ? c : more);
-}
-ATLAS_HD inline uint32_t attn_range_of(uint64_t total, uint32_t ranges, uint64_t x) {
-    const uint64_t each = attn_quotient(total, ranges), more = total - each * ranges;
-    const uint64_t longer = more * (each + 1);
-    return x < longer ? uint32_t(attn_quotient(x, each + 1)) : uint32_t(more + attn_quotient(x - longer, each));
-}
-// how many of the `ctas` CTAs take part where each is to have `least` places at least
-ATLAS_HD inline uint32_t attn_ranges(uint64_t total, uint32_t ctas, uint32_t least) {
-    const uint64_t n = attn_quotient(total + least - 1, least);
-    return n < 1 ? 1u : n < ctas ? uint32_t(n) : ctas;
-}
+// A line of `total` places, cut into as many ranges as there are CTAs, or fewer where each is to have `least` places at least.  The
+// first `more` are one place longer.
+struct AttnRanges {
+    uint64_t total, each, more;
+    uint32_t n;
+    ATLAS_HD AttnRanges(uint64_t places, uint32_t ctas, uint32_t least) : total(places) {
+        n = total >= uint64_t(ctas) * least ? ctas : total <= least ? 1u : uint32_t(attn_quotient(total + least - 1, least));
+        each = attn_quotient(total, n);
+        more = total - each * n;
+    }
+    ATLAS_HD uint64_t begin(uint32_t c) const { return each * c + (c < more ? c : more); }
+    // the range that place x belongs to
+    ATLAS_HD uint32_t of(uint64_t x) const {
+        const uint64_t longer = more * (each + 1);
+        return x < longer ? uint32_t(attn_quotient(x, each + 1)) : uint32_t(more + attn_quotient(x - longer, each));
+    }
+};
 
 }  // namespace atlas

@@ -120,6 +120,11 @@ AttnParams attention_params(const atlas_b200_attention_desc& d) {
 #endif
 constexpr uint32_t MMA_EXTRA = MMA_EXTRA_, TC_EXTRA = TC_EXTRA_;
 
+constexpr uint32_t log2_of(uint32_t n) { return n <= 1 ? 0u : 1u + log2_of(n / 2); }
+AttnShape shape_of(const AttnParams& p, uint32_t rows, uint32_t keys, uint32_t extra) {
+    return attn_shape(p.group, log2_of(rows), log2_of(keys), extra, uint64_t(p.table_stride) * p.block_size, uint64_t(p.n_tokens) * p.group);
+}
+
 // The mma.sync form: how many CTAs, and whether each takes whole items.
 struct MmaPlan {
     uint32_t ctas, by_item, least, tile, block_rows;
@@ -148,7 +153,7 @@ template <int DP, bool FP8, int RT> int launch_mma_rows(AttnParams p, const MmaP
     static std::atomic<bool> done[kMaxDevices] = {};
     const int rc = allow_smem(attn::attn_mma_kernel<DP, FP8, RT>, C::SMEM, done);
     if (rc) return rc;
-    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.extra = MMA_EXTRA;
+    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.shape = shape_of(p, C::ROWS, C::TILE, MMA_EXTRA);
     const int rc2 = launch_dependent(attn::attn_mma_kernel<DP, FP8, RT>, plan.ctas, attn::MMA_THREADS, C::SMEM, st, p);
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
     return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, p);
@@ -206,7 +211,7 @@ template <int DP, bool FP8> int launch_tc(AttnParams p, const TcPlan& plan, cuda
     const CUtensorMapSwizzle swz = FP8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
     if (!encode_tensor_map(&map_k, dt, 3, p.k_cache, dims, strides, box, swz) || !encode_tensor_map(&map_v, dt, 3, p.v_cache, dims, strides, box, swz))
         return ATLAS_B200_ERR_DIMS;
-    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.extra = TC_EXTRA;
+    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.shape = shape_of(p, C::ROWS, attn::TC_KEYS, TC_EXTRA);
     const int rc2 = launch_dependent(attn::attn_tc_kernel<DP, FP8>, plan.ctas, C::THREADS, C::SMEM, st, map_k, map_v, p, plan.box_rows);
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
     return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, p);

@@ -23,18 +23,6 @@ namespace atlas {
 
 constexpr float ATTN_LOG2E = 1.4426950408889634f, ATTN_LN2 = 0.6931471805599453f;
 
-// page and place in it of a position: a product with a rounded-up reciprocal is exact for positions below 2^31 (checked at launch by
-// its construction: m = ceil(2^(31 + s) / d) with 2^s >= d)
-struct AttnDivisor {
-    uint32_t d, mul, shift;
-};
-__host__ __device__ inline AttnDivisor attn_divisor(uint32_t d) {
-    uint32_t s = 0;
-    while ((1ull << s) < d) ++s;
-    return AttnDivisor{d, uint32_t(((1ull << (31 + s)) + d - 1) / d), s};
-}
-__device__ __forceinline__ uint32_t attn_div(uint32_t x, const AttnDivisor& v) { return uint32_t((uint64_t(x) * v.mul) >> (31 + v.shift)); }
-
 struct AttnParams {
     const uint16_t* q;            // first column of row 0, rows q_row_stride elements apart
     uint16_t* out;
@@ -49,7 +37,7 @@ struct AttnParams {
     uint32_t n_seqs, n_tokens, n_pages, table_stride, q_heads, kv_heads, head_dim, block_size, group, q_row_stride, out_row_stride;
     uint32_t ctas, least_tiles;   // ranges: at most `ctas`, of `least_tiles` tiles each at least
     uint32_t by_item;             // every CTA takes whole items: no pieces
-    uint32_t extra;               // what an item costs besides its tiles, in tiles
+    AttnShape shape;              // of the kernel's blocks and tiles
     AttnDivisor page_div, group_div;
     float scale, k_scale, v_scale;
 };
@@ -99,9 +87,9 @@ struct AttnStart {
     AttnSeqAt sq;
     uint32_t seq;
 };
-__device__ __forceinline__ uint64_t attn_seq_places(const AttnParams& p, uint32_t s, uint32_t rows, uint32_t keys) {
+__device__ __forceinline__ uint64_t attn_seq_places(const AttnParams& p, uint32_t s) {
     const AttnSeqAt q = attn_seq(p, s);
-    const AttnSeq a(q.q_len, q.kv_len, p.group, rows, keys, p.extra);
+    const AttnSeq a(q.q_len, q.kv_len, p.shape);
     return p.by_item ? uint64_t(a.blocks) * p.kv_heads : a.total(p.kv_heads);
 }
 __device__ __forceinline__ uint64_t attn_warp_scan(uint64_t mine) {          // inclusive
@@ -114,11 +102,10 @@ __device__ __forceinline__ uint64_t attn_warp_scan(uint64_t mine) {          // 
     return mine;
 }
 // By one warp: the place `begin` of the sequence's part of the line, whose first place is seq_begin; and a note of the cut there.
-__device__ __forceinline__ void attn_begin_at(const AttnParams& p, uint32_t rows, uint32_t keys, uint64_t total, uint32_t n, uint64_t begin, uint64_t end, uint32_t seq,
-                                              uint64_t seq_begin, AttnStart* start) {
+__device__ __forceinline__ void attn_begin_at(const AttnParams& p, const AttnRanges& ranges, uint64_t begin, uint64_t end, uint32_t seq, uint64_t seq_begin, AttnStart* start) {
     const uint32_t lane = threadIdx.x & 31u, c = blockIdx.x;
     const AttnSeqAt sq = attn_seq(p, seq);
-    const AttnSeq plan(sq.q_len, sq.kv_len, p.group, rows, keys, p.extra);
+    const AttnSeq plan(sq.q_len, sq.kv_len, p.shape);
     const uint64_t x = begin - seq_begin;
     AttnPlace at;
     if (p.by_item) {
@@ -142,22 +129,22 @@ __device__ __forceinline__ void attn_begin_at(const AttnParams& p, uint32_t rows
     start->sq = sq;
     start->seq = seq;
     if (p.by_item) return;
-    const uint64_t first_tile = begin - at.place + p.extra;
+    const uint64_t first_tile = begin - at.place + p.shape.extra;
     AttnCut cut{0u, seq, at.block, at.head};
-    if (c > 0 && begin > first_tile && attn_range_begin(total, n, c - 1) <= first_tile) cut.pieces = attn_range_of(total, n, first_tile + at.tiles - 1) - c + 2u;
+    if (c > 0 && begin > first_tile && ranges.begin(c - 1) <= first_tile) cut.pieces = ranges.of(first_tile + at.tiles - 1) - c + 2u;
     p.cuts[c] = cut;
 }
 // By all THREADS threads of a CTA; `sh`: THREADS / 32 words of 64 bits.  Ends with a barrier.
 constexpr uint32_t ATTN_WARP_SEQS = 256;
 template <int THREADS>
-__device__ __forceinline__ void attn_begin(const AttnParams& p, uint32_t rows, uint32_t keys, uint64_t* sh, AttnStart* start) {
+__device__ __forceinline__ void attn_begin(const AttnParams& p, uint64_t* sh, AttnStart* start) {
     constexpr uint32_t WARPS = THREADS / 32;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, c = blockIdx.x;
     const bool few = p.n_seqs <= ATTN_WARP_SEQS;                             // one warp sums up the sequences too
     if (!few || warp == 0) {
         const uint32_t by = few ? 32u : uint32_t(THREADS), each = (p.n_seqs + by - 1) / by, s0 = min(tid * each, p.n_seqs), s1 = min(s0 + each, p.n_seqs);
         uint64_t mine = 0;
-        for (uint32_t s = s0; s < s1; ++s) mine += attn_seq_places(p, s, rows, keys);
+        for (uint32_t s = s0; s < s1; ++s) mine += attn_seq_places(p, s);
         uint64_t upto = attn_warp_scan(mine), total = __shfl_sync(0xFFFFFFFFu, upto, 31);
         if (!few) {
             if (lane == 31u) sh[warp] = upto;
@@ -168,8 +155,8 @@ __device__ __forceinline__ void attn_begin(const AttnParams& p, uint32_t rows, u
                 total += sh[w];
             }
         }
-        const uint32_t n = attn_ranges(total, p.ctas, p.least_tiles);
-        const uint64_t begin = c < n ? attn_range_begin(total, n, c) : 0, end = c < n ? attn_range_begin(total, n, c + 1) : 0;
+        const AttnRanges ranges(total, p.ctas, p.least_tiles);
+        const uint64_t begin = c < ranges.n ? ranges.begin(c) : 0, end = c < ranges.n ? ranges.begin(c + 1) : 0;
         if (begin == end) {
             if (tid == 0) {
                 start->left = 0;
@@ -182,9 +169,9 @@ __device__ __forceinline__ void attn_begin(const AttnParams& p, uint32_t rows, u
                 uint32_t seq = s0;
                 uint64_t at = upto - mine;
                 if (owns && s1 - s0 > 1)
-                    for (uint64_t k; seq + 1 < s1 && begin >= at + (k = attn_seq_places(p, seq, rows, keys)); ++seq) at += k;
+                    for (uint64_t k; seq + 1 < s1 && begin >= at + (k = attn_seq_places(p, seq)); ++seq) at += k;
                 const uint32_t lane_of = __ffs(who) - 1u;
-                attn_begin_at(p, rows, keys, total, n, begin, end, __shfl_sync(0xFFFFFFFFu, seq, lane_of), __shfl_sync(0xFFFFFFFFu, at, lane_of), start);
+                attn_begin_at(p, ranges, begin, end, __shfl_sync(0xFFFFFFFFu, seq, lane_of), __shfl_sync(0xFFFFFFFFu, at, lane_of), start);
             }
         }
     }
@@ -195,11 +182,10 @@ __device__ __forceinline__ void attn_begin(const AttnParams& p, uint32_t rows, u
 struct AttnWalk {
     AttnSeqAt sq;
     AttnPlace at;                 // of the item; its piece is tiles t0 .. t1 - 1
-    uint32_t seq, t0, t1, rows, keys;
+    uint32_t seq, t0, t1;
 
-    __device__ __forceinline__ AttnWalk(const AttnStart& s, uint32_t block_rows, uint32_t tile_keys)
-        : sq(s.sq), at(s.at), seq(s.seq), t0(0), t1(0), rows(block_rows), keys(tile_keys), left_(s.left), fresh_(true) {}
-    __device__ __forceinline__ AttnSeq plan(const AttnParams& p) const { return AttnSeq(sq.q_len, sq.kv_len, p.group, rows, keys, p.extra); }
+    __device__ __forceinline__ AttnWalk(const AttnStart& s) : sq(s.sq), at(s.at), seq(s.seq), t0(0), t1(0), left_(s.left), fresh_(true) {}
+    __device__ __forceinline__ AttnSeq plan(const AttnParams& p) const { return AttnSeq(sq.q_len, sq.kv_len, p.shape); }
     __device__ __forceinline__ bool next(const AttnParams& p) {
         if (!left_) return false;
         if (!fresh_ && !attn_next(plan(p), p.kv_heads, at)) {
@@ -214,10 +200,10 @@ struct AttnWalk {
             --left_;
             return true;
         }
-        const uint32_t there = p.extra + at.tiles, end = there - at.place <= left_ ? there : at.place + uint32_t(left_);
+        const uint32_t there = p.shape.extra + at.tiles, end = there - at.place <= left_ ? there : at.place + uint32_t(left_);
         left_ -= end - at.place;
-        t0 = at.place > p.extra ? at.place - p.extra : 0u;
-        t1 = end > p.extra ? end - p.extra : 0u;
+        t0 = at.place > p.shape.extra ? at.place - p.shape.extra : 0u;
+        t1 = end > p.shape.extra ? end - p.shape.extra : 0u;
         return t1 != 0u;                                                     // (a range that ends ahead of an item's first tile)
     }
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == at.tiles; }

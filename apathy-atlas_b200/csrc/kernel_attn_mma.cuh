@@ -99,8 +99,8 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_m
     pdl_release();
 
     AttnStart* const start = reinterpret_cast<AttnStart*>(sh + MMA_WARPS);
-    attn_begin<MMA_THREADS>(p, MMA_ROWS, C::TILE, sh, start);
-    AttnWalk walk(*start, MMA_ROWS, C::TILE);
+    attn_begin<MMA_THREADS>(p, sh, start);
+    AttnWalk walk(*start);
     while (walk.next(p)) {
         const AttnSeqAt sq = walk.sq;
         const AttnPlace at = walk.at;

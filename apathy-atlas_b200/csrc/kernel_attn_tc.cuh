@@ -146,8 +146,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     pdl_release();
 
     AttnStart* const start = reinterpret_cast<AttnStart*>(sh + C::WARPS);
-    attn_begin<C::THREADS>(p, C::ROWS, TC_KEYS, sh, start);
-    AttnWalk walk(*start, C::ROWS, TC_KEYS);
+    attn_begin<C::THREADS>(p, sh, start);
+    AttnWalk walk(*start);
     // rows of a row tile of the item, and the steps that it takes of the piece
     auto tile_rows = [&](uint32_t g) {
         const uint32_t all = walk.sq.q_len * p.group, r0 = walk.at.block * C::ROWS + g * TC_TILE_ROWS;
