@@ -20,7 +20,7 @@
 // correction off the path of nearly every step.  (Exponentials by a polynomial on the FMA pipe for a quarter to a half of the scores,
 // the special-function unit being the busiest of the softmax: no faster.)
 //
-// Warps: 0 TMA, 1 and 3 MMA of a row tile each (converged, one lane issues), 2 tensor memory and the next items' Q to L2; 4-7 and 8-11 softmax, epilogue and Q
+// Warps: 0 TMA, 1 and 3 MMA of a row tile each (converged, one lane issues), 2 tensor memory; 4-7 and 8-11 softmax, epilogue and Q
 // of a row tile each, the next item's Q before this one's output; E4M3 caches: 12-15 turn raw tiles into FP16 ones (one instruction for
 // two values, exact, NaN kept; Q as FP16 with a power of two per row, see the mma.sync form).  Every wait is bounded as elsewhere in the
 // library.
@@ -49,8 +49,7 @@ template <int DP, bool FP8> struct TcCfg {
     static constexpr int SLOTS = DP <= 64 ? 8 : DP <= 128 ? (FP8 ? 4 : 5) : 2;
     static constexpr int RAW = FP8 ? 128 * DP : 0, RAW_STAGES = FP8 ? (DP <= 128 ? 2 : 1) : 0;
     static constexpr int OFF_Q = 0, OFF_KV = NQ * TILE, OFF_RAW = OFF_KV + SLOTS * TILE;
-    static constexpr int OFF_SCALE = OFF_RAW + RAW_STAGES * RAW;             // float[ROWS]: E4M3: what takes a row's power of two back
-    static constexpr int OFF_BAR = OFF_SCALE + (FP8 ? ROWS * 4 : 0);
+    static constexpr int OFF_BAR = OFF_RAW + RAW_STAGES * RAW;
     static constexpr int N_BAR = 2 * SLOTS + 1 + 7 * NQ + 2 * RAW_STAGES;
     static constexpr int OFF_MISC = OFF_BAR + N_BAR * 8;                     // tensor memory, -, abort; attn_find's words
     static constexpr int SMEM = OFF_MISC + 16 + 16 * 8 + int(sizeof(AttnStart)) + 1024;
@@ -312,62 +311,64 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                 }
             }
-        } else {
-            // ---- Q of the items ahead to L2, so that its rows' latency is that of L2 when their turn comes ----
-            const uint32_t t = NQ == 2 ? lane : (warp - 2) * 32u + lane, all = NQ == 2 ? 32u : 64u;
-            while (walk.next(p)) {
-                const uint32_t row0 = walk.at.block * C::ROWS, rows = tile_rows(0) + (NQ == 2 ? tile_rows(NQ - 1) : 0u), lines = (p.head_dim * 2u + 127u) / 128u;
-                for (uint32_t i = t; i < rows * lines; i += all) {
-                    const uint32_t row = row0 + i / lines, tok = attn_div(row, p.group_div);
-                    const uint16_t* at = p.q + size_t(walk.sq.row0 + tok) * p.q_row_stride + size_t(walk.at.head * p.group + row - tok * p.group) * p.head_dim + (i % lines) * 64u;
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
-                }
-            }
         }
     } else if (warp < uint32_t(C::CONV_WARP0)) {
         // ---- softmax: a row a thread ----
         const uint32_t g = (warp - 4) >> 2, quad = warp & 3u, row_in = quad * 32u + lane;
         const uint32_t t_s = tmem + g * 128u + ((quad * 32u) << 16), t_o = tmem + NQ * 128u + g * uint32_t(DP) + ((quad * 32u) << 16);
         const uint32_t q_tile = base + C::OFF_Q + g * C::TILE;
-        float* const scale_s = reinterpret_cast<float*>(gen + C::OFF_SCALE) + g * TC_TILE_ROWS;
         const uint32_t D = p.head_dim;
         const AttnDivisor group_div = p.group_div;
         uint32_t s_ph[2] = {0, 0};                                           // of the next step's barriers, and of the ones after
-        // Q of the item that the walk is at: this warp's 32 rows, sixteen bytes a lane, eight loads in flight.  (The item before has had its
-        // last scores computed.  All sixteen in flight were a thousand instructions in a row, which a CTA has to fetch before its first
-        // scores: 6 to 26 thousand cycles.)
+        // Q of the item that the walk is at: this warp's 32 rows, copied past the registers sixteen bytes a lane.  (The item before has had its
+        // last scores computed.)  The rows of the item after it are asked for from L2, a token's heads at a time.  (By a warp of their
+        // own, a line a lane and all items at once, they stood in front of the first item's rows: 4 to 20 thousand cycles.)
+        float next_scale = 1.0f;                                             // E4M3: takes this row's power of two back
         auto load_q = [&] {
             const uint32_t rows = tile_rows(g), row0 = walk.at.block * C::ROWS + g * TC_TILE_ROWS;
             if (rows == 0 || steps_of(g) == 0) return;
-            constexpr uint32_t CH = DP / 8, LOADS = 8;
+            constexpr uint32_t CH = DP / 8;
             const uint16_t* const q_head = p.q + size_t(walk.sq.row0) * p.q_row_stride + size_t(walk.at.head) * p.group * D;
-#pragma unroll 1
-            for (uint32_t i0 = 0; i0 < CH; i0 += LOADS) {
-                uint4 qv[LOADS];
-#pragma unroll
-                for (uint32_t i = 0; i < LOADS; ++i) {
-                    const uint32_t idx = (i0 + i) * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH, row = row0 + r, tok = attn_div(row, group_div);
-                    qv[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (r < rows && ch * 8u < D) qv[i] = *reinterpret_cast<const uint4*>(q_head + size_t(tok) * p.q_row_stride + (row - tok * p.group) * D + ch * 8u);
+#pragma unroll 2
+            for (uint32_t i = 0; i < CH; ++i) {
+                const uint32_t idx = i * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH, row = row0 + r, tok = attn_div(row, group_div);
+                const bool there = r < rows && ch * 8u < D;
+                cp_async_16_zfill(q_tile + (ch >> 3) * C::PANEL + sw128_off(r, ch & 7u),
+                                  there ? q_head + size_t(tok) * p.q_row_stride + (row - tok * p.group) * D + ch * 8u : p.q, there ? 16u : 0u);
+            }
+            cp_async_commit();
+            AttnWalk ahead = walk;
+            if (ahead.next(p)) {
+                const uint32_t r0 = ahead.at.block * C::ROWS + g * TC_TILE_ROWS + quad * 32u, all = ahead.sq.q_len * p.group;
+                if (r0 < all) {
+                    const uint32_t tok = attn_div(r0, group_div) + lane;
+                    if (tok <= attn_div(min(r0 + 31u, all - 1u), group_div))
+                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
+                                     ::"l"(p.q + size_t(ahead.sq.row0 + tok) * p.q_row_stride + size_t(ahead.at.head) * p.group * D), "r"(p.group * D * 2u) : "memory");
                 }
-#pragma unroll
-                for (uint32_t i = 0; i < LOADS; ++i) {
-                    const uint32_t idx = (i0 + i) * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH;
-                    uint4 v = qv[i];
-                    if constexpr (FP8) {
-                        uint32_t w[4] = {v.x, v.y, v.z, v.w}, top = 0;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7FFFu, (w[k] >> 16) & 0x7FFFu));
-#pragma unroll
-                        for (uint32_t o = 1; o < CH && o < 32u; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-                        const int e = int(top >> 7), by = e == 0 || e == 255 ? 0 : min(max(141 - e, -120), 120);
-                        const float up = __uint_as_float(uint32_t(127 + by) << 23);
-                        if (ch == 0) scale_s[r] = __uint_as_float(uint32_t(127 - by) << 23);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) w[k] = pack_pair<true>(bf16_lo(w[k]) * up, bf16_hi(w[k]) * up);
-                        v = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                    sts128(q_tile + (ch >> 3) * C::PANEL + sw128_off(r, ch & 7u), v.x, v.y, v.z, v.w);
+            }
+            cp_async_wait_group<0>();
+            __syncwarp();
+            if constexpr (FP8) {
+                // FP16, by the power of two that brings the row's largest value to [2^14, 2^15); a thread has its row
+                const uint32_t mine = q_tile + row_in * 128u, turn = row_in & 7u;
+                uint32_t top = 0;
+#pragma unroll 4
+                for (uint32_t ch = 0; ch < CH; ++ch) {
+                    const uint4 v = lds128(mine + (ch >> 3) * C::PANEL + (((ch & 7u) ^ turn) << 4));
+                    const uint32_t a = v.x & 0x7FFF7FFFu, b = v.y & 0x7FFF7FFFu, c = v.z & 0x7FFF7FFFu, d = v.w & 0x7FFF7FFFu;
+                    top = __vmaxu2(top, __vmaxu2(__vmaxu2(a, b), __vmaxu2(c, d)));
+                }
+                top = max(top & 0xFFFFu, top >> 16);
+                const int e = int(top >> 7), by = e == 0 || e == 255 ? 0 : min(max(141 - e, -120), 120);
+                const float up = __uint_as_float(uint32_t(127 + by) << 23);
+                next_scale = __uint_as_float(uint32_t(127 - by) << 23);
+#pragma unroll 4
+                for (uint32_t ch = 0; ch < CH; ++ch) {
+                    const uint32_t at = mine + (ch >> 3) * C::PANEL + (((ch & 7u) ^ turn) << 4);
+                    const uint4 v = lds128(at);
+                    sts128(at, pack_pair<true>(bf16_lo(v.x) * up, bf16_hi(v.x) * up), pack_pair<true>(bf16_lo(v.y) * up, bf16_hi(v.y) * up),
+                           pack_pair<true>(bf16_lo(v.z) * up, bf16_hi(v.z) * up), pack_pair<true>(bf16_lo(v.w) * up, bf16_hi(v.w) * up));
                 }
             }
             fence_proxy_async();
@@ -383,10 +384,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const uint32_t row = row0 + row_in, tok = attn_div(row, group_div), head = walk.at.head * p.group + row - tok * p.group;
             const uint32_t keys = row_in < rows ? attn_row_keys(walk.sq, tok) : 0u, all_see = attn_row_keys(walk.sq, attn_div(row0, group_div));
             float c = p.scale * p.k_scale * ATTN_LOG2E, m = -INFINITY, l = 0.0f;
-            if constexpr (FP8) {
-                if (n) c *= scale_s[row_in];
-                __syncwarp();                                                // read before the next item's are written
-            }
+            if constexpr (FP8) c *= next_scale;
             const uint64_t c2 = pair_of(c, c);
 #pragma unroll 1
             for (uint32_t u = 0; ok && u < n; ++u) {
