@@ -48,17 +48,20 @@ template <typename K> int allow_smem(K kernel, int bytes, std::atomic<bool> (&do
 }
 
 template <typename... P, typename... A>
-int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, uint32_t cluster, A... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cuda_status(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
 }
 
@@ -113,12 +116,10 @@ AttnParams attention_params(const atlas_b200_attention_desc& d) {
     return p;
 }
 
-// What an item costs besides its tiles, in tiles of its kernel.
-#ifndef MMA_EXTRA_
-#define MMA_EXTRA_ 1
-#define TC_EXTRA_ 2
-#endif
-constexpr uint32_t MMA_EXTRA = MMA_EXTRA_, TC_EXTRA = TC_EXTRA_;
+// What an item costs besides its tiles, in tiles of its kernel.  256 sequences of up to 1000 tokens, mma.sync: 0 / 1 / 2 / 3 of them give
+// 112 / 101 / 96.5 / 97.3 us; tcgen05, 8192 tokens by themselves: 1 / 2 / 3 give 569 / 475 / 476 us (head_dim 256: 860 / 877 / 893).
+constexpr uint32_t MMA_EXTRA = 2;
+constexpr uint32_t tc_extra(uint32_t dim) { return dim <= 128 ? 2u : 1u; }
 
 constexpr uint32_t log2_of(uint32_t n) { return n <= 1 ? 0u : 1u + log2_of(n / 2); }
 AttnShape shape_of(const AttnParams& p, uint32_t rows, uint32_t keys, uint32_t extra) {
@@ -127,7 +128,7 @@ AttnShape shape_of(const AttnParams& p, uint32_t rows, uint32_t keys, uint32_t e
 
 // The mma.sync form: how many CTAs, and whether each takes whole items.
 struct MmaPlan {
-    uint32_t ctas, by_item, least, tile, block_rows;
+    uint32_t ctas, by_item, least, tile, block_rows, cluster_log2;
     size_t ws_bytes;
 };
 MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms) {
@@ -140,10 +141,15 @@ MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms) {
     const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * std::max<uint64_t>((rows + r.block_rows - 1) / r.block_rows, 1);
     r.tile = uint32_t(attn::MMA_WARPS) * (row_bytes <= 128u ? 32u : 16u);
     const uint64_t tiles = std::max<uint64_t>((uint64_t(d.max_kv_len) + r.tile - 1) / r.tile, 1);
-    r.by_item = tiles <= 4;
+    // Few items: a cluster each, of as many CTAs as there are tiles for (four a CTA, where SMs take more than one) and places on the SMs; unless
+    // that leaves a CTA more than eight tiles, which the line's equal ranges share better.
+    const auto wider = [&] { return items << (r.cluster_log2 + 1); };
+    while (r.cluster_log2 < 3 && wider() <= resident && (wider() <= sms ? 2ull : 8ull) << r.cluster_log2 <= tiles) ++r.cluster_log2;
+    if (tiles > 8ull << r.cluster_log2) r.cluster_log2 = 0;
+    r.by_item = r.cluster_log2 || tiles <= 4;
     r.least = r.by_item ? 1u : 4u;
     const uint64_t places = r.by_item ? items : (items * (tiles + MMA_EXTRA) + r.least - 1) / r.least;
-    r.ctas = uint32_t(std::min<uint64_t>(resident, std::max<uint64_t>(places, 1)));
+    r.ctas = uint32_t(std::min<uint64_t>(r.cluster_log2 ? items : resident, std::max<uint64_t>(places, 1)));
     r.ws_bytes = r.by_item ? 0 : ATTN_CUT_BYTES + size_t(resident) * 2 * attn_part_floats(r.block_rows, dim) * sizeof(float);
     return r;
 }
@@ -153,10 +159,11 @@ template <int DP, bool FP8, int RT> int launch_mma_rows(AttnParams p, const MmaP
     static std::atomic<bool> done[kMaxDevices] = {};
     const int rc = allow_smem(attn::attn_mma_kernel<DP, FP8, RT>, C::SMEM, done);
     if (rc) return rc;
-    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.shape = shape_of(p, C::ROWS, C::TILE, MMA_EXTRA);
-    const int rc2 = launch_dependent(attn::attn_mma_kernel<DP, FP8, RT>, plan.ctas, attn::MMA_THREADS, C::SMEM, st, p);
+    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.cluster_log2 = plan.cluster_log2;
+    p.shape = shape_of(p, C::ROWS, C::TILE, MMA_EXTRA);
+    const int rc2 = launch_dependent(attn::attn_mma_kernel<DP, FP8, RT>, plan.ctas << plan.cluster_log2, attn::MMA_THREADS, C::SMEM, st, 1u << plan.cluster_log2, p);
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
-    return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, p);
+    return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, 1u, p);
 }
 
 template <int DP, bool FP8> int launch_mma(const AttnParams& p, const MmaPlan& plan, cudaStream_t st) {
@@ -191,7 +198,7 @@ TcPlan plan_tc(const atlas_b200_attention_desc& d, uint32_t sms) {
     r.box_rows = tc_box_rows(d.block_size);
     r.by_item = tiles <= 2;
     r.least = r.by_item ? 1u : 2u;
-    const uint64_t places = r.by_item ? items : (items * (tiles + TC_EXTRA) + r.least - 1) / r.least;
+    const uint64_t places = r.by_item ? items : (items * (tiles + tc_extra(dim)) + r.least - 1) / r.least;
     r.ctas = uint32_t(std::min<uint64_t>(sms, std::max<uint64_t>(places, 1)));
     r.ws_bytes = r.by_item ? 0 : ATTN_CUT_BYTES + size_t(sms) * 2 * attn_part_floats(block_rows, dim) * sizeof(float);
     return r;
@@ -211,10 +218,10 @@ template <int DP, bool FP8> int launch_tc(AttnParams p, const TcPlan& plan, cuda
     const CUtensorMapSwizzle swz = FP8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
     if (!encode_tensor_map(&map_k, dt, 3, p.k_cache, dims, strides, box, swz) || !encode_tensor_map(&map_v, dt, 3, p.v_cache, dims, strides, box, swz))
         return ATLAS_B200_ERR_DIMS;
-    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.shape = shape_of(p, C::ROWS, attn::TC_KEYS, TC_EXTRA);
-    const int rc2 = launch_dependent(attn::attn_tc_kernel<DP, FP8>, plan.ctas, C::THREADS, C::SMEM, st, map_k, map_v, p, plan.box_rows);
+    p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.shape = shape_of(p, C::ROWS, attn::TC_KEYS, tc_extra(DP));
+    const int rc2 = launch_dependent(attn::attn_tc_kernel<DP, FP8>, plan.ctas, C::THREADS, C::SMEM, st, 1u, map_k, map_v, p, plan.box_rows);
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
-    return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, p);
+    return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, 1u, p);
 }
 
 int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
@@ -239,7 +246,7 @@ int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
     if (!d.ws && !plan.by_item) { plan.by_item = 1; plan.least = 1; }        // (no scratch: nothing is cut)
     const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3;
     const AttnParams p = attention_params(d);
-    t_attn_shape[0] = plan.block_rows; t_attn_shape[1] = plan.ctas; t_attn_shape[2] = plan.by_item; t_attn_shape[3] = plan.tile;
+    t_attn_shape[0] = plan.block_rows; t_attn_shape[1] = plan.ctas << plan.cluster_log2; t_attn_shape[2] = plan.by_item; t_attn_shape[3] = plan.tile;
     if (dim == 64) return fp8 ? launch_mma<64, true>(p, plan, st) : launch_mma<64, false>(p, plan, st);
     if (dim == 128) return fp8 ? launch_mma<128, true>(p, plan, st) : launch_mma<128, false>(p, plan, st);
     return fp8 ? launch_mma<256, true>(p, plan, st) : launch_mma<256, false>(p, plan, st);
@@ -311,7 +318,7 @@ int atlas_b200_cache_append(const atlas_b200_cache_desc* desc, const int32_t* se
     pages::PagesParams p{};
     const int bad = check_pages(*desc, n, false, p);
     if (bad) return bad;
-    return launch_dependent(pages::append_kernel, 1, pages::PLAN_THREADS, 0, static_cast<cudaStream_t>(stream), p, seqs, n_new, n, max_tokens, slot_mapping, status);
+    return launch_dependent(pages::append_kernel, 1, pages::PLAN_THREADS, 0, static_cast<cudaStream_t>(stream), 1u, p, seqs, n_new, n, max_tokens, slot_mapping, status);
 }
 
 int atlas_b200_cache_fork(const atlas_b200_cache_desc* desc, const int32_t* src, const int32_t* dst, uint32_t n, int32_t* status, void* stream) {
@@ -323,9 +330,9 @@ int atlas_b200_cache_fork(const atlas_b200_cache_desc* desc, const int32_t* src,
     const int bad = check_pages(*desc, n, true, p);
     if (bad) return bad;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int rc = launch_dependent(pages::fork_plan_kernel, 1, pages::PLAN_THREADS, 0, st, p, src, dst, n, status);
+    const int rc = launch_dependent(pages::fork_plan_kernel, 1, pages::PLAN_THREADS, 0, st, 1u, p, src, dst, n, status);
     if (rc) return rc;
-    return launch_dependent(pages::fork_copy_kernel, dim3(n, std::max(desc->n_bases, 1u)), pages::COPY_THREADS, 0, st, p, src, dst);
+    return launch_dependent(pages::fork_copy_kernel, dim3(n, std::max(desc->n_bases, 1u)), pages::COPY_THREADS, 0, st, 1u, p, src, dst);
 }
 
 int atlas_b200_cache_free(const atlas_b200_cache_desc* desc, const int32_t* seqs, uint32_t n, void* stream) {
@@ -336,7 +343,7 @@ int atlas_b200_cache_free(const atlas_b200_cache_desc* desc, const int32_t* seqs
     pages::PagesParams p{};
     const int bad = check_pages(*desc, n, false, p);
     if (bad) return bad;
-    return launch_dependent(pages::free_kernel, n, pages::FREE_THREADS, 0, static_cast<cudaStream_t>(stream), p, seqs);
+    return launch_dependent(pages::free_kernel, n, pages::FREE_THREADS, 0, static_cast<cudaStream_t>(stream), 1u, p, seqs);
 }
 
 int atlas_b200_cache_compact(const atlas_b200_cache_desc* desc, int32_t* refcount_out, int32_t* block_table_out, int32_t* page_map, int32_t* n_used, void* stream) {
@@ -346,9 +353,9 @@ int atlas_b200_cache_compact(const atlas_b200_cache_desc* desc, int32_t* refcoun
     const int bad = check_pages(*desc, 0, true, p);
     if (bad) return bad;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int rc = launch_dependent(pages::compact_plan_kernel, 1, pages::PLAN_THREADS, 0, st, p, refcount_out, page_map, n_used);
+    const int rc = launch_dependent(pages::compact_plan_kernel, 1, pages::PLAN_THREADS, 0, st, 1u, p, refcount_out, page_map, n_used);
     if (rc) return rc;
-    return launch_dependent(pages::compact_move_kernel, uint32_t(device_sm_count()) * 4, pages::COPY_THREADS, 0, st, p, page_map, block_table_out);
+    return launch_dependent(pages::compact_move_kernel, uint32_t(device_sm_count()) * 4, pages::COPY_THREADS, 0, st, 1u, p, page_map, block_table_out);
 }
 
 }  // extern "C"

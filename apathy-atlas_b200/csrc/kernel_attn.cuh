@@ -36,7 +36,8 @@ struct AttnParams {
     float* parts;                 // two slots a range of block_rows rows: O, then M and L (see attn_part_floats)
     uint32_t n_seqs, n_tokens, n_pages, table_stride, q_heads, kv_heads, head_dim, block_size, group, q_row_stride, out_row_stride;
     uint32_t ctas, least_tiles;   // ranges: at most `ctas`, of `least_tiles` tiles each at least
-    uint32_t by_item;             // every CTA takes whole items: no pieces
+    uint32_t by_item;             // every CTA (or cluster) takes whole items: no pieces in scratch
+    uint32_t cluster_log2;        // by_item: an item is a cluster's of 2^this CTAs, each with a share of its tiles
     AttnShape shape;              // of the kernel's blocks and tiles
     AttnDivisor page_div, group_div;
     float scale, k_scale, v_scale;
@@ -103,7 +104,7 @@ __device__ __forceinline__ uint64_t attn_warp_scan(uint64_t mine) {          // 
 }
 // By one warp: the place `begin` of the sequence's part of the line, whose first place is seq_begin; and a note of the cut there.
 __device__ __forceinline__ void attn_begin_at(const AttnParams& p, const AttnRanges& ranges, uint64_t begin, uint64_t end, uint32_t seq, uint64_t seq_begin, AttnStart* start) {
-    const uint32_t lane = threadIdx.x & 31u, c = blockIdx.x;
+    const uint32_t lane = threadIdx.x & 31u, c = blockIdx.x >> p.cluster_log2;
     const AttnSeqAt sq = attn_seq(p, seq);
     const AttnSeq plan(sq.q_len, sq.kv_len, p.shape);
     const uint64_t x = begin - seq_begin;
@@ -139,7 +140,7 @@ constexpr uint32_t ATTN_WARP_SEQS = 256;
 template <int THREADS>
 __device__ __forceinline__ void attn_begin(const AttnParams& p, uint64_t* sh, AttnStart* start) {
     constexpr uint32_t WARPS = THREADS / 32;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, c = blockIdx.x;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, c = blockIdx.x >> p.cluster_log2;
     const bool few = p.n_seqs <= ATTN_WARP_SEQS;                             // one warp sums up the sequences too
     if (!few || warp == 0) {
         const uint32_t by = few ? 32u : uint32_t(THREADS), each = (p.n_seqs + by - 1) / by, s0 = min(tid * each, p.n_seqs), s1 = min(s0 + each, p.n_seqs);
