@@ -131,22 +131,23 @@ struct MmaPlan {
     uint32_t ctas, by_item, least, tile, block_rows, cluster_log2;
     size_t ws_bytes;
 };
-MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms) {
+MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms, bool scratch) {
     const uint32_t dim = attn_dim(d.head_dim);
     const uint64_t group = d.q_heads / d.kv_heads;
     const uint64_t rows = std::min<uint64_t>(d.max_q_len, d.n_tokens) * group;
     MmaPlan r{};
     r.block_rows = rows <= 8 ? 8u : 16u;
-    const uint32_t row_bytes = dim * (d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 1u : 2u), resident = std::min(sms, ATTN_MAX_CTAS / 3) * uint32_t(attn::attn_mma_ctas(int(row_bytes), d.cache_dtype == ATLAS_B200_CACHE_E4M3, r.block_rows == 8u ? 1 : 2));
+    const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3;
+    const uint32_t row_bytes = dim * (fp8 ? 1u : 2u), resident = std::min(sms, ATTN_MAX_CTAS / 3) * uint32_t(attn::attn_mma_ctas(int(row_bytes), fp8, r.block_rows == 8u ? 1 : 2));
     const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * std::max<uint64_t>((rows + r.block_rows - 1) / r.block_rows, 1);
     r.tile = uint32_t(attn::MMA_WARPS) * (row_bytes <= 128u ? 32u : 16u);
     const uint64_t tiles = std::max<uint64_t>((uint64_t(d.max_kv_len) + r.tile - 1) / r.tile, 1);
     // Few items: a cluster each, of as many CTAs as there are tiles for (four a CTA, where SMs take more than one) and places on the SMs; unless
-    // that leaves a CTA more than eight tiles, which the line's equal ranges share better.
+    // that leaves a CTA more than eight tiles, which the line's equal ranges share better, given scratch.
     const auto wider = [&] { return items << (r.cluster_log2 + 1); };
     while (r.cluster_log2 < 3 && wider() <= resident && (wider() <= sms ? 2ull : 8ull) << r.cluster_log2 <= tiles) ++r.cluster_log2;
-    if (tiles > 8ull << r.cluster_log2) r.cluster_log2 = 0;
-    r.by_item = r.cluster_log2 || tiles <= 4;
+    if (scratch && tiles > 8ull << r.cluster_log2) r.cluster_log2 = 0;
+    r.by_item = !scratch || r.cluster_log2 || tiles <= 4;                    // (no scratch: nothing is cut)
     r.least = r.by_item ? 1u : 4u;
     const uint64_t places = r.by_item ? items : (items * (tiles + MMA_EXTRA) + r.least - 1) / r.least;
     r.ctas = uint32_t(std::min<uint64_t>(r.cluster_log2 ? items : resident, std::max<uint64_t>(places, 1)));
@@ -224,15 +225,18 @@ template <int DP, bool FP8> int launch_tc(AttnParams p, const TcPlan& plan, cuda
     return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, 1u, p);
 }
 
+// (Which kernel runs also goes by the alignment of pointers that may not be set yet when scratch is asked for: enough for either.)
+size_t attention_ws_bytes(const atlas_b200_attention_desc& d, uint32_t sms) { return std::max(plan_mma(d, sms, true).ws_bytes, plan_tc(d, sms).ws_bytes); }
+
 int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
     if (d.n_seqs == 0 || d.n_tokens == 0) return ATLAS_B200_OK;
     const int bad = check_attention(d);
     if (bad) return bad;
     if (!device_is_sm100()) return ATLAS_B200_ERR_ARCH;
     const uint32_t sms = uint32_t(device_sm_count()), dim = attn_dim(d.head_dim);
+    if (d.ws ? d.ws_bytes < attention_ws_bytes(d, sms) : d.ws_bytes != 0) return ATLAS_B200_ERR_WORKSPACE;
     if (takes_tc(d)) {
         TcPlan plan = plan_tc(d, sms);
-        if (d.ws ? d.ws_bytes < plan.ws_bytes : d.ws_bytes != 0) return ATLAS_B200_ERR_WORKSPACE;
         if (!d.ws && !plan.by_item) { plan.by_item = 1; plan.least = 1; }
         const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3;
         const AttnParams p = attention_params(d);
@@ -241,9 +245,7 @@ int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
         if (dim == 128) return fp8 ? launch_tc<128, true>(p, plan, st) : launch_tc<128, false>(p, plan, st);
         return fp8 ? launch_tc<256, true>(p, plan, st) : launch_tc<256, false>(p, plan, st);
     }
-    MmaPlan plan = plan_mma(d, sms);
-    if (d.ws ? d.ws_bytes < plan.ws_bytes : d.ws_bytes != 0) return ATLAS_B200_ERR_WORKSPACE;
-    if (!d.ws && !plan.by_item) { plan.by_item = 1; plan.least = 1; }        // (no scratch: nothing is cut)
+    const MmaPlan plan = plan_mma(d, sms, d.ws != nullptr);
     const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3;
     const AttnParams p = attention_params(d);
     t_attn_shape[0] = plan.block_rows; t_attn_shape[1] = plan.ctas << plan.cluster_log2; t_attn_shape[2] = plan.by_item; t_attn_shape[3] = plan.tile;
@@ -295,9 +297,7 @@ int atlas_b200_paged_attention(const atlas_b200_attention_desc* desc, void* stre
 
 size_t atlas_b200_paged_attention_ws_bytes(const atlas_b200_attention_desc* desc) {
     if (!desc || desc->kv_heads == 0 || desc->q_heads % desc->kv_heads || desc->n_seqs == 0 || desc->n_tokens == 0) return 0;
-    // (which kernel runs also goes by the alignment of pointers that may not be set yet: enough for either)
-    const uint32_t sms = uint32_t(device_sm_count());
-    return std::max(plan_mma(*desc, sms).ws_bytes, plan_tc(*desc, sms).ws_bytes);
+    return attention_ws_bytes(*desc, uint32_t(device_sm_count()));
 }
 
 int atlas_b200_last_attention_shape(uint32_t out[4]) {

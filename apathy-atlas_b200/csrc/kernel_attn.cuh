@@ -226,36 +226,95 @@ __device__ __forceinline__ float attn_e4m3(uint8_t b) { return __half2float(__ha
 // Logarithm of a row's sum of exponentials from its M and L.
 __device__ __forceinline__ float attn_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) * ATTN_LN2; }
 
-// One row again from its own keys alone, by one warp.  The kernels multiply masked places with zeros, and zero times an infinity or a
-// NaN in the values of a later token is a NaN; a row that came out not finite is computed here instead, which leaves other tokens'
-// values unread.  The cost (a chain over the row's keys) is paid by such rows only.
-static __device__ __noinline__ void attn_row_again(const AttnParams& p, bool fp8, uint32_t seq, uint32_t token, uint32_t head, uint32_t keys) {
+// The kernels multiply masked places with zeros, and zero times an infinity or a NaN in the values of a later token is a NaN.  So a row
+// that came out not finite is computed once more, by one warp from its own keys alone, where such values stand among the keys that its
+// block reads and it does not see: ATTN_MASKED_MOST behind its own at most (256 rows of a block, and what is left of a tile of 128).
+// Where there are none the row is what its formula gives.  32 keys at a time: a lane has a key's score, then the warp the key's values.
+constexpr uint32_t ATTN_MASKED_MOST = 384;
+
+__device__ __forceinline__ float attn_cache_value(const uint8_t* cache, bool fp8, size_t at) {
+    return fp8 ? attn_e4m3(cache[at]) : __uint_as_float(uint32_t(reinterpret_cast<const uint16_t*>(cache)[at]) << 16);
+}
+// Whether a value of keys from .. to - 1 is not finite; by one warp.
+static __device__ __noinline__ bool attn_odd_values(const AttnParams& p, bool fp8, uint32_t seq, uint32_t kv_head, uint32_t from, uint32_t to) {
     const uint32_t lane = threadIdx.x & 31u, D = p.head_dim;
     const int32_t* table = p.block_table + size_t(seq) * p.table_stride;
-    const uint16_t* q = p.q + size_t(token) * p.q_row_stride + size_t(head) * D;
-    float qv[8], o[8] = {}, m = -INFINITY, l = 0.0f;
-    for (uint32_t i = 0; i < 8; ++i) qv[i] = lane + 32u * i < D ? __uint_as_float(uint32_t(q[lane + 32u * i]) << 16) : 0.0f;
+    bool odd = false;
+    for (uint32_t j0 = from; j0 < to; j0 += 32) {
+        const int32_t row = j0 + lane < to ? attn_cache_row(p, table, j0 + lane) : -1;
+        for (uint32_t d = lane; d < D; d += 32)
+#pragma unroll 8
+            for (uint32_t k = 0; k < 32; ++k) {
+                const int32_t r = __shfl_sync(0xFFFFFFFFu, row, k);
+                if (r >= 0) odd |= !isfinite(attn_cache_value(p.v_cache, fp8, (size_t(r) * p.kv_heads + kv_head) * D + d));
+            }
+        if (__any_sync(0xFFFFFFFFu, odd)) return true;
+    }
+    return false;
+}
+template <bool fp8>
+__device__ __noinline__ void attn_row_again(const AttnParams& p, uint32_t seq, uint32_t token, uint32_t head, uint32_t keys, uint32_t kv_len) {
+    const uint32_t lane = threadIdx.x & 31u, D = p.head_dim, kv_head = head / p.group;
+    if (!attn_odd_values(p, fp8, seq, kv_head, keys, min(kv_len, keys + ATTN_MASKED_MOST))) return;
+    const int32_t* table = p.block_table + size_t(seq) * p.table_stride;
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(p.q + size_t(token) * p.q_row_stride + size_t(head) * D);
+    constexpr uint32_t size = fp8 ? 1 : 2, AT_ONCE = 4;
+    float o[8] = {}, m = -INFINITY, l = 0.0f;
     const float c = p.scale * p.k_scale * ATTN_LOG2E;
-    for (uint32_t j = 0; j < keys; ++j) {
-        const int32_t row = attn_cache_row(p, table, j);
-        const size_t at = (size_t(row < 0 ? 0 : row) * p.kv_heads + head / p.group) * D;
-        float s = 0.0f, v[8];
-        for (uint32_t i = 0; i < 8; ++i) {
-            const uint32_t d = lane + 32u * i;
-            v[i] = 0.0f;
-            if (row < 0 || d >= D) continue;
-            const float k = fp8 ? attn_e4m3(p.k_cache[at + d]) : __uint_as_float(uint32_t(reinterpret_cast<const uint16_t*>(p.k_cache)[at + d]) << 16);
-            v[i] = fp8 ? attn_e4m3(p.v_cache[at + d]) : __uint_as_float(uint32_t(reinterpret_cast<const uint16_t*>(p.v_cache)[at + d]) << 16);
-            s = fmaf(qv[i], k, s);
+    for (uint32_t j0 = 0; j0 < keys; j0 += 32) {
+        const uint32_t n = min(keys - j0, 32u);
+        const int32_t row = lane < n ? attn_cache_row(p, table, j0 + lane) : -1;
+        float s = 0.0f;
+        if (row >= 0) {
+            const uint4* k_row = reinterpret_cast<const uint4*>(p.k_cache + (size_t(row) * p.kv_heads + kv_head) * D * size);
+            const uint32_t chunks = D * size / 16;
+            for (uint32_t c0 = 0; c0 < chunks; c0 += AT_ONCE) {
+                uint4 v[AT_ONCE];
+#pragma unroll
+                for (uint32_t i = 0; i < AT_ONCE; ++i) v[i] = c0 + i < chunks ? k_row[c0 + i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (uint32_t i = 0; i < AT_ONCE; ++i) {
+                    if (c0 + i >= chunks) break;
+                    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                    for (uint32_t e = 0; e < 8 / size; ++e) {
+                        const uint32_t qq = q[8 / size * (c0 + i) + e];
+                        if constexpr (fp8) {
+                            const uint32_t two = w[e >> 1] >> (16 * (e & 1));
+                            s = fmaf(bf16_lo(qq), attn_e4m3(uint8_t(two)), s);
+                            s = fmaf(bf16_hi(qq), attn_e4m3(uint8_t(two >> 8)), s);
+                        } else {
+                            s = fmaf(bf16_lo(qq), bf16_lo(w[e]), s);
+                            s = fmaf(bf16_hi(qq), bf16_hi(w[e]), s);
+                        }
+                    }
+                }
+            }
         }
-        for (uint32_t x = 16; x; x >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, x);
-        s *= c;
-        const float top = fmaxf(m, s), base = top == -INFINITY ? 0.0f : top;
-        const float keep = exp2f(m - base), w = exp2f(s - base);
+        s = lane < n ? s * c : -INFINITY;
+        float top = fmaxf(m, s);
+        for (uint32_t x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+        const float base = top == -INFINITY ? 0.0f : top, keep = exp2f(m - base), w = exp2f(s - base);
         l = l * keep + w;
-        for (uint32_t i = 0; i < 8; ++i) o[i] = o[i] * keep + w * v[i];
+        for (uint32_t i = 0; i < 8; ++i) o[i] *= keep;
+        for (uint32_t k0 = 0; k0 < n; k0 += AT_ONCE) {                       // (lanes behind n have no row and no weight)
+            float v[AT_ONCE][8], w_k[AT_ONCE];
+#pragma unroll
+            for (uint32_t k = 0; k < AT_ONCE; ++k) {
+                const int32_t r = __shfl_sync(0xFFFFFFFFu, row, k0 + k);
+                w_k[k] = __shfl_sync(0xFFFFFFFFu, w, k0 + k);
+                const size_t at = (size_t(r < 0 ? 0 : r) * p.kv_heads + kv_head) * D;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) v[k][i] = r >= 0 && lane + 32u * i < D ? attn_cache_value(p.v_cache, fp8, at + lane + 32u * i) : 0.0f;
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) o[i] += w_k[k] * v[k][i];
+        }
         m = top;
     }
+    for (uint32_t x = 16; x; x >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
     const float f = l == 0.0f ? 0.0f : p.v_scale / l;
     if (p.lse && lane == 0) p.lse[size_t(token) * p.q_heads + head] = attn_lse(m, l);
     for (uint32_t i = 0; i < 8; ++i)
@@ -368,12 +427,12 @@ __global__ void __launch_bounds__(ATTN_JOIN_THREADS, 4) attn_join_kernel(const _
         for (uint32_t k = warp; k < n_rows; k += ATTN_JOIN_WARPS)
             if ((odd_s >> k) & 1u) {
                 place(r0 + k, in_seq, token, head);
-                attn_row_again(p, FP8, cut.seq, token, head, attn_row_keys(sq, in_seq));
+                attn_row_again<FP8>(p, cut.seq, token, head, attn_row_keys(sq, in_seq), sq.kv_len);
             }
         return;
     }
     constexpr int V = DP / 32;                                               // channels of a lane, side by side
-    for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    for (uint32_t r = blockIdx.y; r < rows; r += ATTN_JOIN_Y) {
         float m = -INFINITY, l = 0.0f;
         for (uint32_t i = lane; i < cut.pieces; i += 32) m = fmaxf(m, piece(i)[size_t(ROWS) * DP + r]);
         for (uint32_t x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
@@ -413,10 +472,15 @@ __global__ void __launch_bounds__(ATTN_JOIN_THREADS, 4) attn_join_kernel(const _
             place(r, in_seq, token, head);
             const bool odd = attn_store<V>(p, token, head, lane * V, o, l);
             if (p.lse && lane == 0) p.lse[size_t(token) * p.q_heads + head] = attn_lse(m, l);
-            if (__any_sync(0xFFFFFFFFu, odd)) attn_row_again(p, FP8, cut.seq, token, head, attn_row_keys(sq, in_seq));
+            if (__any_sync(0xFFFFFFFFu, odd) && lane == 0) odd_s |= 1u << (r / ATTN_JOIN_Y);
         }
         __syncthreads();
     }
+    for (uint32_t k = warp; k < uint32_t(ROWS) / ATTN_JOIN_Y; k += ATTN_JOIN_WARPS)
+        if ((odd_s >> k) & 1u) {
+            place(blockIdx.y + k * ATTN_JOIN_Y, in_seq, token, head);
+            attn_row_again<FP8>(p, cut.seq, token, head, attn_row_keys(sq, in_seq), sq.kv_len);
+        }
 }
 
 }  // namespace atlas

@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_m
                 }
             }
             if (p.lse && lane == 0) p.lse[size_t(sq.row0 + tok) * p.q_heads + head] = attn_lse(top, total);
-            if (__any_sync(0xFFFFFFFFu, odd) && sq.q_len > 1) attn_row_again(p, FP8, seq, sq.row0 + tok, head, attn_row_keys(sq, tok));
+            if (__any_sync(0xFFFFFFFFu, odd) && sq.q_len > 1) attn_row_again<FP8>(p, seq, sq.row0 + tok, head, attn_row_keys(sq, tok), sq.kv_len);
         };
         for (uint32_t r = warp; r < rows; r += MMA_WARPS) {                  // a warp takes whole rows
             float top = -INFINITY, w[MMA_WARPS], total = 0.0f;

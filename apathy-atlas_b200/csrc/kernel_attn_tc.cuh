@@ -375,7 +375,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             __syncwarp();
             mbar_arrive(Q_FULL + 8 * g);
         };
-        bool ok = true, more = walk.next(p);
+        bool ok = true, more = walk.next(p), some_odd = false;
         if (more) load_q();
         while (ok && more) {
             // this item, as the walk goes on to the next one before its output is written
@@ -512,14 +512,26 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                 }
                 if (p.lse && row_in < rows) p.lse[size_t(seq_row0 + tok) * p.q_heads + head] = attn_lse(m, l);
-                uint32_t again = __ballot_sync(0xFFFFFFFFu, odd && row_in < rows);
-                while (again) {
-                    const uint32_t k = __ffs(again) - 1u;
-                    again &= again - 1u;
-                    attn_row_again(p, FP8, seq, seq_row0 + __shfl_sync(0xFFFFFFFFu, tok, k), __shfl_sync(0xFFFFFFFFu, head, k), __shfl_sync(0xFFFFFFFFu, keys, k));
-                }
+                some_odd |= __any_sync(0xFFFFFFFFu, odd && row_in < rows);
             }
             tcgen05_fence_before();                                          // O has been read before the next item's P is handed over
+        }
+        // Rows that came out not finite (see attn_row_again), once nobody waits for this warp any more: they can take longer than a wait may.
+        if (ok && some_odd) {
+            walk = AttnWalk(*start);
+            while (walk.next(p)) {
+                const uint32_t rows = tile_rows(g), row0 = walk.at.block * C::ROWS + g * TC_TILE_ROWS + quad * 32u;
+                if (!walk.whole() || rows <= quad * 32u) continue;
+                const uint32_t keys0 = attn_row_keys(walk.sq, attn_div(row0, group_div)), kv_len = walk.sq.kv_len;
+                if (!attn_odd_values(p, FP8, walk.seq, walk.at.head, keys0, min(kv_len, keys0 + ATTN_MASKED_MOST))) continue;
+                for (uint32_t r = 0; r < min(rows - quad * 32u, 32u); ++r) {
+                    const uint32_t row = row0 + r, tok = attn_div(row, group_div), head = walk.at.head * p.group + row - tok * p.group;
+                    const uint16_t* const o_row = p.out + size_t(walk.sq.row0 + tok) * p.out_row_stride + size_t(head) * D;
+                    bool odd = false;
+                    for (uint32_t d = lane; d < D; d += 32) odd |= (o_row[d] & 0x7F80u) == 0x7F80u;
+                    if (__any_sync(0xFFFFFFFFu, odd)) attn_row_again<FP8>(p, walk.seq, walk.sq.row0 + tok, head, attn_row_keys(walk.sq, tok), kv_len);
+                }
+            }
         }
     } else if constexpr (FP8) {
         // ---- raw tiles to FP16 ones ----

@@ -484,7 +484,8 @@ ATLAS_B200_API int32_t atlas_b200_registry_select_victim(const atlas_b200_regist
  * a few while drafts are verified, many while its prompt is read).  The chunk's keys and values stand in the cache already (the
  * *_cache_write calls above put them there).  For new token i of a sequence with n cached and c new tokens, and query head h:
  *     o[i,h] = sum_j p_j v[j, h / group],   p = softmax over j <= n - c + i of  softmax_scale * q[i,h] . k[j, h / group]
- * with group = q_heads / kv_heads.  A token that sees no key (c > n) gives zeros, and -inf in lse.  Scores, the softmax's maximum and
+ * with group = q_heads / kv_heads.  A token that sees no key (c > n), or none whose score is above -inf, gives zeros, and -inf in lse.
+ * An infinity or a NaN in the values of a token that is seen makes its channel an infinity or a NaN; one that is not seen is not read into any.  Scores, the softmax's maximum and
  * sum and the outputs' sums are FP32; p is rounded to BF16 (FP16 over an E4M3 cache) for its product with v; o is rounded once.
  *   q, out       [n_tokens, q_heads * head_dim] BF16, row strides in elements; q may be a column range of a fused QKV buffer;
  *                they must not overlap
@@ -546,7 +547,8 @@ ATLAS_B200_API size_t atlas_b200_paged_attention_ws_bytes(const atlas_b200_atten
  *   offset) of all entries' new tokens one after the other, as the writers take them: -1 for those of an entry that failed and behind the last.
  * cache_fork: sequence dst[i], empty, becomes a copy of src[i] as it was before the call: full pages are shared, a part-filled one is
  *   copied into a page of its own, the tokens it holds and no more.
- * cache_free: the sequences give back their pages; their rows become -1 and their lengths 0.  A sequence named twice is freed once.
+ * cache_free: the sequences give back their pages; their rows become -1 and their lengths 0.  A sequence named twice is freed once.  One that the tables do
+ *   not have, and a page that nothing held, are recorded in the device status word (6, 7), a page that is not of the pool as 4 (here, in the others too).
  * cache_compact: with U pages in use, the k-th one in use behind the first U moves to the k-th free one among them.  Results into
  *   refcount_out and block_table_out (may be refcount and block_table), page_map [n_pages] (where a page went, -1 if it was free) and
  *   *n_used = U.  Contents of pages U .. are left as they are. */
