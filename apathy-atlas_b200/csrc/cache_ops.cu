@@ -126,6 +126,14 @@ AttnShape shape_of(const AttnParams& p, uint32_t rows, uint32_t keys, uint32_t e
     return attn_shape(p.group, log2_of(rows), log2_of(keys), extra, uint64_t(p.table_stride) * p.block_size, uint64_t(p.n_tokens) * p.group);
 }
 
+// Whole items, where the CTA that has the most of them takes less than what equal ranges take with the scratch that cuts need and its
+// join: some twelve tiles' time.  The sequences' lengths, which the host does not know, are taken for three quarters of the longest one's
+// on the average: whole items wait for the longest.  (One or two items a CTA: beyond, equal ranges lose little.)
+bool whole_items_pay(uint64_t items, uint64_t places, uint64_t ctas) {
+    const uint64_t rounds = (items + ctas - 1) / ctas;
+    return rounds <= 2 && rounds * places <= items * places * 3 / (4 * ctas) + 12;
+}
+
 // The mma.sync form: how many CTAs, and whether each takes whole items.
 struct MmaPlan {
     uint32_t ctas, by_item, least, tile, block_rows, cluster_log2;
@@ -147,7 +155,9 @@ MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms, bool scratch)
     const auto wider = [&] { return items << (r.cluster_log2 + 1); };
     while (r.cluster_log2 < 3 && wider() <= resident && (wider() <= sms ? 2ull : 8ull) << r.cluster_log2 <= tiles) ++r.cluster_log2;
     if (scratch && tiles > 8ull << r.cluster_log2) r.cluster_log2 = 0;
-    r.by_item = !scratch || r.cluster_log2 || tiles <= 4;                    // (no scratch: nothing is cut)
+    // 64 sequences of 500 tokens, 8 KV heads of 128, 29.8 us whole and 35.0 cut; 64 of 300, 22.0 and 26.5; 40 of 700, 33.4 and 31.3; over E4M3
+    // 40 of 700, 22.9 and 29.1.
+    r.by_item = !scratch || r.cluster_log2 || tiles <= 4 || whole_items_pay(items, tiles + MMA_EXTRA, resident);      // (no scratch: nothing is cut)
     r.least = r.by_item ? 1u : 4u;
     const uint64_t places = r.by_item ? items : (items * (tiles + MMA_EXTRA) + r.least - 1) / r.least;
     r.ctas = uint32_t(std::min<uint64_t>(r.cluster_log2 ? items : resident, std::max<uint64_t>(places, 1)));
@@ -197,12 +207,10 @@ TcPlan plan_tc(const atlas_b200_attention_desc& d, uint32_t sms) {
     const uint64_t tiles = std::max<uint64_t>((uint64_t(d.max_kv_len) + attn::TC_KEYS - 1) / attn::TC_KEYS, 1);
     TcPlan r{};
     r.box_rows = tc_box_rows(d.block_size);
-    // Whole items, where the CTA that has the most of them takes less than what equal ranges take with the scratch that cuts need and its
-    // join: some ten tiles' time.  (One or two items a CTA: where there are more their lengths, which the host does not know, matter.)
     // Two chunks of 512 over 1024 tokens, 8 KV heads of 128, 24.2 us whole and 42.3 cut; 300 over 300, 12.2 and 22.2; eight of 64 over
     // 2000, head_dim 64, 32.6 and 30.5.
-    const uint64_t rounds = (items + sms - 1) / sms, item = tiles + tc_extra(dim);
-    r.by_item = tiles <= 2 || (rounds <= 2 && rounds * item <= items * item / sms + 10);
+    const uint64_t item = tiles + tc_extra(dim);
+    r.by_item = tiles <= 2 || whole_items_pay(items, item, sms);
     r.least = r.by_item ? 1u : 2u;
     const uint64_t places = r.by_item ? items : (items * item + r.least - 1) / r.least;
     r.ctas = uint32_t(std::min<uint64_t>(sms, std::max<uint64_t>(places, 1)));
