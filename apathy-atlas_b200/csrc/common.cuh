@@ -35,7 +35,7 @@ __device__ __forceinline__ void record_status(uint32_t code) { atomicCAS(&g_stat
 // microseconds.  A kernel may (a) release the next launch once all its own CTAs run, and (b) be launched as a dependent, which may
 // then start early and has to wait until everything before it in the stream has completed and is visible.
 //   launched as dependents     both tensor-core shrinks, the main kernel behind a shrink and without adapters, the tensor-core expand, the
-//                              dense linear, the QKV consumers, SwiGLU in both forms, the quantiser
+//                              dense linear, the QKV consumers, SwiGLU in both forms, the quantiser; the attention, its join, the page operators
 //   releasing                  all of these but lora_shrink_mma_kernel and lora_shrink_grouped_kernel, which do so only in front of a
 //                              main kernel or of the dense linear
 //   neither                    a main kernel over a t that an earlier call left, and the small-batch kernel for more than eight tokens without
