@@ -181,8 +181,8 @@ template <int DP, bool FP8> int launch_mma(const AttnParams& p, const MmaPlan& p
     return plan.block_rows == 8 ? launch_mma_rows<DP, FP8, 1>(p, plan, st) : launch_mma_rows<DP, FP8, 2>(p, plan, st);
 }
 
-// The tcgen05 form.  It reads pages in boxes of the largest power of two that divides page and tile, at least a swizzle atom's eight rows,
-// and Q and the outputs in sixteen bytes.
+// The tcgen05 form.  It reads pages in boxes of the largest power of two that divides page and tile, or row by row where that is less than a
+// swizzle atom's eight rows; and Q and the outputs in sixteen bytes.
 struct TcPlan {
     uint32_t ctas, by_item, least, box_rows;
     size_t ws_bytes;
@@ -196,8 +196,12 @@ bool takes_tc(const atlas_b200_attention_desc& d) {
     // Rows of a KV head from which on the tensor cores' 256-row blocks pay, although most of such a block is empty.  16 sequences of 4000
     // tokens, 8 KV heads of 128, this form / mma.sync: BF16, 12 rows 64 / 56 us, 24 rows 64 / 89, 40 rows 66 / 129; E4M3, whose tiles
     // are converted by four warps, 24 rows 92 / 79.
-    const uint64_t rows = uint64_t(std::min(d.max_q_len, d.n_tokens)) * (d.q_heads / d.kv_heads), from = d.cache_dtype == ATLAS_B200_CACHE_E4M3 ? 32 : 16;
-    return rows > from && tc_box_rows(d.block_size) >= 8 && aligned(d.q, 16) && aligned(d.out, 16) && d.q_row_stride % 8 == 0 && d.out_row_stride % 8 == 0;
+    // Over pages that are copied row by row it costs half as much again (pages of 5: BF16 head_dim 128, 20 rows 136 / 93, 48 rows 136 / 131,
+    // 64 rows 136 / 168; head_dim 256, 209 / 266 with 20 rows; E4M3 head_dim 128, 111 / 112 with 48 rows).
+    const uint64_t rows = uint64_t(std::min(d.max_q_len, d.n_tokens)) * (d.q_heads / d.kv_heads);
+    const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3, boxes = tc_box_rows(d.block_size) >= 8;
+    const uint64_t from = boxes ? (fp8 ? 32 : 16) : !fp8 && d.head_dim > 128 ? 16 : 48;
+    return rows > from && aligned(d.q, 16) && aligned(d.out, 16) && d.q_row_stride % 8 == 0 && d.out_row_stride % 8 == 0;
 }
 TcPlan plan_tc(const atlas_b200_attention_desc& d, uint32_t sms) {
     sms = std::min(sms, ATTN_MAX_CTAS);
@@ -227,7 +231,7 @@ template <int DP, bool FP8> int launch_tc(AttnParams p, const TcPlan& plan, cuda
     const uint64_t size = FP8 ? 1 : 2;
     const uint64_t dims[3] = {p.head_dim, p.kv_heads, uint64_t(p.n_pages) * p.block_size};
     const uint64_t strides[2] = {p.head_dim * size, uint64_t(p.kv_heads) * p.head_dim * size};
-    const uint32_t box[3] = {FP8 ? uint32_t(DP) : 64u, 1u, plan.box_rows};
+    const uint32_t box[3] = {FP8 ? uint32_t(DP) : 64u, 1u, std::max(plan.box_rows, 8u)};   // (below eight: not used)
     const CUtensorMapDataType dt = FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const CUtensorMapSwizzle swz = FP8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
     if (!encode_tensor_map(&map_k, dt, 3, p.k_cache, dims, strides, box, swz) || !encode_tensor_map(&map_v, dt, 3, p.v_cache, dims, strides, box, swz))

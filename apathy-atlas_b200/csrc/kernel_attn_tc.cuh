@@ -12,8 +12,9 @@
 // One thread owns a row: its scores come to its registers (tcgen05.ld), maximum and sum need no exchange with other threads, P goes back
 // to tensor memory as the A operand.  Q, K, V are 128-byte-swizzled tiles in shared memory: Q and K K-major, V as it lies in the cache
 // ([key][channel]), the MN-major form of the B operand.  K and V come 128 keys at a time, page by page by TMA, in boxes of the largest
-// power of two that divides page and tile (8 rows at least); zero fill stands in for pages that do not exist and for channels behind
-// head_dim.
+// power of two that divides page and tile; zero fill stands in for pages that do not exist and for channels behind head_dim.  Pages that no
+// box of eight rows divides are copied row by row past the registers, K by warp 0 and V by warp 2 (pages of 5, 2048
+// tokens over 8192, 8 Q + 2 KV heads of 128: 118 us, the mma.sync form 433; BF16 pages of 16 by TMA 70).
 //
 // O is multiplied with 2^(M_old - M_new) only where a row's maximum has grown by more than 2^15 (TC_RESCALE) since O's last factor: until
 // then the weights are 2^(s - M) with the old M, up to 2^15 (which FP16 holds) and in the same FP32 sums, which is the same quotient.  That
@@ -162,8 +163,58 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     // key tiles of the piece that any row tile wants (the last row tile that has rows wants the most)
     auto tiles_wanted = [&] { return ((NQ == 2 ? max(steps_of(0), steps_of(NQ - 1)) : steps_of(0)) + 1u) / 2u; };
 
+    // Tiles row by row, where no box of eight rows divides a page; a row that is not there is zeros.  K by one warp and V by another, each
+    // in its turns of the ring (K 0, V 0, K 1, V 1, ...); a ring of one place has one warp, as two turns of a place would be two phases of
+    // its barrier apart, which a wait cannot tell.
+    constexpr uint32_t GATHER_RING = FP8 ? C::RAW_STAGES : SLOTS;
+    auto gather = [&](uint32_t first, uint32_t last) {                       // sides
+        constexpr uint32_t SIZE = FP8 ? 1 : 2, CH = DP * SIZE / 16;          // 16-byte pieces of a row
+        const uint32_t EMPTY_OF = FP8 ? RAW_EMPTY : EMPTY, FULL_OF = FP8 ? RAW_FULL : FULL, bytes = p.head_dim * SIZE;
+        uint32_t tile = 0;                                                   // of the CTA
+        bool ok = true;
+        while (ok && walk.next(p)) {
+            const int32_t* table = p.block_table + size_t(walk.seq) * p.table_stride;
+            const uint32_t n = tiles_wanted(), kv_len = walk.sq.kv_len;
+            for (uint32_t j = 0; ok && j < n; ++j, ++tile) {
+                const uint32_t pos0 = (walk.t0 + j) * TC_KEYS;
+                int32_t rows[4];
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const uint32_t pos = pos0 + 32u * k + lane;
+                    rows[k] = pos < kv_len ? attn_cache_row(p, table, pos) : -1;
+                }
+                for (uint32_t side = first; ok && side <= last; ++side) {
+                    const uint8_t* const cache = side ? p.v_cache : p.k_cache;
+                    const uint32_t turn = 2u * tile + side, at = turn % GATHER_RING;
+                    ok = mbar_wait_warp(EMPTY_OF + 8 * at, ((turn / GATHER_RING) & 1u) ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER, 20);
+                    if (!ok) break;
+                    const uint32_t dst = FP8 ? base + C::OFF_RAW + at * C::RAW : base + C::OFF_KV + at * C::TILE;
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k)
+#pragma unroll 8
+                        for (uint32_t i = 0; i < CH; ++i) {
+                            const uint32_t in = i * (32u / CH) + lane / CH, r = 32u * k + in, ch = lane % CH;
+                            const int32_t row = __shfl_sync(0xFFFFFFFFu, rows[k], in);
+                            const bool there = row >= 0 && ch * 16u < bytes;
+                            const uint8_t* from = there ? cache + (size_t(row) * p.kv_heads + walk.at.head) * bytes + ch * 16u : cache;
+                            cp_async_16_zfill(FP8 ? dst + r * uint32_t(DP) + ch * 16u : dst + (ch >> 3) * C::PANEL + sw128_off(r, ch & 7u), from, there ? 16u : 0u);
+                        }
+                    cp_async_commit();
+                    cp_async_wait_group<0>();
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(FULL_OF + 8 * at);
+                    __syncwarp();
+                }
+            }
+        }
+    };
+
     if (warp < 4) {
-        if (warp == 0) {
+        if (box_rows < 8u && (warp == 0 || warp == 2)) {
+            if (GATHER_RING > 1u) gather(warp >> 1, warp >> 1);
+            else if (warp == 0) gather(0, 1);
+        } else if (warp == 0) {
             // ---- TMA: K and V of a tile, one lane a box ----
             const uint32_t per_tile = TC_KEYS / box_rows;
             const AttnDivisor div = p.page_div;

@@ -62,6 +62,17 @@ def test_more_than_promised(cuda, atlas, lens, promise, fp8):
 
 
 @BOTH
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 256])
+@pytest.mark.parametrize("page", [1, 5, 12])
+def test_chunks_over_pages_of_any_size(cuda, atlas, page, d, fp8):
+    """Pages that no box of eight rows divides: tiles of keys are gathered row by row."""
+    b = Batch(cuda, atlas, [(70, 1111), (33, 33), (0, 9), (257, 300), (1, 128)], 4, 2, d, page, fp8, seed=d + page)
+    atlas.paged_attention(b.desc())
+    assert atlas.last_attention_shape()["block_rows"] == (256 if d <= 128 else 128)
+    b.check()
+
+
+@BOTH
 @pytest.mark.parametrize("heads,lens", [(3, [(700, 3000), (90, 700), (301, 301)]), (5, [(257, 900), (1, 4), (600, 601)]), (7, [(110, 4000), (37, 38)])])
 def test_blocks_that_begin_inside_a_token(cuda, atlas, heads, lens, fp8):
     """Groups that do not divide a block: a token's heads lie in two blocks, and the line of tiles has no period."""
@@ -80,7 +91,7 @@ def test_which_kernel(cuda, atlas):
     assert rows([(1, 300)], 8, 1) == 8 and rows([(1, 300)], 9, 1) == 16 and rows([(2, 300)], 8, 1) == 16
     assert rows([(1, 300)], 17, 1) == 256 and rows([(3, 300)], 8, 1, d=256) == 128
     assert rows([(4, 300)], 8, 1, fp8=True) == 16 and rows([(5, 300)], 8, 1, fp8=True) == 256
-    assert rows([(9, 300)], 8, 1, page=4) == 16                    # pages that no box of eight rows fits
+    assert rows([(9, 300)], 8, 1, page=4) == 256                   # pages that no box of eight rows fits: row by row
     assert rows([(9, 300)], 8, 1, page=24) == 256                  # boxes of eight
     assert rows([(9, 300)], 8, 1, q_extra=2) == 16                 # rows of q that are not on 16 bytes
 
@@ -102,9 +113,10 @@ def test_q_and_out_at_odd_addresses(cuda, atlas, fp8):
 
 
 @BOTH
-def test_wrong_tables_under_a_chunk(cuda, atlas, fp8):
+@pytest.mark.parametrize("page", [16, 4])
+def test_wrong_tables_under_a_chunk(cuda, atlas, page, fp8):
     """A page that is not of the pool reads as zeros; a length beyond the table's row is cut to it."""
-    b = Batch(cuda, atlas, [(40, 333), (20, 90)], 8, 2, 128, 16, fp8, seed=6)
+    b = Batch(cuda, atlas, [(40, 333), (20, 90)], 8, 2, 128, page, fp8, seed=6)
     for bad in (-1, b.n_pages, 0x7FFFFFFF):
         keep = int(b.table_np[0, 3])
         b.table[0, 3] = bad
@@ -113,7 +125,7 @@ def test_wrong_tables_under_a_chunk(cuda, atlas, fp8):
         assert atlas.last_attention_shape()["block_rows"] == 256 and atlas.device_status() == 4
         got, got_l = b.out.clone(), b.lse.clone()
         b.table[0, 3] = keep
-        at = cuda.from_numpy(b.slots(0, 333)[48:64]).cuda()
+        at = cuda.from_numpy(b.slots(0, 333)[3 * page:4 * page]).cuda()
         sides = [t.view(cuda.uint8) for t in (b.k, b.v)]
         held = [t[at].clone() for t in sides]
         for t in sides:
