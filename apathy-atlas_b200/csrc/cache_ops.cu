@@ -231,13 +231,14 @@ template <int DP, bool FP8> int launch_tc(AttnParams p, const TcPlan& plan, cuda
     const uint64_t size = FP8 ? 1 : 2;
     const uint64_t dims[3] = {p.head_dim, p.kv_heads, uint64_t(p.n_pages) * p.block_size};
     const uint64_t strides[2] = {p.head_dim * size, uint64_t(p.kv_heads) * p.head_dim * size};
-    const uint32_t box[3] = {FP8 ? uint32_t(DP) : 64u, 1u, std::max(plan.box_rows, 8u)};   // (below eight: not used)
+    const uint32_t box_rows = std::min(plan.box_rows, uint32_t(C::KEYS));
+    const uint32_t box[3] = {FP8 ? uint32_t(DP) : 64u, 1u, std::max(box_rows, 8u)};   // (below eight: not used)
     const CUtensorMapDataType dt = FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const CUtensorMapSwizzle swz = FP8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
     if (!encode_tensor_map(&map_k, dt, 3, p.k_cache, dims, strides, box, swz) || !encode_tensor_map(&map_v, dt, 3, p.v_cache, dims, strides, box, swz))
         return ATLAS_B200_ERR_DIMS;
     p.ctas = plan.ctas; p.least_tiles = plan.least; p.by_item = plan.by_item; p.shape = shape_of(p, C::ROWS, attn::TC_KEYS, tc_extra(DP));
-    const int rc2 = launch_dependent(attn::attn_tc_kernel<DP, FP8>, plan.ctas, C::THREADS, C::SMEM, st, 1u, map_k, map_v, p, plan.box_rows);
+    const int rc2 = launch_dependent(attn::attn_tc_kernel<DP, FP8>, plan.ctas, C::THREADS, C::SMEM, st, 1u, map_k, map_v, p, box_rows);
     if (rc2 || plan.by_item || plan.ctas < 2) return rc2;
     return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, 1u, p);
 }

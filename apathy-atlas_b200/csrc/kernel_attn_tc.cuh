@@ -42,14 +42,18 @@ template <int DP, bool FP8> struct TcCfg {
     static constexpr int NQ = DP <= 128 ? 2 : 1;                             // row tiles
     static constexpr int ROWS = NQ * int(TC_TILE_ROWS);
     static constexpr int PANELS = DP / 64;                                   // 128-byte panels of a row
-    static constexpr int PANEL = 128 * 128;
-    static constexpr int TILE = PANELS * PANEL;                              // Q of a row tile; K or V of a key tile
-    // K and V tiles share a ring, in the order the products take them: K 0, V 0, K 1, V 1, ...  A tile takes some 3000 cycles from request to
+    // Keys of a tile of K or V: two steps, or one for E4M3 rows of 256, where tiles of two leave room for a raw one, a K and a V alone (8192
+    // tokens, 8 Q + 2 KV heads: 508 us, with one step 471; eight times 64 over 2000, 32 + 8 heads: 85 and 68).  BF16 rows of 256 are
+    // bound by what their boxes bring (421 us, with one step 441).
+    static constexpr int KEYS = DP <= 128 || !FP8 ? 128 : 64;
+    static constexpr int Q_PANEL = 128 * 128, Q_TILE = PANELS * Q_PANEL;     // Q of a row tile
+    static constexpr int PANEL = KEYS * 128, TILE = PANELS * PANEL;          // K or V of a key tile
+    // K and V tiles share a ring, in the order the products take them (tc_turn).  A tile takes some 3000 cycles from request to
     // arrival where every SM asks for one a thousand cycles; with two stages of either side, each released with the last product of an
     // iteration, the MMA warp waited 870 cycles an iteration of 2090.
-    static constexpr int SLOTS = DP <= 64 ? 8 : DP <= 128 ? (FP8 ? 4 : 5) : 2;
-    static constexpr int RAW = FP8 ? 128 * DP : 0, RAW_STAGES = FP8 ? (DP <= 128 ? 2 : 1) : 0;
-    static constexpr int OFF_Q = 0, OFF_KV = NQ * TILE, OFF_RAW = OFF_KV + SLOTS * TILE;
+    static constexpr int SLOTS = DP <= 64 ? 8 : FP8 ? 4 : DP <= 128 ? 5 : 2;
+    static constexpr int RAW = FP8 ? KEYS * DP : 0, RAW_STAGES = FP8 ? 2 : 0;
+    static constexpr int OFF_Q = 0, OFF_KV = NQ * Q_TILE, OFF_RAW = OFF_KV + SLOTS * TILE;
     static constexpr int OFF_BAR = OFF_RAW + RAW_STAGES * RAW;
     static constexpr int N_BAR = 2 * SLOTS + 1 + 7 * NQ + 2 * RAW_STAGES;
     static constexpr int OFF_MISC = OFF_BAR + N_BAR * 8;                     // tensor memory, -, abort; attn_find's words
@@ -108,11 +112,24 @@ template <bool HALF> __device__ __forceinline__ uint32_t pack_pair(float a, floa
     }
 }
 
+// What lies at turn t of a piece of n tiles: tiles of two steps K 0, V 0, K 1, V 1, ...; of one step K 0, K 1, V 0, K 2, V 1, ..., V n - 1,
+// as the scores are two steps ahead of the product with P.
+template <int STEPS> __device__ __forceinline__ void tc_turn(uint32_t t, uint32_t n, uint32_t& side, uint32_t& tile) {
+    if constexpr (STEPS == 2) {
+        side = t & 1u;
+        tile = t >> 1;
+    } else {
+        side = t != 0u && ((t & 1u) == 0u || t == 2u * n - 1u) ? 1u : 0u;
+        tile = t == 2u * n - 1u ? n - 1u : side ? (t - 2u) / 2u : (t + 1u) / 2u;
+    }
+}
+
 template <int DP, bool FP8>
 __global__ void __launch_bounds__(TcCfg<DP, FP8>::THREADS, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnParams p, const uint32_t box_rows) {
     using C = TcCfg<DP, FP8>;
-    constexpr int NQ = C::NQ, SLOTS = C::SLOTS;
+    constexpr int NQ = C::NQ, SLOTS = C::SLOTS, STEPS = C::KEYS / int(TC_STEP);
+    constexpr uint32_t KEYS = C::KEYS;
     extern __shared__ uint8_t attn_smem_raw[];
     const uint32_t base = (smem_u32(attn_smem_raw) + 1023u) & ~1023u;
     uint8_t* const gen = attn_smem_raw + (base - smem_u32(attn_smem_raw));
@@ -161,62 +178,58 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         return t > 2u * walk.t0 ? t - 2u * walk.t0 : 0u;
     };
     // key tiles of the piece that any row tile wants (the last row tile that has rows wants the most)
-    auto tiles_wanted = [&] { return ((NQ == 2 ? max(steps_of(0), steps_of(NQ - 1)) : steps_of(0)) + 1u) / 2u; };
+    auto tiles_wanted = [&] { return ((NQ == 2 ? max(steps_of(0), steps_of(NQ - 1)) : steps_of(0)) + STEPS - 1u) / STEPS; };
 
-    // Tiles row by row, where no box of eight rows divides a page; a row that is not there is zeros.  K by one warp and V by another, each
-    // in its turns of the ring (K 0, V 0, K 1, V 1, ...); a ring of one place has one warp, as two turns of a place would be two phases of
-    // its barrier apart, which a wait cannot tell.
-    constexpr uint32_t GATHER_RING = FP8 ? C::RAW_STAGES : SLOTS;
-    auto gather = [&](uint32_t first, uint32_t last) {                       // sides
-        constexpr uint32_t SIZE = FP8 ? 1 : 2, CH = DP * SIZE / 16;          // 16-byte pieces of a row
+    // Tiles row by row, where no box of eight rows divides a page; a row that is not there is zeros.  Two warps, for the even and the odd
+    // turns: of a ring of two places or more, so that a wait is never two phases of its barrier ahead.
+    auto gather = [&](uint32_t odd) {
+        constexpr uint32_t SIZE = FP8 ? 1 : 2, CH = DP * SIZE / 16, RING = FP8 ? C::RAW_STAGES : SLOTS;      // 16-byte pieces of a row
         const uint32_t EMPTY_OF = FP8 ? RAW_EMPTY : EMPTY, FULL_OF = FP8 ? RAW_FULL : FULL, bytes = p.head_dim * SIZE;
-        uint32_t tile = 0;                                                   // of the CTA
+        uint32_t turn = odd;                                                 // of the CTA
         bool ok = true;
         while (ok && walk.next(p)) {
             const int32_t* table = p.block_table + size_t(walk.seq) * p.table_stride;
             const uint32_t n = tiles_wanted(), kv_len = walk.sq.kv_len;
-            for (uint32_t j = 0; ok && j < n; ++j, ++tile) {
-                const uint32_t pos0 = (walk.t0 + j) * TC_KEYS;
-                int32_t rows[4];
+            for (uint32_t t = odd; ok && t < 2u * n; t += 2, turn += 2) {
+                uint32_t side, j;
+                tc_turn<STEPS>(t, n, side, j);
+                const uint32_t pos0 = walk.t0 * TC_KEYS + j * KEYS, at = turn % RING;
+                int32_t rows[KEYS / 32];
 #pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) {
+                for (uint32_t k = 0; k < KEYS / 32; ++k) {
                     const uint32_t pos = pos0 + 32u * k + lane;
                     rows[k] = pos < kv_len ? attn_cache_row(p, table, pos) : -1;
                 }
-                for (uint32_t side = first; ok && side <= last; ++side) {
-                    const uint8_t* const cache = side ? p.v_cache : p.k_cache;
-                    const uint32_t turn = 2u * tile + side, at = turn % GATHER_RING;
-                    ok = mbar_wait_warp(EMPTY_OF + 8 * at, ((turn / GATHER_RING) & 1u) ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER, 20);
-                    if (!ok) break;
-                    const uint32_t dst = FP8 ? base + C::OFF_RAW + at * C::RAW : base + C::OFF_KV + at * C::TILE;
+                const uint8_t* const cache = side ? p.v_cache : p.k_cache;
+                ok = mbar_wait_warp(EMPTY_OF + 8 * at, ((turn / RING) & 1u) ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER, 20);
+                if (!ok) break;
+                const uint32_t dst = FP8 ? base + C::OFF_RAW + at * C::RAW : base + C::OFF_KV + at * C::TILE;
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k)
+                for (uint32_t k = 0; k < KEYS / 32; ++k)
 #pragma unroll 8
-                        for (uint32_t i = 0; i < CH; ++i) {
-                            const uint32_t in = i * (32u / CH) + lane / CH, r = 32u * k + in, ch = lane % CH;
-                            const int32_t row = __shfl_sync(0xFFFFFFFFu, rows[k], in);
-                            const bool there = row >= 0 && ch * 16u < bytes;
-                            const uint8_t* from = there ? cache + (size_t(row) * p.kv_heads + walk.at.head) * bytes + ch * 16u : cache;
-                            cp_async_16_zfill(FP8 ? dst + r * uint32_t(DP) + ch * 16u : dst + (ch >> 3) * C::PANEL + sw128_off(r, ch & 7u), from, there ? 16u : 0u);
-                        }
-                    cp_async_commit();
-                    cp_async_wait_group<0>();
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(FULL_OF + 8 * at);
-                    __syncwarp();
-                }
+                    for (uint32_t i = 0; i < CH; ++i) {
+                        const uint32_t in = i * (32u / CH) + lane / CH, r = 32u * k + in, ch = lane % CH;
+                        const int32_t row = __shfl_sync(0xFFFFFFFFu, rows[k], in);
+                        const bool there = row >= 0 && ch * 16u < bytes;
+                        const uint8_t* from = there ? cache + (size_t(row) * p.kv_heads + walk.at.head) * bytes + ch * 16u : cache;
+                        cp_async_16_zfill(FP8 ? dst + r * uint32_t(DP) + ch * 16u : dst + (ch >> 3) * C::PANEL + sw128_off(r, ch & 7u), from, there ? 16u : 0u);
+                    }
+                cp_async_commit();
+                cp_async_wait_group<0>();
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(FULL_OF + 8 * at);
+                __syncwarp();
             }
         }
     };
 
     if (warp < 4) {
         if (box_rows < 8u && (warp == 0 || warp == 2)) {
-            if (GATHER_RING > 1u) gather(warp >> 1, warp >> 1);
-            else if (warp == 0) gather(0, 1);
+            gather(warp >> 1);
         } else if (warp == 0) {
             // ---- TMA: K and V of a tile, one lane a box ----
-            const uint32_t per_tile = TC_KEYS / box_rows;
+            const uint32_t per_tile = KEYS / box_rows;
             const AttnDivisor div = p.page_div;
             uint32_t slot = 0, ph = 0, tail_ph = 0, rs = 0, rph = 0;
             bool ok = true;
@@ -224,64 +237,67 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 const int32_t* table = p.block_table + size_t(walk.seq) * p.table_stride;
                 const uint32_t n = tiles_wanted(), kv_len = walk.sq.kv_len;
                 const uint32_t none = p.n_pages * p.block_size;              // a row behind the last page: TMA fills with zeros
-                auto page_of = [&](uint32_t j) -> uint32_t {                 // this lane's box of tile j: its page, as the table has it
-                    const uint32_t pos = (walk.t0 + j) * TC_KEYS + lane * box_rows;
-                    return j < n && lane < per_tile && pos < kv_len ? uint32_t(table[attn_div(pos, div)]) : 0u;
+                auto page_of = [&](uint32_t t) -> uint32_t {                 // this lane's box at turn t: its page, as the table has it
+                    uint32_t side, j;
+                    tc_turn<STEPS>(t, n, side, j);
+                    const uint32_t pos = walk.t0 * TC_KEYS + j * KEYS + lane * box_rows;
+                    return t < 2u * n && lane < per_tile && pos < kv_len ? uint32_t(table[attn_div(pos, div)]) : 0u;
                 };
-                uint32_t id_next = page_of(0);
-                for (uint32_t j = 0; ok && j < n; ++j) {
-                    const uint32_t id = id_next, pos0 = (walk.t0 + j) * TC_KEYS, pos = pos0 + lane * box_rows;
-                    id_next = page_of(j + 1);
-                    uint32_t row = id * p.block_size + (pos - attn_div(pos, div) * p.block_size);
-                    if (id >= p.n_pages) {
-                        record_status(STATUS_PAGE_OUT_OF_RANGE);
-                        row = none;
+                uint32_t id_next = page_of(0), row = 0, left = 0, boxes = 0;
+#pragma unroll STEPS
+                for (uint32_t t = 0; ok && t < 2u * n; ++t) {
+                    uint32_t side, j;
+                    tc_turn<STEPS>(t, n, side, j);
+                    if (STEPS == 1 || side == 0) {                           // (V 0 lies where K 0 lies, and comes next)
+                        const uint32_t id = id_next, pos0 = walk.t0 * TC_KEYS + j * KEYS, pos = pos0 + lane * box_rows;
+                        id_next = page_of(t + STEPS);
+                        row = id * p.block_size + (pos - attn_div(pos, div) * p.block_size);
+                        if (id >= p.n_pages) {
+                            record_status(STATUS_PAGE_OUT_OF_RANGE);
+                            row = none;
+                        }
+                        left = kv_len > pos0 ? kv_len - pos0 : 0u;
+                        boxes = min((left + box_rows - 1) / box_rows, per_tile);
                     }
-                    const uint32_t left = kv_len > pos0 ? kv_len - pos0 : 0u, boxes = min((left + box_rows - 1) / box_rows, per_tile);
+                    const CUtensorMap* const map = side ? &map_v : &map_k;
                     if constexpr (!FP8) {
+                        ok = mbar_wait_warp(EMPTY + 8 * slot, ph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER, 20);
+                        if (!ok) break;
+                        const uint32_t dst = base + C::OFF_KV + slot * C::TILE;
+                        const bool tail = side == 1 && left < KEYS;
+                        const uint32_t full = tail ? V_TAIL : FULL + 8 * slot;
+                        if (lane == 0) mbar_arrive_expect_tx(full, boxes * box_rows * 128u * C::PANELS);
+                        __syncwarp();
+                        if (lane < boxes)
 #pragma unroll
-                        for (int side = 0; side < 2; ++side) {
-                            ok = ok && mbar_wait_warp(EMPTY + 8 * slot, ph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER, 20);
+                            for (int pn = 0; pn < C::PANELS; ++pn)
+                                tma_load_3d(dst + pn * C::PANEL + lane * box_rows * 128u, map, pn * 64, int32_t(walk.at.head), int32_t(row), full);
+                        __syncwarp();
+                        if (tail) {
+                            // behind the sequence's end a page holds anything, and zero times a NaN is one: zeros before the product
+                            ok = mbar_wait_warp(V_TAIL, tail_ph, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER);
+                            tail_ph ^= 1u;
                             if (!ok) break;
-                            const uint32_t dst = base + C::OFF_KV + slot * C::TILE;
-                            const bool tail = side == 1 && left < TC_KEYS;
-                            const uint32_t full = tail ? V_TAIL : FULL + 8 * slot;
-                            if (lane == 0) mbar_arrive_expect_tx(full, boxes * box_rows * 128u * C::PANELS);
-                            __syncwarp();
-                            if (lane < boxes)
+                            for (uint32_t i = lane; i < (KEYS - left) * 8u; i += 32)
 #pragma unroll
-                                for (int pn = 0; pn < C::PANELS; ++pn)
-                                    tma_load_3d(dst + pn * C::PANEL + lane * box_rows * 128u, side ? &map_v : &map_k, pn * 64, int32_t(walk.at.head), int32_t(row), full);
+                                for (int pn = 0; pn < C::PANELS; ++pn) sts128(dst + pn * C::PANEL + left * 128u + i * 16u, 0u, 0u, 0u, 0u);
+                            fence_proxy_async();
                             __syncwarp();
-                            if (tail) {
-                                // behind the sequence's end a page holds anything, and zero times a NaN is one: zeros before the product
-                                ok = mbar_wait_warp(V_TAIL, tail_ph, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER);
-                                tail_ph ^= 1u;
-                                if (!ok) break;
-                                for (uint32_t i = lane; i < (TC_KEYS - left) * 8u; i += 32)
-#pragma unroll
-                                    for (int pn = 0; pn < C::PANELS; ++pn) sts128(dst + pn * C::PANEL + left * 128u + i * 16u, 0u, 0u, 0u, 0u);
-                                fence_proxy_async();
-                                __syncwarp();
-                                if (lane == 0) mbar_arrive(FULL + 8 * slot);
-                                __syncwarp();
-                            }
-                            if (++slot == uint32_t(SLOTS)) { slot = 0; ph ^= 1u; }
+                            if (lane == 0) mbar_arrive(FULL + 8 * slot);
+                            __syncwarp();
                         }
+                        if (++slot == uint32_t(SLOTS)) { slot = 0; ph ^= 1u; }
                     } else {
-#pragma unroll 1
-                        for (int side = 0; side < 2; ++side) {
-                            ok = ok && mbar_wait_warp(RAW_EMPTY + 8 * rs, rph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER, 20);
-                            if (!ok) break;
-                            if (lane == 0) mbar_arrive_expect_tx(RAW_FULL + 8 * rs, boxes * box_rows * uint32_t(DP));
-                            __syncwarp();
-                            if (lane < boxes) {
-                                const uint32_t dst = base + C::OFF_RAW + rs * C::RAW + lane * box_rows * uint32_t(DP);
-                                tma_load_3d(dst, side ? &map_v : &map_k, 0, int32_t(walk.at.head), int32_t(row), RAW_FULL + 8 * rs);
-                            }
-                            __syncwarp();
-                            if (++rs == uint32_t(C::RAW_STAGES)) { rs = 0; rph ^= 1u; }
+                        ok = mbar_wait_warp(RAW_EMPTY + 8 * rs, rph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_PRODUCER, 20);
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(RAW_FULL + 8 * rs, boxes * box_rows * uint32_t(DP));
+                        __syncwarp();
+                        if (lane < boxes) {
+                            const uint32_t dst = base + C::OFF_RAW + rs * C::RAW + lane * box_rows * uint32_t(DP);
+                            tma_load_3d(dst, map, 0, int32_t(walk.at.head), int32_t(row), RAW_FULL + 8 * rs);
                         }
+                        __syncwarp();
+                        if (++rs == uint32_t(C::RAW_STAGES)) { rs = 0; rph ^= 1u; }
                     }
                 }
             }
@@ -301,16 +317,27 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             };
             auto scores = [&](uint32_t h) {                                  // of half h of the key tile in `slot`
                 if (elect_one()) {
-                    const uint64_t q = make_kmajor_sw128_desc(base + C::OFF_Q + g * C::TILE), k = make_kmajor_sw128_desc(base + C::OFF_KV + slot * C::TILE + h * (TC_STEP * 128u));
+                    const uint64_t q = make_kmajor_sw128_desc(base + C::OFF_Q + g * C::Q_TILE);
+                    const uint64_t k = make_kmajor_sw128_desc(base + C::OFF_KV + slot * C::TILE + (STEPS == 2 ? h * (TC_STEP * 128u) : 0u));
 #pragma unroll
                     for (int s = 0; s < DP / 16; ++s)
-                        umma_bf16_ss<false>(t_s + h * TC_STEP, q + (s >> 2) * (C::PANEL >> 4) + (s & 3) * 2, k + (s >> 2) * (C::PANEL >> 4) + (s & 3) * 2, idesc_s, s ? 1u : 0u);
+                        umma_bf16_ss<false>(t_s + h * TC_STEP, q + (s >> 2) * (C::Q_PANEL >> 4) + (s & 3) * 2, k + (s >> 2) * (C::PANEL >> 4) + (s & 3) * 2, idesc_s, s ? 1u : 0u);
                     umma_commit<false>(S_FULL + 8 * (2 * g + h));
                 }
                 __syncwarp();
             };
+            auto product = [&](uint32_t v_at, uint32_t u, uint32_t h) {      // of step u's P with the V at v_at
+                if (elect_one()) {
+                    const uint64_t v = make_mnmajor_sw128_desc(v_at, C::PANEL);
+#pragma unroll
+                    for (int s = 0; s < int(TC_STEP) / 16; ++s)
+                        umma_bf16_ts<false>(t_o, t_s + h * TC_STEP + s * 8u, v + s * (2048 >> 4), idesc_o, (u | s) ? 1u : 0u);
+                    umma_commit<false>(PV_DONE + 8 * (2 * g + h));
+                }
+                __syncwarp();
+            };
             while (ok && walk.next(p)) {
-                const uint32_t mine = steps_of(g), n = 2u * tiles_wanted();
+                const uint32_t mine = steps_of(g), n = uint32_t(STEPS) * tiles_wanted();
                 if (n == 0) continue;
                 ok = tile_there();
                 if (ok && mine) ok = mbar_wait_warp(Q_FULL + 8 * g, q_ph, abort_flag, STATUS_WAIT_EXPIRED_MMA, 20);
@@ -319,11 +346,35 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     q_ph ^= 1u;
                     tcgen05_fence_after();
                     scores(0);
-                    if (mine > 1) scores(1);
+                    if (STEPS == 2 && mine > 1) scores(1);
                 }
                 release(slot);
                 advance();
-                for (uint32_t u0 = 0; ok && u0 < n; u0 += 2) {
+                if (STEPS == 1 && mine > 1) {
+                    ok = tile_there();
+                    if (!ok) break;
+                    scores(1);
+                    release(slot);
+                    advance();
+                }
+                for (uint32_t u = 0; STEPS == 1 && ok && u < n; ++u) {       // (one row tile: mine is n)
+                    const uint32_t h = u & 1u;
+                    ok = tile_there() && mbar_wait_warp(P_FULL + 8 * (2 * g + h), p_ph[h], abort_flag, STATUS_WAIT_EXPIRED_MMA);
+                    if (!ok) break;
+                    p_ph[h] ^= 1u;
+                    tcgen05_fence_after();
+                    product(base + C::OFF_KV + slot * C::TILE, u, h);
+                    release(slot);
+                    advance();
+                    if (u + 2 < n) {
+                        ok = tile_there();
+                        if (!ok) break;
+                        scores(h);
+                        release(slot);
+                        advance();
+                    }
+                }
+                for (uint32_t u0 = 0; STEPS == 2 && ok && u0 < n; u0 += 2) {
                     ok = tile_there();
                     if (!ok) break;
                     const uint32_t v_slot = slot, vd = base + C::OFF_KV + slot * C::TILE;
@@ -338,15 +389,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         if (!ok) continue;
                         p_ph[h] ^= 1u;
                         tcgen05_fence_after();
-                        if (elect_one()) {
-                            const uint64_t v = make_mnmajor_sw128_desc(vd + h * (TC_STEP * 128u), C::PANEL);
-#pragma unroll
-                            for (int s = 0; s < int(TC_STEP) / 16; ++s)
-                                umma_bf16_ts<false>(t_o, t_s + h * TC_STEP + s * 8u, v + s * (2048 >> 4), idesc_o, (u | s) ? 1u : 0u);
-                            umma_commit<false>(PV_DONE + 8 * (2 * g + h));
-                            if (h == 1 || u + 1 == mine) umma_commit<false>(EMPTY + 8 * v_slot);
-                        }
-                        __syncwarp();
+                        product(vd + h * (TC_STEP * 128u), u, h);
+                        if (h == 1 || u + 1 == mine) release(v_slot);
                         if (u + 2 < mine) {
                             if (!k_there) ok = tile_there();
                             if (!ok) continue;
@@ -367,7 +411,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         // ---- softmax: a row a thread ----
         const uint32_t g = (warp - 4) >> 2, quad = warp & 3u, row_in = quad * 32u + lane;
         const uint32_t t_s = tmem + g * 128u + ((quad * 32u) << 16), t_o = tmem + NQ * 128u + g * uint32_t(DP) + ((quad * 32u) << 16);
-        const uint32_t q_tile = base + C::OFF_Q + g * C::TILE;
+        const uint32_t q_tile = base + C::OFF_Q + g * C::Q_TILE;
         const uint32_t D = p.head_dim;
         const AttnDivisor group_div = p.group_div;
         uint32_t s_ph[2] = {0, 0};                                           // of the next step's barriers, and of the ones after
@@ -384,7 +428,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             for (uint32_t i = 0; i < CH; ++i) {
                 const uint32_t idx = i * 32u + lane, r = quad * 32u + idx / CH, ch = idx % CH, row = row0 + r, tok = attn_div(row, group_div);
                 const bool there = r < rows && ch * 8u < D;
-                cp_async_16_zfill(q_tile + (ch >> 3) * C::PANEL + sw128_off(r, ch & 7u),
+                cp_async_16_zfill(q_tile + (ch >> 3) * C::Q_PANEL + sw128_off(r, ch & 7u),
                                   there ? q_head + size_t(tok) * p.q_row_stride + (row - tok * p.group) * D + ch * 8u : p.q, there ? 16u : 0u);
             }
             cp_async_commit();
@@ -406,7 +450,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 uint32_t top = 0;
 #pragma unroll 4
                 for (uint32_t ch = 0; ch < CH; ++ch) {
-                    const uint4 v = lds128(mine + (ch >> 3) * C::PANEL + (((ch & 7u) ^ turn) << 4));
+                    const uint4 v = lds128(mine + (ch >> 3) * C::Q_PANEL + (((ch & 7u) ^ turn) << 4));
                     const uint32_t a = v.x & 0x7FFF7FFFu, b = v.y & 0x7FFF7FFFu, c = v.z & 0x7FFF7FFFu, d = v.w & 0x7FFF7FFFu;
                     top = __vmaxu2(top, __vmaxu2(__vmaxu2(a, b), __vmaxu2(c, d)));
                 }
@@ -416,7 +460,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 next_scale = __uint_as_float(uint32_t(127 - by) << 23);
 #pragma unroll 4
                 for (uint32_t ch = 0; ch < CH; ++ch) {
-                    const uint32_t at = mine + (ch >> 3) * C::PANEL + (((ch & 7u) ^ turn) << 4);
+                    const uint32_t at = mine + (ch >> 3) * C::Q_PANEL + (((ch & 7u) ^ turn) << 4);
                     const uint4 v = lds128(at);
                     sts128(at, pack_pair<true>(bf16_lo(v.x) * up, bf16_hi(v.x) * up), pack_pair<true>(bf16_lo(v.y) * up, bf16_hi(v.y) * up),
                            pack_pair<true>(bf16_lo(v.z) * up, bf16_hi(v.z) * up), pack_pair<true>(bf16_lo(v.w) * up, bf16_hi(v.w) * up));
@@ -591,39 +635,38 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         bool ok = true;
         while (ok && walk.next(p)) {
             const uint32_t n = tiles_wanted(), kv_len = walk.sq.kv_len;
-            for (uint32_t j = 0; ok && j < n; ++j) {
-                const uint32_t pos0 = (walk.t0 + j) * TC_KEYS, left = kv_len > pos0 ? min(kv_len - pos0, TC_KEYS) : 0u;
-#pragma unroll
-                for (int side = 0; side < 2; ++side) {
-                    ok = ok && mbar_wait(RAW_FULL + 8 * rs, rph, abort_flag, STATUS_WAIT_EXPIRED_DEQUANT) &&
-                         mbar_wait(EMPTY + 8 * slot, ph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_DEQUANT);
-                    if (!ok) break;
-                    const uint32_t raw = base + C::OFF_RAW + rs * C::RAW, to = base + C::OFF_KV + slot * C::TILE;
-                    constexpr uint32_t CH = DP / 16;                         // 16-byte pieces of a raw row
+            for (uint32_t turn = 0; ok && turn < 2u * n; ++turn) {
+                uint32_t side, j;
+                tc_turn<STEPS>(turn, n, side, j);
+                const uint32_t pos0 = walk.t0 * TC_KEYS + j * KEYS, left = kv_len > pos0 ? min(kv_len - pos0, KEYS) : 0u;
+                ok = mbar_wait(RAW_FULL + 8 * rs, rph, abort_flag, STATUS_WAIT_EXPIRED_DEQUANT) &&
+                     mbar_wait(EMPTY + 8 * slot, ph ^ 1u, abort_flag, STATUS_WAIT_EXPIRED_DEQUANT);
+                if (!ok) break;
+                const uint32_t raw = base + C::OFF_RAW + rs * C::RAW, to = base + C::OFF_KV + slot * C::TILE;
+                constexpr uint32_t CH = DP / 16;                             // 16-byte pieces of a raw row
 #pragma unroll 4
-                    for (uint32_t i = 0; i < CH; ++i) {
-                        const uint32_t idx = i * 128u + t, r = idx / CH, ch = idx % CH;
-                        uint4 v = lds128(raw + idx * 16u);
-                        if (r >= left) v = make_uint4(0u, 0u, 0u, 0u);       // behind the sequence's end: what was there before, or nothing
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                        uint32_t h[8];
+                for (uint32_t i = 0; i < KEYS * CH / 128u; ++i) {
+                    const uint32_t idx = i * 128u + t, r = idx / CH, ch = idx % CH;
+                    uint4 v = lds128(raw + idx * 16u);
+                    if (r >= left) v = make_uint4(0u, 0u, 0u, 0u);           // behind the sequence's end: what was there before, or nothing
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    uint32_t h[8];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w[k] & 0xFFFFu), __NV_E4M3);
-                            const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w[k] >> 16), __NV_E4M3);
-                            h[2 * k] = uint32_t(a.x) | uint32_t(a.y) << 16;
-                            h[2 * k + 1] = uint32_t(b.x) | uint32_t(b.y) << 16;
-                        }
-                        const uint32_t panel = to + (ch >> 2) * C::PANEL, c0 = (2u * ch) & 7u;
-                        sts128(panel + sw128_off(r, c0), h[0], h[1], h[2], h[3]);
-                        sts128(panel + sw128_off(r, c0 + 1u), h[4], h[5], h[6], h[7]);
+                    for (int k = 0; k < 4; ++k) {
+                        const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w[k] & 0xFFFFu), __NV_E4M3);
+                        const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w[k] >> 16), __NV_E4M3);
+                        h[2 * k] = uint32_t(a.x) | uint32_t(a.y) << 16;
+                        h[2 * k + 1] = uint32_t(b.x) | uint32_t(b.y) << 16;
                     }
-                    fence_proxy_async();
-                    mbar_arrive(FULL + 8 * slot);
-                    mbar_arrive(RAW_EMPTY + 8 * rs);
-                    if (++rs == uint32_t(C::RAW_STAGES)) { rs = 0; rph ^= 1u; }
-                    if (++slot == uint32_t(SLOTS)) { slot = 0; ph ^= 1u; }
+                    const uint32_t panel = to + (ch >> 2) * C::PANEL, c0 = (2u * ch) & 7u;
+                    sts128(panel + sw128_off(r, c0), h[0], h[1], h[2], h[3]);
+                    sts128(panel + sw128_off(r, c0 + 1u), h[4], h[5], h[6], h[7]);
                 }
+                fence_proxy_async();
+                mbar_arrive(FULL + 8 * slot);
+                mbar_arrive(RAW_EMPTY + 8 * rs);
+                if (++rs == uint32_t(C::RAW_STAGES)) { rs = 0; rph ^= 1u; }
+                if (++slot == uint32_t(SLOTS)) { slot = 0; ph ^= 1u; }
             }
         }
     }
