@@ -12,16 +12,17 @@
 // One thread owns a row: its scores come to its registers (tcgen05.ld), maximum and sum need no exchange with other threads, P goes back
 // to tensor memory as the A operand.  Q, K, V are 128-byte-swizzled tiles in shared memory: Q and K K-major, V as it lies in the cache
 // ([key][channel]), the MN-major form of the B operand.  K and V come 128 keys at a time, page by page by TMA, in boxes of the largest
-// power of two that divides page and tile; zero fill stands in for pages that do not exist and for channels behind head_dim.  Pages that no
-// box of eight rows divides are copied row by row past the registers, K by warp 0 and V by warp 2 (pages of 5, 2048
-// tokens over 8192, 8 Q + 2 KV heads of 128: 118 us, the mma.sync form 433; BF16 pages of 16 by TMA 70).
+// power of two that divides page and tile; zero fill stands in for pages that do not exist and for channels behind head_dim.  Pages that
+// no box of eight rows divides are copied row by row past the registers, by warps 0 and 2 in turn (pages of 5, 2048 tokens over 8192,
+// 8 Q + 2 KV heads of 128: 118 us; the mma.sync form takes 433, pages of 16 by TMA 70).
 //
 // O is multiplied with 2^(M_old - M_new) only where a row's maximum has grown by more than 2^15 (TC_RESCALE) since O's last factor: until
 // then the weights are 2^(s - M) with the old M, up to 2^15 (which FP16 holds) and in the same FP32 sums, which is the same quotient.  That
-// takes the correction off the path of nearly every step (8192 tokens, scores' deviations from 1 to 4: 490 us with 2^8, 481 with 2^15).  (Exponentials by a polynomial on the FMA pipe for a quarter to a half of the scores,
-// the special-function unit being the busiest of the softmax: no faster.)
+// takes the correction off the path of nearly every step (8192 tokens, scores' deviations from 1 to 4: 490 us with 2^8, 481 with 2^15).
+// (Exponentials by a polynomial on the FMA pipe for a quarter to a half of the scores, the special-function unit being the busiest of the
+// softmax: no faster.  The next step's scores asked for between the exponentials of this one: they are not there yet, 484 -> 564 us.)
 //
-// Warps: 0 TMA, 1 and 3 MMA of a row tile each (converged, one lane issues), 2 tensor memory; 4-7 and 8-11 softmax, epilogue and Q
+// Warps: 0 TMA (or 0 and 2 copies), 1 and 3 MMA of a row tile each (converged, one lane issues), 2 tensor memory; 4-7 and 8-11 softmax, epilogue and Q
 // of a row tile each, the next item's Q before this one's output; E4M3 caches: 12-15 turn raw tiles into FP16 ones (one instruction for
 // two values, exact, NaN kept; Q as FP16 with a power of two per row, see the mma.sync form).  Every wait is bounded as elsewhere in the
 // library.
@@ -56,7 +57,7 @@ template <int DP, bool FP8> struct TcCfg {
     static constexpr int OFF_Q = 0, OFF_KV = NQ * Q_TILE, OFF_RAW = OFF_KV + SLOTS * TILE;
     static constexpr int OFF_BAR = OFF_RAW + RAW_STAGES * RAW;
     static constexpr int N_BAR = 2 * SLOTS + 1 + 7 * NQ + 2 * RAW_STAGES;
-    static constexpr int OFF_MISC = OFF_BAR + N_BAR * 8;                     // tensor memory, -, abort; attn_find's words
+    static constexpr int OFF_MISC = OFF_BAR + N_BAR * 8;                     // tensor memory, -, abort; attn_begin's words
     static constexpr int SMEM = OFF_MISC + 16 + 16 * 8 + int(sizeof(AttnStart)) + 1024;
     static constexpr int SOFT_WARPS = 4 * NQ, WARPS = 4 + SOFT_WARPS + (FP8 ? 4 : 0), THREADS = 32 * WARPS;
     static constexpr int CONV_WARP0 = 4 + SOFT_WARPS;
