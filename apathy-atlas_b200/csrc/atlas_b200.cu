@@ -1495,8 +1495,8 @@ static int qkv_norm_rope_cache_write(void* q, const void* k_in, const void* v_in
     if (head_dim == 0 || head_dim % 2 || head_dim > uint32_t(KVE_MAX_HEAD_DIM) || rotary_dim > head_dim || rotary_dim % 2 ||
         block_size == 0 || q_row_stride < q_heads * head_dim || kv_row_stride < kv_heads * head_dim)
         return ATLAS_B200_ERR_DIMS;
-    // packed pairs are read as 32-bit words
-    if (!aligned(q, 4) || !aligned(k_in, 4) || !aligned(v_in, 4) || !aligned(v_cache, 4) || !aligned(q_norm_weight, 4) ||
+    // packed pairs are read and written as 32-bit words (pairs of E4M3 codes as 16-bit ones: their entry point looks at k_cache)
+    if (!aligned(q, 4) || !aligned(k_in, 4) || !aligned(v_in, 4) || (!fp8 && !aligned(k_cache, 4)) || !aligned(v_cache, 4) || !aligned(q_norm_weight, 4) ||
         !aligned(k_norm_weight, 4) || q_row_stride % 2 || kv_row_stride % 2)
         return ATLAS_B200_ERR_ALIGN;
     QkvEpilogueParams p{};

@@ -178,7 +178,8 @@ ATLAS_B200_API int atlas_b200_k_norm_rope_cache_write_fp8(const void* k_in, uint
  * convention (norm_offset_one: 1 -> x * rms * (1 + w), 0 -> x * rms * w) and its summation order: same bits.  Unlike the
  * reference, q / k_in / v_in point into the fused QKV output where the projection wrote it: first column of token 0 of each
  * part, with row strides in elements (q_row_stride for q, kv_row_stride for k_in and v_in).
- * head_dim and rotary_dim even, head_dim <= 256 (-1 otherwise); q, k_in and both strides 4-byte aligned (-3). */
+ * head_dim and rotary_dim even, head_dim <= 256 (-1 otherwise); q, k_in, v_in, both norm weights, k_cache and v_cache 4-byte aligned, both
+ * strides even (-3). */
 ATLAS_B200_API int atlas_b200_qkv_norm_rope_cache_write(void* q, const void* k_in, const void* v_in, uint32_t q_row_stride, uint32_t kv_row_stride,
                                          const void* q_norm_weight, const void* k_norm_weight, const uint32_t* positions,
                                          const float* inv_freq, const long long* slot_mapping, void* k_cache, void* v_cache,
