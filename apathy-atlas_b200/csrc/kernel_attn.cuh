@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(ATTN_JOIN_THREADS, 4) attn_join_kernel(const _
             }
         return;
     }
+    if (blockIdx.y >= rows) return;                                          // (the barriers that odd_s needs are in the loop)
     constexpr int V = DP / 32;                                               // channels of a lane, side by side
     for (uint32_t r = blockIdx.y; r < rows; r += ATTN_JOIN_Y) {
         float m = -INFINITY, l = 0.0f;
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(ATTN_JOIN_THREADS, 4) attn_join_kernel(const _
         }
         __syncthreads();
     }
-    for (uint32_t k = warp; k < uint32_t(ROWS) / ATTN_JOIN_Y; k += ATTN_JOIN_WARPS)
+    for (uint32_t k = warp; blockIdx.y + k * ATTN_JOIN_Y < rows; k += ATTN_JOIN_WARPS)
         if ((odd_s >> k) & 1u) {
             place(blockIdx.y + k * ATTN_JOIN_Y, in_seq, token, head);
             attn_row_again<FP8>(p, cut.seq, token, head, attn_row_keys(sq, in_seq), sq.kv_len);
