@@ -1499,7 +1499,7 @@ static int qkv_norm_rope_cache_write(void* q, const void* k_in, const void* v_in
     if (!aligned(q, 4) || !aligned(k_in, 4) || !aligned(v_in, 4) || (!fp8 && !aligned(k_cache, 4)) || !aligned(v_cache, 4) || !aligned(q_norm_weight, 4) ||
         !aligned(k_norm_weight, 4) || q_row_stride % 2 || kv_row_stride % 2)
         return ATLAS_B200_ERR_ALIGN;
-    QkvEpilogueParams p{};
+    QkvEpilogueFp8Params p{};
     p.q = static_cast<uint16_t*>(q);
     p.k_in = static_cast<const uint16_t*>(k_in);
     p.v_in = static_cast<const uint16_t*>(v_in);
@@ -1516,17 +1516,17 @@ static int qkv_norm_rope_cache_write(void* q, const void* k_in, const void* v_in
     // which part of the head is rotated, where the instances know it: 64 channels, or all (see the kernel)
     const bool known = head_dim == 64 || head_dim == 128 || head_dim == 256;
     const uint32_t rot = !known ? 0u : rotary_dim == 64 ? 1u : rotary_dim == head_dim ? 2u : 0u;
-    auto launch = [&](auto kernel) { return launch_chained(kernel, tokens, KVE_WARPS * 32, st, p); };
+    auto launch = [&](auto kernel) { return launch_chained(kernel, tokens, KVE_WARPS * 32, st, p); };   // (BF16 instances take the base's part)
     if (head_dim <= 64) {
-        if (fp8) return rot ? launch(qkv_norm_rope_cache_kernel<1, 1, true>) : launch(qkv_norm_rope_cache_kernel<1, 0, true>);
-        return rot ? launch(qkv_norm_rope_cache_kernel<1, 1>) : launch(qkv_norm_rope_cache_kernel<1, 0>);
+        if (fp8) return rot ? launch(qkv_norm_rope_cache_kernel<1, 1, true>) : launch(qkv_norm_rope_cache_general_kernel<1, true>);
+        return rot ? launch(qkv_norm_rope_cache_kernel<1, 1>) : launch(qkv_norm_rope_cache_general_kernel<1, false>);
     }
     if (head_dim <= 128) {
-        if (fp8) return rot == 2 ? launch(qkv_norm_rope_cache_kernel<2, 2, true>) : rot ? launch(qkv_norm_rope_cache_kernel<2, 1, true>) : launch(qkv_norm_rope_cache_kernel<2, 0, true>);
-        return rot == 2 ? launch(qkv_norm_rope_cache_kernel<2, 2>) : rot ? launch(qkv_norm_rope_cache_kernel<2, 1>) : launch(qkv_norm_rope_cache_kernel<2, 0>);
+        if (fp8) return rot == 2 ? launch(qkv_norm_rope_cache_kernel<2, 2, true>) : rot ? launch(qkv_norm_rope_cache_kernel<2, 1, true>) : launch(qkv_norm_rope_cache_general_kernel<2, true>);
+        return rot == 2 ? launch(qkv_norm_rope_cache_kernel<2, 2>) : rot ? launch(qkv_norm_rope_cache_kernel<2, 1>) : launch(qkv_norm_rope_cache_general_kernel<2, false>);
     }
-    if (fp8) return rot == 2 ? launch(qkv_norm_rope_cache_kernel<4, 2, true>) : rot ? launch(qkv_norm_rope_cache_kernel<4, 1, true>) : launch(qkv_norm_rope_cache_kernel<4, 0, true>);
-    return rot == 2 ? launch(qkv_norm_rope_cache_kernel<4, 2>) : rot ? launch(qkv_norm_rope_cache_kernel<4, 1>) : launch(qkv_norm_rope_cache_kernel<4, 0>);
+    if (fp8) return rot == 2 ? launch(qkv_norm_rope_cache_kernel<4, 2, true>) : rot ? launch(qkv_norm_rope_cache_kernel<4, 1, true>) : launch(qkv_norm_rope_cache_general_kernel<4, true>);
+    return rot == 2 ? launch(qkv_norm_rope_cache_kernel<4, 2>) : rot ? launch(qkv_norm_rope_cache_kernel<4, 1>) : launch(qkv_norm_rope_cache_general_kernel<4, false>);
 }
 
 int atlas_b200_qkv_norm_rope_cache_write(void* q, const void* k_in, const void* v_in, uint32_t q_row_stride, uint32_t kv_row_stride,

@@ -20,6 +20,7 @@
 #include <cstdint>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -95,7 +96,7 @@ __device__ __forceinline__ float kve_mean(const float total, const uint32_t head
 
 constexpr int KVE_TOKENS = 8;                // tokens per CTA (prefill form)
 constexpr int KVE_INFLIGHT = 4;              // heads a warp has loaded before it starts on the first of them
-constexpr int KVE_INFLIGHT_KV = 2;           // decode form: and of K and V
+constexpr int KVE_INFLIGHT_KV = 2;           // decode form, known shapes: and of K and V
 
 // NG: head_dim / 32 rounded up to 2, 4 or 8 (register arrays sized for the head at hand).  EXACT: head_dim = 32 NG,
 // rotary_dim = 64 and a BF16 cache, known when the kernel is compiled (the common shapes): no masked groups, and which
@@ -221,9 +222,10 @@ kv_norm_rope_cache_kernel(KvEpilogueParams p) {
 // (kernels/gb10/common/fused_verify_elemwise.cu:78-224): the normed head is rounded to BF16 before the rotation
 // (the chain it replaced stored it), the angle is position * inv_freq[pair] from a table, cosine and sine are scaled by
 // the attention factor (YaRN), and the weight is `w` or `1 + w`.  One warp per (token, head), Q, K and V read where the
-// projection wrote them (row strides given).  A lane reads the partner element of its pair by one shuffle when
-// rotary_dim = 64 (the halves of a pair are then 16 lanes apart in the head's first 64 channels), otherwise from the
-// BF16 normed head staged in the warp's own shared-memory strip.
+// projection wrote them (row strides given).  A lane has the partner element of its pair by one shuffle when
+// rotary_dim = 64 (the halves of a pair are then 16 lanes apart in the head's first 64 channels), in its own registers
+// when a head of 128 or 256 is rotated whole, otherwise from the BF16 normed head staged in the warp's own shared-memory
+// strip.
 //
 // Summation order of the reference (one block of head_dim threads, thread t squaring the packed pair (2t, 2t + 1), a
 // butterfly per warp, then a butterfly over the warp sums): group g of 64 elements = the reference's warp g, lane l of
@@ -243,47 +245,42 @@ struct QkvEpilogueParams {
     uint32_t tokens, q_heads, kv_heads, head_dim, rotary_dim, block_size, q_row_stride, kv_row_stride;
     float rms_eps, attention_factor;
     uint32_t norm_offset_one;
-    float k_inv_scale, v_inv_scale;   // E4M3 caches (k_cache, v_cache: one byte per element): value * inv_scale, saturating cast
+};
+// E4M3 caches (k_cache, v_cache: one byte per element): value * inv_scale, saturating cast.  (A struct of its own: the general BF16 form
+// is compiled to 3 % more time with these two fields among its parameters, which it does not read.)
+struct QkvEpilogueFp8Params : QkvEpilogueParams {
+    float k_inv_scale, v_inv_scale;
 };
 
 __device__ __forceinline__ uint32_t e4m3_pair(const float lo, const float hi, const float inv_scale) {
     return uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(lo, inv_scale), __fmul_rn(hi, inv_scale)), __NV_SATFINITE, __NV_E4M3));
 }
 
-// MAX_GRP: head_dim / 64 rounded up to 1, 2 or 4.  ROT != 0: head_dim = 64 MAX_GRP is known when the kernel is compiled, and so is
-// rotary_dim, 64 (ROT = 1) or the whole head (ROT = 2), so that no lane is masked, a pair's halves meet by one shuffle or in their
-// lane, and the general form (ROT = 0) with its shared-memory strip drops out.  (64 tokens, 32 Q and 8 KV heads of 128, rotated whole, E4M3
-// caches, alone: 10.5 us by the general form, 6.6 by ROT = 2.)  FP8: the caches are E4M3; a rotated K value goes to its code in one rounding
-// (the normed head is rounded to BF16 before the rotation either way, as Q's is).
+// Heads of 64 MAX_GRP channels (1, 2 or 4 groups), of which 64 (ROT = 1) or all (ROT = 2) are rotated, both known when the kernel is compiled, so
+// that no lane is masked, a pair's halves meet by one shuffle or in their lane, and nothing goes through shared memory but the angles.
+// (64 tokens, 32 Q and 8 KV heads of 128, rotated whole, E4M3 caches, alone: 10.5 us by the general form, 6.6 by this one.)  FP8: the caches are
+// E4M3; a rotated K value goes to its code in one rounding (the normed head is rounded to BF16 before the rotation either way, as Q's is).
 template <uint32_t MAX_GRP, uint32_t ROT, bool FP8 = false>
 __global__ void __launch_bounds__(KVE_WARPS * 32, MAX_GRP == 4 ? 4 : 6)     // (occupancy matters more here than a few held values)
-qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
-    constexpr bool EXACT = ROT != 0;
-    static_assert(ROT != 2 || MAX_GRP > 1, "a head of 64 rotated whole is rotary_dim = 64");
+qkv_norm_rope_cache_kernel(std::conditional_t<FP8, QkvEpilogueFp8Params, QkvEpilogueParams> p) {
+    static_assert(ROT == 1 || (ROT == 2 && MAX_GRP > 1), "a head of 64 rotated whole is rotary_dim = 64");
     pdl_release();
     pdl_wait();
     p.q = pdl_after(p.q); p.k_in = pdl_after(p.k_in); p.v_in = pdl_after(p.v_in); p.positions = pdl_after(p.positions);
     p.slot_mapping = pdl_after(p.slot_mapping);
-    if constexpr (EXACT) { p.head_dim = 64u * MAX_GRP; p.rotary_dim = ROT == 2 ? 64u * MAX_GRP : 64u; }
+    p.head_dim = 64u * MAX_GRP;
+    p.rotary_dim = ROT == 2 ? 64u * MAX_GRP : 64u;
     // one CTA per token; cosine and sine of the token's angles evaluated once for all its heads (see above)
-    __shared__ uint16_t normed_s[EXACT ? 1 : KVE_WARPS][EXACT ? 2 : KVE_MAX_HEAD_DIM];
     __shared__ float cos_s[KVE_MAX_HEAD_DIM / 2], sin_s[KVE_MAX_HEAD_DIM / 2];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t token = blockIdx.x;
     const uint32_t pairs = p.rotary_dim / 2u;
-    const uint32_t n_grp = EXACT ? MAX_GRP : (p.head_dim + 63u) / 64u;     // the reference's warps that hold data
-    const bool in_lanes = EXACT || (p.rotary_dim == 64u && (p.head_dim & 63u) == 0u);
-    uint32_t have = EXACT ? (1u << MAX_GRP) - 1u : 0u;                     // bit g: this lane holds a pair of group g
-    if constexpr (!EXACT) {
-#pragma unroll
-        for (uint32_t g = 0; g < MAX_GRP; ++g)
-            if (g < n_grp && 64u * g + 2u * lane < p.head_dim) have |= 1u << g;
-    }
-
+    float k_inv_scale = 0.0f, v_inv_scale = 0.0f;
+    if constexpr (FP8) { k_inv_scale = p.k_inv_scale; v_inv_scale = p.v_inv_scale; }
     auto load_head = [&](uint32_t (&rw)[MAX_GRP], const uint16_t* x) {
 #pragma unroll
         for (uint32_t g = 0; g < MAX_GRP; ++g)
-            rw[g] = ((have >> g) & 1u) ? *reinterpret_cast<const uint32_t*>(x + 64u * g + 2u * lane) : 0u;
+            rw[g] = *reinterpret_cast<const uint32_t*>(x + 64u * g + 2u * lane);
     };
     // The warp's first heads of either side are asked for before the cosines, whose range reduction for far positions takes as long as they do.
     uint16_t* const q_tok = p.q + size_t(token) * p.q_row_stride;
@@ -317,7 +314,7 @@ qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
         }
     }
     __syncthreads();
-    // in-lane forms: this lane's angles, held for all of the token's heads (rotated whole: two for each of the lower groups)
+    // this lane's angles, held for all of the token's heads (rotated whole: two for each of the lower groups)
     constexpr uint32_t LOW = ROT == 2 ? MAX_GRP / 2 : 1;
     float cs[LOW][2], sn[LOW][2];
 #pragma unroll
@@ -325,8 +322,8 @@ qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
         const uint32_t t = ROT == 2 ? 64u * g + 2u * lane : (2u * lane) & 31u;
 #pragma unroll
         for (uint32_t k = 0; k < 2; ++k) {
-            cs[g][k] = in_lanes ? cos_s[t + k] : 0.0f;
-            sn[g][k] = in_lanes ? sin_s[t + k] : 0.0f;
+            cs[g][k] = cos_s[t + k];
+            sn[g][k] = sin_s[t + k];
         }
     }
     const float c0 = cs[0][0], s0 = sn[0][0], c1 = cs[0][1], s1 = sn[0][1];
@@ -335,7 +332,7 @@ qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
     auto load_factors = [&](float (&f)[MAX_GRP][2], const uint16_t* w) {
 #pragma unroll
         for (uint32_t g = 0; g < MAX_GRP; ++g) {
-            const uint32_t wk = ((have >> g) & 1u) ? *reinterpret_cast<const uint32_t*>(w + 64u * g + 2u * lane) : 0u;
+            const uint32_t wk = *reinterpret_cast<const uint32_t*>(w + 64u * g + 2u * lane);
             const float w0 = __uint_as_float(wk << 16), w1 = __uint_as_float(wk & 0xFFFF0000u);
             f[g][0] = p.norm_offset_one ? __fadd_rn(1.0f, w0) : w0;
             f[g][1] = p.norm_offset_one ? __fadd_rn(1.0f, w1) : w1;
@@ -348,7 +345,7 @@ qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
         constexpr bool CODES = sizeof(*dst) == 1;
         float x0v[MAX_GRP], x1v[MAX_GRP], sq[MAX_GRP];
 #pragma unroll
-        for (uint32_t g = 0; g < MAX_GRP; ++g) {                           // (a group the head does not have was loaded as zero)
+        for (uint32_t g = 0; g < MAX_GRP; ++g) {
             x0v[g] = __uint_as_float(rw[g] << 16);
             x1v[g] = __uint_as_float(rw[g] & 0xFFFF0000u);
             sq[g] = __fadd_rn(__fmul_rn(x0v[g], x0v[g]), __fmul_rn(x1v[g], x1v[g]));
@@ -367,8 +364,8 @@ qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
                 const float h0 = __fadd_rn(__fmul_rn(b0, cs[g][0]), __fmul_rn(a0, sn[g][0])), h1 = __fadd_rn(__fmul_rn(b1, cs[g][1]), __fmul_rn(a1, sn[g][1]));
                 const uint32_t e = 64u * g + 2u * lane;
                 if constexpr (CODES) {
-                    *reinterpret_cast<uint16_t*>(dst + e) = uint16_t(e4m3_pair(l0, l1, p.k_inv_scale));
-                    *reinterpret_cast<uint16_t*>(dst + e + 64u * LOW) = uint16_t(e4m3_pair(h0, h1, p.k_inv_scale));
+                    *reinterpret_cast<uint16_t*>(dst + e) = uint16_t(e4m3_pair(l0, l1, k_inv_scale));
+                    *reinterpret_cast<uint16_t*>(dst + e + 64u * LOW) = uint16_t(e4m3_pair(h0, h1, k_inv_scale));
                 } else {
                     *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(l0, l1);
                     *reinterpret_cast<uint32_t*>(dst + e + 64u * LOW) = pack_bf16x2(h0, h1);
@@ -376,62 +373,28 @@ qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
             }
             return;
         }
-        if (in_lanes) {
-            // rotary_dim = 64 over whole 64-channel groups: a pair's two halves sit 16 lanes apart in group 0, so they
-            // meet by one shuffle and nothing goes through shared memory; the arithmetic is that of the general form
-#pragma unroll
-            for (uint32_t g = 0; g < MAX_GRP; ++g) {
-                if (g >= n_grp) continue;
-                const uint32_t e = 64u * g + 2u * lane;
-                const uint32_t own = pack_bf16x2(__fmul_rn(__fmul_rn(x0v[g], rms), f[g][0]), __fmul_rn(__fmul_rn(x1v[g], rms), f[g][1]));
-                uint32_t out = own;
-                if (g == 0) {
-                    const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, own, 16);
-                    const bool low = lane < 16u;
-                    const uint32_t first = low ? own : other, second = low ? other : own;   // channels t and t + 32
-                    const float a0 = __uint_as_float(first << 16), a1 = __uint_as_float(first & 0xFFFF0000u);
-                    const float b0 = __uint_as_float(second << 16), b1 = __uint_as_float(second & 0xFFFF0000u);
-                    const float r0 = low ? __fsub_rn(__fmul_rn(a0, c0), __fmul_rn(b0, s0)) : __fadd_rn(__fmul_rn(b0, c0), __fmul_rn(a0, s0));
-                    const float r1 = low ? __fsub_rn(__fmul_rn(a1, c1), __fmul_rn(b1, s1)) : __fadd_rn(__fmul_rn(b1, c1), __fmul_rn(a1, s1));
-                    if constexpr (CODES) out = e4m3_pair(r0, r1, p.k_inv_scale);
-                    else out = pack_bf16x2(r0, r1);
-                } else if constexpr (CODES) {
-                    out = e4m3_pair(bf16_lo(own), bf16_hi(own), p.k_inv_scale);
-                }
-                if constexpr (CODES) *reinterpret_cast<uint16_t*>(dst + e) = uint16_t(out);
-                else *reinterpret_cast<uint32_t*>(dst + e) = out;
-            }
-            return;
-        }
-        if constexpr (EXACT) return;
-        __syncwarp();                                                      // the strip's previous head has been read
+        // rotary_dim = 64 over whole 64-channel groups: a pair's two halves sit 16 lanes apart in group 0, so they
+        // meet by one shuffle and nothing goes through shared memory; the arithmetic is that of the general form
 #pragma unroll
         for (uint32_t g = 0; g < MAX_GRP; ++g) {
-            if (!((have >> g) & 1u)) continue;
             const uint32_t e = 64u * g + 2u * lane;
-            normed_s[warp][e] = f32_to_bf16_bits(__fmul_rn(__fmul_rn(x0v[g], rms), f[g][0]));
-            normed_s[warp][e + 1] = f32_to_bf16_bits(__fmul_rn(__fmul_rn(x1v[g], rms), f[g][1]));
-        }
-        __syncwarp();
-        for (uint32_t t = lane; t < p.head_dim; t += 32) {
-            if (t < pairs) {
-                const float a = __uint_as_float(uint32_t(normed_s[warp][t]) << 16);
-                const float b = __uint_as_float(uint32_t(normed_s[warp][t + pairs]) << 16);
-                const float c = cos_s[t], s = sin_s[t];
-                const float r0 = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)), r1 = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
-                if constexpr (CODES) {
-                    const uint32_t codes = e4m3_pair(r0, r1, p.k_inv_scale);
-                    dst[t] = uint8_t(codes);
-                    dst[t + pairs] = uint8_t(codes >> 8);
-                } else {
-                    dst[t] = f32_to_bf16_bits(r0);
-                    dst[t + pairs] = f32_to_bf16_bits(r1);
-                }
-            } else if (t >= p.rotary_dim) {
-                // channels beyond the rotary part pass through
-                if constexpr (CODES) dst[t] = uint8_t(e4m3_pair(__uint_as_float(uint32_t(normed_s[warp][t]) << 16), 0.0f, p.k_inv_scale));
-                else dst[t] = normed_s[warp][t];
+            const uint32_t own = pack_bf16x2(__fmul_rn(__fmul_rn(x0v[g], rms), f[g][0]), __fmul_rn(__fmul_rn(x1v[g], rms), f[g][1]));
+            uint32_t out = own;
+            if (g == 0) {
+                const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, own, 16);
+                const bool low = lane < 16u;
+                const uint32_t first = low ? own : other, second = low ? other : own;   // channels t and t + 32
+                const float a0 = __uint_as_float(first << 16), a1 = __uint_as_float(first & 0xFFFF0000u);
+                const float b0 = __uint_as_float(second << 16), b1 = __uint_as_float(second & 0xFFFF0000u);
+                const float r0 = low ? __fsub_rn(__fmul_rn(a0, c0), __fmul_rn(b0, s0)) : __fadd_rn(__fmul_rn(b0, c0), __fmul_rn(a0, s0));
+                const float r1 = low ? __fsub_rn(__fmul_rn(a1, c1), __fmul_rn(b1, s1)) : __fadd_rn(__fmul_rn(b1, c1), __fmul_rn(a1, s1));
+                if constexpr (CODES) out = e4m3_pair(r0, r1, k_inv_scale);
+                else out = pack_bf16x2(r0, r1);
+            } else if constexpr (CODES) {
+                out = e4m3_pair(bf16_lo(own), bf16_hi(own), k_inv_scale);
             }
+            if constexpr (CODES) *reinterpret_cast<uint16_t*>(dst + e) = uint16_t(out);
+            else *reinterpret_cast<uint32_t*>(dst + e) = out;
         }
     };
 
@@ -461,13 +424,185 @@ qkv_norm_rope_cache_kernel(QkvEpilogueParams p) {
                 uint8_t* dst = reinterpret_cast<uint8_t*>(p.v_cache) + cache_at + (item - p.kv_heads) * p.head_dim;
 #pragma unroll
                 for (uint32_t g = 0; g < MAX_GRP; ++g)
-                    if ((have >> g) & 1u)
-                        *reinterpret_cast<uint16_t*>(dst + 64u * g + 2u * lane) = uint16_t(e4m3_pair(bf16_lo(raw_kv[r][g]), bf16_hi(raw_kv[r][g]), p.v_inv_scale));
+                    *reinterpret_cast<uint16_t*>(dst + 64u * g + 2u * lane) = uint16_t(e4m3_pair(bf16_lo(raw_kv[r][g]), bf16_hi(raw_kv[r][g]), v_inv_scale));
             } else {
                 uint16_t* dst = p.v_cache + cache_at + (item - p.kv_heads) * p.head_dim;
 #pragma unroll
                 for (uint32_t g = 0; g < MAX_GRP; ++g)
-                    if ((have >> g) & 1u) *reinterpret_cast<uint32_t*>(dst + 64u * g + 2u * lane) = raw_kv[r][g];
+                    *reinterpret_cast<uint32_t*>(dst + 64u * g + 2u * lane) = raw_kv[r][g];
+            }
+        }
+    }
+}
+
+// Any other shape; MAX_GRP: head_dim / 64 rounded up to 1, 2 or 4.  (A kernel of its own: with loads ahead of the angles and factors held, as
+// above, and as one template with that one, 16384 tokens of 32 Q and 8 KV heads of 128, 32 channels rotated, took 217 us for 206; 16 Q and
+// 2 KV heads of 256, half rotated, 193 for 174.)
+template <uint32_t MAX_GRP, bool FP8>
+__global__ void __launch_bounds__(KVE_WARPS * 32, MAX_GRP == 4 ? 4 : 6)     // (occupancy matters more here than a few held values)
+qkv_norm_rope_cache_general_kernel(std::conditional_t<FP8, QkvEpilogueFp8Params, QkvEpilogueParams> p) {
+    pdl_release();
+    pdl_wait();
+    p.q = pdl_after(p.q); p.k_in = pdl_after(p.k_in); p.v_in = pdl_after(p.v_in); p.positions = pdl_after(p.positions);
+    p.slot_mapping = pdl_after(p.slot_mapping);
+    // one CTA per token; cosine and sine of the token's angles evaluated once for all its heads (see above)
+    __shared__ uint16_t normed_s[KVE_WARPS][KVE_MAX_HEAD_DIM];
+    __shared__ float cos_s[KVE_MAX_HEAD_DIM / 2], sin_s[KVE_MAX_HEAD_DIM / 2];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t token = blockIdx.x;
+    const uint32_t pairs = p.rotary_dim / 2u;
+    float k_inv_scale = 0.0f, v_inv_scale = 0.0f;
+    if constexpr (FP8) { k_inv_scale = p.k_inv_scale; v_inv_scale = p.v_inv_scale; }
+    {
+        const float pos = float(p.positions[token]);
+        for (uint32_t t = threadIdx.x; t < pairs; t += KVE_WARPS * 32) {
+            const float angle = __fmul_rn(pos, p.inv_freq[t]);
+            cos_s[t] = __fmul_rn(cosf(angle), p.attention_factor);
+            sin_s[t] = __fmul_rn(sinf(angle), p.attention_factor);
+        }
+    }
+    __syncthreads();
+    const long long slot = p.slot_mapping[token];
+    const uint32_t n_grp = (p.head_dim + 63u) / 64u;                      // the reference's warps that hold data
+    const bool in_lanes = p.rotary_dim == 64u && (p.head_dim & 63u) == 0u;
+    // in-lane form: this lane's two angles, held for all of the token's heads
+    float c0 = 0.0f, s0 = 0.0f, c1 = 0.0f, s1 = 0.0f;
+    if (in_lanes) {
+        const uint32_t t = (2u * lane) & 31u;
+        c0 = cos_s[t], s0 = sin_s[t], c1 = cos_s[t + 1], s1 = sin_s[t + 1];
+    }
+    uint32_t have = 0u;                                                    // bit g: this lane holds a pair of group g
+#pragma unroll
+    for (uint32_t g = 0; g < MAX_GRP; ++g)
+        if (g < n_grp && 64u * g + 2u * lane < p.head_dim) have |= 1u << g;
+
+    auto load_head = [&](uint32_t (&rw)[MAX_GRP], const uint16_t* x) {
+#pragma unroll
+        for (uint32_t g = 0; g < MAX_GRP; ++g)
+            rw[g] = ((have >> g) & 1u) ? *reinterpret_cast<const uint32_t*>(x + 64u * g + 2u * lane) : 0u;
+    };
+    // per-head RMS norm, rotation and one rounding of the head held as packed pairs in rw; result to dst (BF16, or E4M3 codes)
+    auto norm_rope_head = [&](const uint32_t (&rw)[MAX_GRP], const uint16_t* w, auto* dst) {
+        constexpr bool CODES = sizeof(*dst) == 1;
+        float x0v[MAX_GRP], x1v[MAX_GRP], sq[MAX_GRP];
+#pragma unroll
+        for (uint32_t g = 0; g < MAX_GRP; ++g) {                           // (a group the head does not have was loaded as zero)
+            x0v[g] = __uint_as_float(rw[g] << 16);
+            x1v[g] = __uint_as_float(rw[g] & 0xFFFF0000u);
+            sq[g] = __fadd_rn(__fmul_rn(x0v[g], x0v[g]), __fmul_rn(x1v[g], x1v[g]));
+        }
+        const float total = kve_group_total<MAX_GRP>(sq, lane);
+        const float rms = rsqrtf(__fadd_rn(kve_mean(total, p.head_dim), p.rms_eps));
+        if (in_lanes) {
+            // rotary_dim = 64 over whole 64-channel groups: a pair's two halves sit 16 lanes apart in group 0, so they
+            // meet by one shuffle and nothing goes through shared memory; the arithmetic is that of the general form
+#pragma unroll
+            for (uint32_t g = 0; g < MAX_GRP; ++g) {
+                if (g >= n_grp) continue;
+                const uint32_t e = 64u * g + 2u * lane;
+                const uint32_t wk = *reinterpret_cast<const uint32_t*>(w + e);
+                const float w0 = __uint_as_float(wk << 16), w1 = __uint_as_float(wk & 0xFFFF0000u);
+                const float f0 = p.norm_offset_one ? __fadd_rn(1.0f, w0) : w0, f1 = p.norm_offset_one ? __fadd_rn(1.0f, w1) : w1;
+                const uint32_t own = pack_bf16x2(__fmul_rn(__fmul_rn(x0v[g], rms), f0), __fmul_rn(__fmul_rn(x1v[g], rms), f1));
+                uint32_t out = own;
+                if (g == 0) {
+                    const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, own, 16);
+                    const bool low = lane < 16u;
+                    const uint32_t first = low ? own : other, second = low ? other : own;   // channels t and t + 32
+                    const float a0 = __uint_as_float(first << 16), a1 = __uint_as_float(first & 0xFFFF0000u);
+                    const float b0 = __uint_as_float(second << 16), b1 = __uint_as_float(second & 0xFFFF0000u);
+                    const float r0 = low ? __fsub_rn(__fmul_rn(a0, c0), __fmul_rn(b0, s0)) : __fadd_rn(__fmul_rn(b0, c0), __fmul_rn(a0, s0));
+                    const float r1 = low ? __fsub_rn(__fmul_rn(a1, c1), __fmul_rn(b1, s1)) : __fadd_rn(__fmul_rn(b1, c1), __fmul_rn(a1, s1));
+                    if constexpr (CODES) out = e4m3_pair(r0, r1, k_inv_scale);
+                    else out = pack_bf16x2(r0, r1);
+                } else if constexpr (CODES) {
+                    out = e4m3_pair(bf16_lo(own), bf16_hi(own), k_inv_scale);
+                }
+                if constexpr (CODES) *reinterpret_cast<uint16_t*>(dst + e) = uint16_t(out);
+                else *reinterpret_cast<uint32_t*>(dst + e) = out;
+            }
+            return;
+        }
+        __syncwarp();                                                      // the strip's previous head has been read
+#pragma unroll
+        for (uint32_t g = 0; g < MAX_GRP; ++g) {
+            if (!((have >> g) & 1u)) continue;
+            const uint32_t e = 64u * g + 2u * lane;
+            const uint32_t wk = *reinterpret_cast<const uint32_t*>(w + e);
+            const float w0 = __uint_as_float(wk << 16), w1 = __uint_as_float(wk & 0xFFFF0000u);
+            const float f0 = p.norm_offset_one ? __fadd_rn(1.0f, w0) : w0, f1 = p.norm_offset_one ? __fadd_rn(1.0f, w1) : w1;
+            normed_s[warp][e] = f32_to_bf16_bits(__fmul_rn(__fmul_rn(x0v[g], rms), f0));
+            normed_s[warp][e + 1] = f32_to_bf16_bits(__fmul_rn(__fmul_rn(x1v[g], rms), f1));
+        }
+        __syncwarp();
+        for (uint32_t t = lane; t < p.head_dim; t += 32) {
+            if (t < pairs) {
+                const float a = __uint_as_float(uint32_t(normed_s[warp][t]) << 16);
+                const float b = __uint_as_float(uint32_t(normed_s[warp][t + pairs]) << 16);
+                const float c = cos_s[t], s = sin_s[t];
+                if constexpr (CODES) {
+                    const uint32_t codes = e4m3_pair(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)), __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s)), k_inv_scale);
+                    dst[t] = uint8_t(codes);
+                    dst[t + pairs] = uint8_t(codes >> 8);
+                } else {
+                    dst[t] = f32_to_bf16_bits(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)));
+                    dst[t + pairs] = f32_to_bf16_bits(__fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s)));
+                }
+            } else if (t >= p.rotary_dim) {
+                // channels beyond the rotary part pass through
+                if constexpr (CODES) dst[t] = uint8_t(e4m3_pair(__uint_as_float(uint32_t(normed_s[warp][t]) << 16), 0.0f, k_inv_scale));
+                else dst[t] = normed_s[warp][t];
+            }
+        }
+    };
+
+    // Q heads, in place: a warp loads KVE_INFLIGHT heads, then works on each
+    uint16_t* const q_tok = p.q + size_t(token) * p.q_row_stride;
+    for (uint32_t h0 = warp; h0 < p.q_heads; h0 += KVE_WARPS * KVE_INFLIGHT) {
+        uint32_t raw[KVE_INFLIGHT][MAX_GRP];
+#pragma unroll
+        for (uint32_t r = 0; r < uint32_t(KVE_INFLIGHT); ++r) {
+            const uint32_t head = h0 + r * KVE_WARPS;
+            if (head < p.q_heads) load_head(raw[r], q_tok + head * p.head_dim);
+        }
+#pragma unroll
+        for (uint32_t r = 0; r < uint32_t(KVE_INFLIGHT); ++r) {
+            const uint32_t head = h0 + r * KVE_WARPS;
+            if (head < p.q_heads) norm_rope_head(raw[r], p.q_norm_w, q_tok + head * p.head_dim);
+        }
+    }
+    if (slot < 0) return;                                                  // (the reference computes a padding token's K and drops it)
+    // K heads into the cache row `slot` (page slot / block_size, offset slot % block_size of [pages, block_size, kv_heads,
+    // head_dim]), V heads copied beside them: items 0 .. kv_heads-1 are K, the rest V
+    const uint16_t* const k_tok = p.k_in + size_t(token) * p.kv_row_stride;
+    const uint16_t* const v_tok = p.v_in + size_t(token) * p.kv_row_stride;
+    const size_t cache_at = size_t(slot) * (size_t(p.kv_heads) * p.head_dim);
+    for (uint32_t i0 = warp; i0 < 2u * p.kv_heads; i0 += KVE_WARPS * KVE_INFLIGHT) {
+        uint32_t raw[KVE_INFLIGHT][MAX_GRP];
+#pragma unroll
+        for (uint32_t r = 0; r < uint32_t(KVE_INFLIGHT); ++r) {
+            const uint32_t item = i0 + r * KVE_WARPS;
+            if (item < 2u * p.kv_heads)
+                load_head(raw[r], item < p.kv_heads ? k_tok + item * p.head_dim : v_tok + (item - p.kv_heads) * p.head_dim);
+        }
+#pragma unroll
+        for (uint32_t r = 0; r < uint32_t(KVE_INFLIGHT); ++r) {
+            const uint32_t item = i0 + r * KVE_WARPS;
+            if (item >= 2u * p.kv_heads) continue;
+            if (item < p.kv_heads) {
+                if constexpr (FP8) norm_rope_head(raw[r], p.k_norm_w, reinterpret_cast<uint8_t*>(p.k_cache) + cache_at + item * p.head_dim);
+                else norm_rope_head(raw[r], p.k_norm_w, p.k_cache + cache_at + item * p.head_dim);
+            } else if constexpr (FP8) {
+                uint8_t* dst = reinterpret_cast<uint8_t*>(p.v_cache) + cache_at + (item - p.kv_heads) * p.head_dim;
+#pragma unroll
+                for (uint32_t g = 0; g < MAX_GRP; ++g)
+                    if ((have >> g) & 1u)
+                        *reinterpret_cast<uint16_t*>(dst + 64u * g + 2u * lane) = uint16_t(e4m3_pair(bf16_lo(raw[r][g]), bf16_hi(raw[r][g]), v_inv_scale));
+            } else {
+                uint16_t* dst = p.v_cache + cache_at + (item - p.kv_heads) * p.head_dim;
+#pragma unroll
+                for (uint32_t g = 0; g < MAX_GRP; ++g)
+                    if ((have >> g) & 1u) *reinterpret_cast<uint32_t*>(dst + 64u * g + 2u * lane) = raw[r][g];
             }
         }
     }
