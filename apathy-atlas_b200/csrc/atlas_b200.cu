@@ -1670,15 +1670,12 @@ int atlas_b200_device_status(uint32_t* out_word, int clear) {
     if (!out_word) return ATLAS_B200_ERR_NULL;
     cudaError_t e = cudaMemcpyFromSymbol(out_word, g_status_word, sizeof(uint32_t));
     if (e != cudaSuccess) return cuda_status(e);
-    if (clear) {
+    if (*out_word == 0) return cache_device_status(out_word, clear);   // the cache operators' kernels have a word of their own
+    if (clear) {                                                       // (that one stays, for the next call to report)
         const uint32_t zero = 0;
         e = cudaMemcpyToSymbol(g_status_word, &zero, sizeof(uint32_t));
-        if (e != cudaSuccess) return cuda_status(e);
     }
-    uint32_t more = 0;                                       // the cache operators' kernels have a word of their own
-    const int rc = cache_device_status(&more, clear);
-    if (*out_word == 0) *out_word = more;
-    return rc;
+    return cuda_status(e);
 }
 
 int atlas_b200_selftest_bounded_wait(uint64_t limit_ns, uint32_t out_host[3]) {

@@ -577,7 +577,8 @@ ATLAS_B200_API int atlas_b200_cache_compact(const atlas_b200_cache_desc* desc, i
  */
 /* Device status word: 0 = clean; otherwise the first problem a kernel recorded (out-of-range
  * slot index, a bounded wait that expired).  Synchronises the device; not for use during
- * stream capture.  `clear` != 0 resets it. */
+ * stream capture.  `clear` != 0 resets what was returned.  The operators around the paged cache (attention, pages) keep a word of their own, which
+ * is returned where the other is 0: one call reports one problem, and after a reset the next call the other. */
 ATLAS_B200_API int atlas_b200_device_status(uint32_t* out_word, int clear);
 /* Kernel family chosen by the most recent fused / base call on this thread. */
 /* Self-test of the bounded wait every kernel of this library is built on (not on any data path; allocates 12 bytes and
