@@ -57,7 +57,7 @@ __device__ __forceinline__ AttnSeqAt attn_seq(const AttnParams& p, uint32_t s) {
     r.q_len = end > r.row0 ? end - r.row0 : 0u;
     const uint64_t room = uint64_t(p.table_stride) * p.block_size;
     r.kv_len = n < 0 ? 0u : (uint64_t(n) > room ? uint32_t(room) : uint32_t(n));
-    if (n > 0 && uint64_t(n) > room) record_status(STATUS_CACHE_LENGTH);
+    if (n > 0 && uint64_t(n) > room && r.q_len) record_status(STATUS_CACHE_LENGTH);   // (a sequence without new tokens is skipped, whatever its length says)
     return r;
 }
 

@@ -23,3 +23,20 @@ def test_neither_record_hides_the_other(cuda, atlas):
         assert atlas.device_status(clear=False) == 4   # a page that is not of the pool, of the attention's
         assert atlas.device_status() == 4
         assert atlas.device_status() == 0
+
+
+@pytest.mark.parametrize("chunk", [1, 60], ids=["decode", "chunk"])
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "e4m3"])
+def test_a_skipped_sequence_leaves_no_record(cuda, atlas, chunk, fp8):
+    """Entries without new tokens pad a captured batch: their lengths and tables may hold anything."""
+    lens = [(chunk, 500), (0, 0), (chunk, 70), (0, 0), (0, 0)]
+    b = Batch(cuda, atlas, lens, 8, 2, 64, 16, fp8, seed=2)
+    b.kv[1], b.kv[3], b.kv[4] = 0x7FFFFFFF, b.stride * 16 + 1, -1
+    desc = b.desc()
+    atlas.paged_attention(desc)
+    b.check()                                          # (and the status is 0)
+    b.kv[0] = 0x7FFFFFFF                               # one that has new tokens is recorded
+    b.table[0] = b.table[0, 0]
+    atlas.paged_attention(desc)
+    cuda.cuda.synchronize()
+    assert atlas.device_status() == 5 and atlas.device_status() == 0
