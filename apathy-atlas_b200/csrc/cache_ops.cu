@@ -134,15 +134,21 @@ bool whole_items_pay(uint64_t items, uint64_t places, uint64_t ctas) {
     return rounds <= 2 && rounds * places <= items * places * 3 / (4 * ctas) + 12;
 }
 
-// The mma.sync form: how many CTAs, and whether each takes whole items.
+// Scratch for the cuts and the pieces of up to `ctas` ranges.
+size_t cuts_bytes(uint32_t ctas, uint32_t block_rows, uint32_t dim) { return ATTN_CUT_BYTES + size_t(ctas) * 2 * attn_part_floats(block_rows, dim) * sizeof(float); }
+
+// Rows that a KV head has in the longest chunk.
+uint64_t chunk_rows(const atlas_b200_attention_desc& d) { return uint64_t(std::min(d.max_q_len, d.n_tokens)) * (d.q_heads / d.kv_heads); }
+
+// The mma.sync form: how many CTAs, and whether each takes whole items.  (Nothing is cut up to MMA_WHOLE_TILES tiles.)
+constexpr uint64_t MMA_WHOLE_TILES = 4;
 struct MmaPlan {
     uint32_t ctas, by_item, least, tile, block_rows, cluster_log2;
-    size_t ws_bytes;
+    size_t ws_bytes, most_ws_bytes;      // that it takes; that fewer sequences or shorter ones may take
 };
 MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms, bool scratch) {
     const uint32_t dim = attn_dim(d.head_dim);
-    const uint64_t group = d.q_heads / d.kv_heads;
-    const uint64_t rows = std::min<uint64_t>(d.max_q_len, d.n_tokens) * group;
+    const uint64_t rows = chunk_rows(d);
     MmaPlan r{};
     r.block_rows = rows <= 8 ? 8u : 16u;
     const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3;
@@ -157,11 +163,12 @@ MmaPlan plan_mma(const atlas_b200_attention_desc& d, uint32_t sms, bool scratch)
     if (scratch && tiles > 8ull << r.cluster_log2) r.cluster_log2 = 0;
     // 64 sequences of 500 tokens, 8 KV heads of 128, 29.8 us whole and 35.0 cut; 64 of 300, 22.0 and 26.5; 40 of 700, 33.4 and 31.3; over E4M3
     // 40 of 700, 22.9 and 29.1.
-    r.by_item = !scratch || r.cluster_log2 || tiles <= 4 || whole_items_pay(items, tiles + MMA_EXTRA, resident);      // (no scratch: nothing is cut)
+    r.by_item = !scratch || r.cluster_log2 || tiles <= MMA_WHOLE_TILES || whole_items_pay(items, tiles + MMA_EXTRA, resident);      // (no scratch: nothing is cut)
     r.least = r.by_item ? 1u : 4u;
     const uint64_t places = r.by_item ? items : (items * (tiles + MMA_EXTRA) + r.least - 1) / r.least;
     r.ctas = uint32_t(std::min<uint64_t>(r.cluster_log2 ? items : resident, std::max<uint64_t>(places, 1)));
-    r.ws_bytes = r.by_item ? 0 : ATTN_CUT_BYTES + size_t(resident) * 2 * attn_part_floats(r.block_rows, dim) * sizeof(float);
+    r.most_ws_bytes = tiles <= MMA_WHOLE_TILES ? 0 : cuts_bytes(resident, r.block_rows, dim);
+    r.ws_bytes = r.by_item ? 0 : r.most_ws_bytes;
     return r;
 }
 
@@ -183,42 +190,45 @@ template <int DP, bool FP8> int launch_mma(const AttnParams& p, const MmaPlan& p
 
 // The tcgen05 form.  It reads pages in boxes of the largest power of two that divides page and tile, or row by row where that is less than a
 // swizzle atom's eight rows; and Q and the outputs in sixteen bytes.
+constexpr uint64_t TC_WHOLE_TILES = 2;
 struct TcPlan {
     uint32_t ctas, by_item, least, box_rows;
-    size_t ws_bytes;
+    size_t ws_bytes, most_ws_bytes;      // as above
 };
 uint32_t tc_box_rows(uint32_t block_size) {
     uint32_t r = attn::TC_KEYS;
     while (block_size % r) r /= 2;
     return r;
 }
-bool takes_tc(const atlas_b200_attention_desc& d) {
+bool rows_pay_for_tc(const atlas_b200_attention_desc& d) {
     // Rows of a KV head from which on the tensor cores' 256-row blocks pay, although most of such a block is empty.  16 sequences of 4000
     // tokens, 8 KV heads of 128, this form / mma.sync: BF16, 12 rows 64 / 56 us, 24 rows 64 / 89, 40 rows 66 / 129; E4M3, whose tiles
     // are converted by four warps, 24 rows 92 / 79.
     // Over pages that are copied row by row it costs half as much again (pages of 5: BF16 head_dim 128, 20 rows 136 / 93, 48 rows 136 / 131,
     // 64 rows 136 / 168; head_dim 256, 209 / 266 with 20 rows; E4M3 head_dim 128, 111 / 112 with 48 rows).
-    const uint64_t rows = uint64_t(std::min(d.max_q_len, d.n_tokens)) * (d.q_heads / d.kv_heads);
     const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3, boxes = tc_box_rows(d.block_size) >= 8;
     const uint64_t from = boxes ? (fp8 ? 32 : 16) : !fp8 && d.head_dim > 128 ? 16 : 48;
-    return rows > from && aligned(d.q, 16) && aligned(d.out, 16) && d.q_row_stride % 8 == 0 && d.out_row_stride % 8 == 0;
+    return chunk_rows(d) > from;
+}
+bool takes_tc(const atlas_b200_attention_desc& d) {
+    return rows_pay_for_tc(d) && aligned(d.q, 16) && aligned(d.out, 16) && d.q_row_stride % 8 == 0 && d.out_row_stride % 8 == 0;
 }
 TcPlan plan_tc(const atlas_b200_attention_desc& d, uint32_t sms) {
     sms = std::min(sms, ATTN_MAX_CTAS);
     const uint32_t dim = attn_dim(d.head_dim), block_rows = dim <= 128 ? 256u : 128u;
-    const uint64_t rows = uint64_t(std::min(d.max_q_len, d.n_tokens)) * (d.q_heads / d.kv_heads);
-    const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * ((rows + block_rows - 1) / block_rows);
+    const uint64_t items = uint64_t(d.n_seqs) * d.kv_heads * ((chunk_rows(d) + block_rows - 1) / block_rows);
     const uint64_t tiles = std::max<uint64_t>((uint64_t(d.max_kv_len) + attn::TC_KEYS - 1) / attn::TC_KEYS, 1);
     TcPlan r{};
     r.box_rows = tc_box_rows(d.block_size);
     // Two chunks of 512 over 1024 tokens, 8 KV heads of 128, 24.2 us whole and 42.3 cut; 300 over 300, 12.2 and 22.2; eight of 64 over
     // 2000, head_dim 64, 32.6 and 30.5.
     const uint64_t item = tiles + tc_extra(dim);
-    r.by_item = tiles <= 2 || whole_items_pay(items, item, sms);
+    r.by_item = tiles <= TC_WHOLE_TILES || whole_items_pay(items, item, sms);
     r.least = r.by_item ? 1u : 2u;
     const uint64_t places = r.by_item ? items : (items * item + r.least - 1) / r.least;
     r.ctas = uint32_t(std::min<uint64_t>(sms, std::max<uint64_t>(places, 1)));
-    r.ws_bytes = r.by_item ? 0 : ATTN_CUT_BYTES + size_t(sms) * 2 * attn_part_floats(block_rows, dim) * sizeof(float);
+    r.most_ws_bytes = tiles <= TC_WHOLE_TILES ? 0 : cuts_bytes(sms, block_rows, dim);
+    r.ws_bytes = r.by_item ? 0 : r.most_ws_bytes;
     return r;
 }
 
@@ -243,8 +253,12 @@ template <int DP, bool FP8> int launch_tc(AttnParams p, const TcPlan& plan, cuda
     return launch_dependent(attn_join_kernel<C::ROWS, DP, FP8>, dim3(plan.ctas - 1, ATTN_JOIN_Y), ATTN_JOIN_THREADS, 0, st, 1u, p);
 }
 
-// (Which kernel runs also goes by the alignment of pointers that may not be set yet when scratch is asked for: enough for either.)
-size_t attention_ws_bytes(const atlas_b200_attention_desc& d, uint32_t sms) { return std::max(plan_mma(d, sms, true).ws_bytes, plan_tc(d, sms).ws_bytes); }
+// What is asked for does not shrink as sequences are added or grow, although fewer of them may be cut: a buffer for a server's largest batch
+// does for all smaller ones.  (Which kernel runs also goes by the alignment of pointers that may not be set yet: enough for either where the
+// rows alone would have it tcgen05.)
+size_t attention_ws_bytes(const atlas_b200_attention_desc& d, uint32_t sms) {
+    return std::max(plan_mma(d, sms, true).most_ws_bytes, rows_pay_for_tc(d) ? plan_tc(d, sms).most_ws_bytes : size_t(0));
+}
 
 int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
     if (d.n_seqs == 0 || d.n_tokens == 0) return ATLAS_B200_OK;
@@ -252,9 +266,10 @@ int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
     if (bad) return bad;
     if (!device_is_sm100()) return ATLAS_B200_ERR_ARCH;
     const uint32_t sms = uint32_t(device_sm_count()), dim = attn_dim(d.head_dim);
-    if (d.ws ? d.ws_bytes < attention_ws_bytes(d, sms) : d.ws_bytes != 0) return ATLAS_B200_ERR_WORKSPACE;
+    if (!d.ws && d.ws_bytes) return ATLAS_B200_ERR_WORKSPACE;
     if (takes_tc(d)) {
         TcPlan plan = plan_tc(d, sms);
+        if (d.ws && d.ws_bytes < plan.ws_bytes) return ATLAS_B200_ERR_WORKSPACE;
         if (!d.ws && !plan.by_item) { plan.by_item = 1; plan.least = 1; }
         const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3;
         const AttnParams p = attention_params(d);
@@ -264,6 +279,7 @@ int attention(const atlas_b200_attention_desc& d, cudaStream_t st) {
         return fp8 ? launch_tc<256, true>(p, plan, st) : launch_tc<256, false>(p, plan, st);
     }
     const MmaPlan plan = plan_mma(d, sms, d.ws != nullptr);
+    if (d.ws && d.ws_bytes < plan.ws_bytes) return ATLAS_B200_ERR_WORKSPACE;
     const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3;
     const AttnParams p = attention_params(d);
     t_attn_shape[0] = plan.block_rows; t_attn_shape[1] = plan.ctas << plan.cluster_log2; t_attn_shape[2] = plan.by_item; t_attn_shape[3] = plan.tile;

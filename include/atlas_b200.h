@@ -500,7 +500,7 @@ ATLAS_B200_API int32_t atlas_b200_registry_select_victim(const atlas_b200_regist
  *   n_tokens     rows of q and out;  max_q_len, max_kv_len: no sequence has more (launch shapes go by them; more is computed all the
  *                same, only slower)
  *   ws           scratch of atlas_b200_paged_attention_ws_bytes(desc) bytes, 32-byte aligned, holding nothing between calls: calls
- *                that may overlap on the GPU need one each.  NULL: no sequence's cache is split over several SMs, which is slow where
+ *                that may overlap on the GPU need one each.  Less than the call's kernel takes is refused (-2).  NULL: no sequence's cache is split over several SMs, which is slow where
  *                there are few sequences.
  * head_dim a multiple of 32 up to 256, any group and block_size; scales positive and finite (-1).  n_pages * block_size and
  * table_stride * block_size below 2^31 (-5).  Caches 16-byte aligned, q 4-byte with an even stride (-3).  A block table entry outside
@@ -528,7 +528,8 @@ typedef struct atlas_b200_attention_desc {
 } atlas_b200_attention_desc;
 
 ATLAS_B200_API int atlas_b200_paged_attention(const atlas_b200_attention_desc* desc, void* stream);
-/* Scratch for this descriptor (its pointers are not looked at) on the current device. */
+/* Scratch for this descriptor (its pointers are not looked at) on the current device.  It does for every call with the same heads, head_dim,
+ * cache_dtype and block_size and no more sequences, tokens, max_q_len and max_kv_len. */
 ATLAS_B200_API size_t atlas_b200_paged_attention_ws_bytes(const atlas_b200_attention_desc* desc);
 
 /* ---------------------------------------------------------------------------------------

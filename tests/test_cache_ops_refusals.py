@@ -1,4 +1,6 @@
 """Refusals of calls around the paged cache that a kernel could not carry out, and what their scratch is asked for: no device is touched."""
+import itertools
+
 import pytest
 
 OK, ALIGN = 0, -3
@@ -18,3 +20,31 @@ def test_bf16_writer_refuses_what_its_words_cannot_reach(atlas, d, rot):
     for which in ("q", "k_in", "v_in", "qw", "kw", "kc", "vc"):
         assert call(**{which: A + 2}) == ALIGN, which
     assert call(stride=1025) == ALIGN
+
+
+def _scratch(atlas, n_seqs, new, kv, heads=32, kv_heads=8, d=128, fp8=False, page=16):
+    desc = atlas.make_attention_desc(q=None, out=None, k_cache=None, v_cache=None, block_table=None, cu_q=None, kv_len=None, n_seqs=n_seqs, n_tokens=n_seqs * new,
+                                     max_q_len=new, max_kv_len=kv, n_pages=1 << 16, block_size=page, table_stride=1 << 14, q_heads=heads, kv_heads=kv_heads,
+                                     head_dim=d, softmax_scale=0.1, cache_dtype=int(fp8))
+    return atlas.attention_ws_bytes(desc)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,fp8,page", [(32, 8, 128, False, 16), (32, 8, 128, True, 16), (8, 2, 64, False, 5), (12, 4, 96, True, 24), (16, 1, 256, False, 16),
+                                                       (16, 2, 256, True, 7), (5, 5, 32, False, 1)])
+def test_scratch_of_the_largest_batch_does_for_all(atlas, heads, kv_heads, d, fp8, page):
+    """Fewer sequences, tokens or cached ones never ask for more."""
+    seqs, new, kv = (1, 2, 4, 8, 16, 18, 32, 64, 300), (1, 2, 3, 5, 8, 9, 17, 64, 700), (1, 64, 200, 257, 300, 600, 4096, 100000)
+    size = {k: _scratch(atlas, *k, heads, kv_heads, d, fp8, page) for k in itertools.product(seqs, new, kv)}
+    for axis, values in enumerate((seqs, new, kv)):
+        for k, n in size.items():
+            at = values.index(k[axis])
+            if at:
+                less = k[:axis] + (values[at - 1],) + k[axis + 1:]
+                assert size[less] <= n, (less, k)
+    assert size[1, 1, 1] == 0                                  # one tile: nothing is ever cut
+
+
+def test_scratch_is_that_of_the_kernel_that_runs(atlas):
+    """Single tokens of four heads never take the tcgen05 form, whose pieces are thirty times as large."""
+    decode, chunk = _scratch(atlas, 8, 1, 4096), _scratch(atlas, 8, 64, 4096)
+    assert 0 < decode < 4 << 20 < 16 << 20 < chunk

@@ -44,3 +44,23 @@ def test_many_pieces_of_few_rows(cuda, atlas, new, heads, kv_heads, d, block_row
     assert ((b.out[:b.rows].double().view(out.shape) - out).abs() <= tol)[keep].all()
     assert ((b.lse[:b.rows].double() - lse).abs() <= tol_l).all()
     assert (b.out[b.rows:] == 77.0).all() and (b.lse[b.rows:] == 77.0).all() and atlas.device_status() == 0
+
+
+@BOTH
+@pytest.mark.parametrize("new,kv", [(1, 5000), (40, 3000)])
+def test_one_scratch_buffer_over_batch_sizes(cuda, atlas, new, kv, fp8):
+    """A buffer as the largest batch asks for it serves the smaller ones, although these are cut into more pieces."""
+    torch = cuda
+    largest = Batch(cuda, atlas, [(new, kv)] * 20, 16, 4, 128, 16, fp8, seed=1).desc(ws=False)
+    n = atlas.attention_ws_bytes(largest)
+    ws = torch.full((n // 4,), math.nan, dtype=torch.float32, device="cuda")
+    cut = 0
+    for seqs in (20, 16, 8, 3, 1):
+        b = Batch(cuda, atlas, [(new, kv - 7 * i) for i in range(seqs)], 16, 4, 128, 16, fp8, seed=seqs)
+        d = b.desc(ws=False)
+        d.ws, d.ws_bytes = ws.data_ptr(), n
+        assert atlas.attention_ws_bytes(d) <= n
+        atlas.paged_attention(d)
+        b.check()
+        cut += not atlas.last_attention_shape()["whole_items"]
+    assert cut
