@@ -83,7 +83,7 @@ int check_attention(const atlas_b200_attention_desc& d) {
     if (d.cache_dtype != ATLAS_B200_CACHE_BF16 && d.cache_dtype != ATLAS_B200_CACHE_E4M3) return ATLAS_B200_ERR_DIMS;
     if (uint64_t(d.q_heads) * d.head_dim > d.q_row_stride || uint64_t(d.q_heads) * d.head_dim > d.out_row_stride) return ATLAS_B200_ERR_DIMS;
     if (!(d.softmax_scale > 0.0f) || !std::isfinite(d.softmax_scale) || !(d.k_scale > 0.0f) || !std::isfinite(d.k_scale) || !(d.v_scale > 0.0f) ||
-        !std::isfinite(d.v_scale))
+        !std::isfinite(d.v_scale) || !std::isfinite(d.softmax_scale * d.k_scale * ATTN_LOG2E))
         return ATLAS_B200_ERR_DIMS;
     if (d.cache_dtype == ATLAS_B200_CACHE_BF16 && (d.k_scale != 1.0f || d.v_scale != 1.0f)) return ATLAS_B200_ERR_DIMS;
     // rows of the cache and places of a sequence are counted in 31 bits

@@ -67,6 +67,9 @@ struct AttnCut {
     uint32_t seq, block, head;
 };
 
+// The scores' factor must not come to zero: zero times a masked place's -inf is a NaN.  From here down all scores are equal.
+__device__ __forceinline__ float attn_factor(float c) { return fmaxf(c, 1.1754944e-38f); }
+
 // 2^x by the special-function unit; off by 2^-22 of the value at most, 0 below 2^-126
 __device__ __forceinline__ float attn_exp2(float x) {
     float y;
@@ -260,7 +263,7 @@ __device__ __noinline__ void attn_row_again(const AttnParams& p, uint32_t seq, u
     const uint32_t* q = reinterpret_cast<const uint32_t*>(p.q + size_t(token) * p.q_row_stride + size_t(head) * D);
     constexpr uint32_t size = fp8 ? 1 : 2, AT_ONCE = 4;
     float o[8] = {}, m = -INFINITY, l = 0.0f;
-    const float c = p.scale * p.k_scale * ATTN_LOG2E;
+    const float c = attn_factor(p.scale * p.k_scale * ATTN_LOG2E);
     for (uint32_t j0 = 0; j0 < keys; j0 += 32) {
         const uint32_t n = min(keys - j0, 32u);
         const int32_t row = lane < n ? attn_cache_row(p, table, j0 + lane) : -1;

@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_m
                 // holds either way; rows of zeros, infinities or NaN are left as they are.)
                 const int e = int(top >> 7), by = e == 0 || e == 255 ? 0 : min(max(141 - e, -120), 120);
                 const float up = __uint_as_float(uint32_t(127 + by) << 23);
-                c *= p.k_scale * __uint_as_float(uint32_t(127 - by) << 23);
+                c = attn_factor(c * p.k_scale * __uint_as_float(uint32_t(127 - by) << 23));
 #pragma unroll
                 for (int s = 0; s < KS; ++s)
 #pragma unroll

@@ -480,7 +480,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const uint32_t row = row0 + row_in, tok = attn_div(row, group_div), head = walk.at.head * p.group + row - tok * p.group;
             const uint32_t keys = row_in < rows ? attn_row_keys(walk.sq, tok) : 0u, all_see = attn_row_keys(walk.sq, attn_div(row0, group_div));
             float c = p.scale * p.k_scale * ATTN_LOG2E, m = -INFINITY, l = 0.0f;
-            if constexpr (FP8) c *= next_scale;
+            if constexpr (FP8) c = attn_factor(c * next_scale);
             const uint64_t c2 = pair_of(c, c);
 #pragma unroll 1
             for (uint32_t u = 0; ok && u < n; ++u) {

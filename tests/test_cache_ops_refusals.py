@@ -3,7 +3,7 @@ import itertools
 
 import pytest
 
-OK, ALIGN = 0, -3
+OK, DIMS, ALIGN = 0, -1, -3
 A = 1 << 20        # an address that no call below gets as far as using
 
 
@@ -48,3 +48,12 @@ def test_scratch_is_that_of_the_kernel_that_runs(atlas):
     """Single tokens of four heads never take the tcgen05 form, whose pieces are thirty times as large."""
     decode, chunk = _scratch(atlas, 8, 1, 4096), _scratch(atlas, 8, 64, 4096)
     assert 0 < decode < 4 << 20 < 16 << 20 < chunk
+
+
+@pytest.mark.parametrize("scale,k_scale,fp8", [(1e30, 1e30, True), (3e38, 1.0, False), (1e20, 3e18, True)])
+def test_scales_whose_product_overflows(atlas, scale, k_scale, fp8):
+    desc = atlas.make_attention_desc(q=A, out=A, k_cache=A, v_cache=A, block_table=A, cu_q=A, kv_len=A, n_seqs=2, n_tokens=2, max_q_len=1, max_kv_len=100, n_pages=10,
+                                     block_size=16, table_stride=7, q_heads=8, kv_heads=2, head_dim=128, softmax_scale=scale, k_scale=k_scale, cache_dtype=int(fp8))
+    with pytest.raises(atlas.AtlasError) as refused:
+        atlas.paged_attention(desc, stream=0)
+    assert refused.value.status == DIMS
