@@ -4,7 +4,8 @@
 //
 // with the running maximum and sum of a softmax held in FP32: of each piece of the keys a kernel has M (largest score, in units of
 // log 2), L = sum 2^(s - M) and O = sum 2^(s - M) v; two pieces join as M = max, L = L1 2^(M1 - M) + L2 2^(M2 - M), O likewise.
-// A row that sees no key has L = 0 and gives zeros, and -inf as its logarithm.
+// A row that sees no key has L = 0 and gives zeros, and -inf as its logarithm.  (Any M does, as long as the weights stay within their type:
+// over E4M3 caches, whose weights are FP16, it is 2^7 below the largest, see ATTN_UP.)
 //
 // The line of tiles of all items (attn_plan.hpp) is cut into one range a CTA.  An item that lies in one range is written at once; the
 // pieces of one that does not go to scratch, two slots a CTA (the item its range begins in, the item its range ends in), and
@@ -66,6 +67,16 @@ struct AttnCut {
     uint32_t pieces;              // of the item, on this range and the next ones and the one before; 0: no item is cut here for the first time
     uint32_t seq, block, head;
 };
+
+// FP16 holds nothing below 2^-24, so beside a largest weight of 1 a weight below 2^-25 would count in the sum and not in the output: over 2^18
+// keys at 2^-25.4 of the largest, 2^-7 of it.  With M lower by ATTN_UP the largest weight is 2^7 and that border 2^-32.  (No more than 7: scores
+// are FP32, whose steps are 16 from 2^27 on.  M rounded to such steps keeps within 2^8 of the largest score's weight, itself off by 2^8 there.)
+constexpr float ATTN_UP = 7.0f;
+// M for a largest product `top` of a row and its factor
+template <bool FP8> __device__ __forceinline__ float attn_base(float top, float c) {
+    if constexpr (FP8) return fmaf(top, c, -ATTN_UP);
+    else return top * c;
+}
 
 // The scores' factor must not come to zero: zero times a masked place's -inf is a NaN.  From here down all scores are equal.
 __device__ __forceinline__ float attn_factor(float c) { return fmaxf(c, 1.1754944e-38f); }

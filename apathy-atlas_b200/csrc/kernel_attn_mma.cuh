@@ -17,7 +17,7 @@
 // An E4M3 cache is multiplied as FP16, which holds every E4M3 value: conversion is one instruction for two values and keeps NaN.  Q is
 // BF16, whose range FP16 has not, so each row is first multiplied by the power of two that brings its largest value to [2^14, 2^15);
 // what then falls below FP16's smallest step is 2^-39 of the row's largest value.  The scores' factor takes the power back.
-// P, in [0, 1], is rounded to BF16 (FP16 with an E4M3 cache) for the product with V; its sum is taken before that, in FP32.
+// P is rounded to BF16 (with an E4M3 cache FP16, of weights up to 2^7: ATTN_UP) for the product with V; its sum is taken before that, in FP32.
 #pragma once
 
 #include "kernel_attn.cuh"
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaCfg<DP, FP8, RT>::CTAS) attn_m
                         for (int n = 0; n < UT; ++n) top = fmaxf(fmaxf(top, s[n][t][e]), s[n][t][2 + e]);
 #pragma unroll
                         for (uint32_t x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-                        top = fmaxf(top * c_row[t][e], m[t][e]);             // (the factor is positive)
+                        top = fmaxf(attn_base<FP8>(top, c_row[t][e]), m[t][e]);   // (the factor is positive)
                         base[e] = top == -INFINITY ? 0.0f : top;
                         keep[t][e] = attn_exp2(m[t][e] - base[e]);
                         turn |= keep[t][e] != 1.0f;

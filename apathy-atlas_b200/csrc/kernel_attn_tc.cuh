@@ -17,7 +17,8 @@
 // 8 Q + 2 KV heads of 128: 118 us; the mma.sync form takes 433, pages of 16 by TMA 70).
 //
 // O is multiplied with 2^(M_old - M_new) only where a row's maximum has grown by more than 2^15 (TC_RESCALE) since O's last factor: until
-// then the weights are 2^(s - M) with the old M, up to 2^15 (which FP16 holds) and in the same FP32 sums, which is the same quotient.  That
+// then the weights are 2^(s - M) with the old M, up to 2^15 and in the same FP32 sums, which is the same quotient.  (E4M3: FP16 holds 2^15, and M
+// begins 2^7 below the largest, see ATTN_UP, so from 2^8 on.)  That
 // takes the correction off the path of nearly every step (8192 tokens, scores' deviations from 1 to 4: 490 us with 2^8, 481 with 2^15).
 // (Exponentials by a polynomial on the FMA pipe for a quarter to a half of the scores, the special-function unit being the busiest of the
 // softmax: no faster.  The next step's scores asked for between the exponentials of this one: they are not there yet, 484 -> 564 us.)
@@ -509,8 +510,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 for (uint32_t k = 0; k < TC_STEP; k += 8)
 #pragma unroll
                     for (int v = 0; v < 4; ++v) top4[v] = fmaxf(fmaxf(top4[v], __uint_as_float(s[k + 2 * v])), __uint_as_float(s[k + 2 * v + 1]));
-                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * c;
-                const bool grow = top > m + TC_RESCALE;
+                const float top = attn_base<FP8>(fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])), c);
+                const bool grow = top > m + (FP8 ? TC_RESCALE - ATTN_UP : TC_RESCALE);   // (weights up to 2^15 either way)
                 if (u == 0) {
                     m = top;
                 } else if (__any_sync(0xFFFFFFFFu, grow)) {

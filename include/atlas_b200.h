@@ -487,7 +487,8 @@ ATLAS_B200_API int32_t atlas_b200_registry_select_victim(const atlas_b200_regist
  *     o[i,h] = sum_j p_j v[j, h / group],   p = softmax over j <= n - c + i of  softmax_scale * q[i,h] . k[j, h / group]
  * with group = q_heads / kv_heads.  A token that sees no key (c > n), or none whose score is above -inf, gives zeros, and -inf in lse.
  * An infinity or a NaN in the values of a token that is seen makes its channel an infinity or a NaN; one that is not seen is not read into any.  Scores, the softmax's maximum and
- * sum and the outputs' sums are FP32; p is rounded to BF16 (FP16 over an E4M3 cache) for its product with v; o is rounded once.
+ * sum and the outputs' sums are FP32; p is rounded to BF16 (FP16 over an E4M3 cache, where what is below 2^-32 of the row's largest counts in the sum alone) for its product
+ * with v; o is rounded once.
  *   q, out       [n_tokens, q_heads * head_dim] BF16, row strides in elements; q may be a column range of a fused QKV buffer;
  *                they must not overlap
  *   lse          [n_tokens, q_heads] f32 or NULL: natural logarithm of the sum of the exponentials
