@@ -117,13 +117,26 @@ ATLAS_HD inline AttnPlace attn_place_in_block(const AttnSeq& s, uint32_t kv_head
     p.place = uint32_t(in_block - uint64_t(p.head) * (s.sh.extra + p.tiles));
     return p;
 }
+// How many of 32 candidates something holds for, looked at one after the other; a warp looks at them at once.
+struct AttnOneByOne {
+    template <typename F> ATLAS_HD uint32_t operator()(F holds) const {
+        uint32_t n = 0;
+        for (uint32_t i = 0; i < 32; ++i) n += holds(i) ? 1u : 0u;
+        return n;
+    }
+};
 // where place x of a sequence's part of the line lies, x < total(kv_heads)
-ATLAS_HD inline AttnPlace attn_locate(const AttnSeq& s, uint32_t kv_heads, uint64_t x) {
+template <typename Count = AttnOneByOne>
+ATLAS_HD inline AttnPlace attn_locate(const AttnSeq& s, uint32_t kv_heads, uint64_t x, Count count = Count()) {
     uint32_t lo = 0, hi = s.blocks - 1;
     while (lo < hi) {                                                                     // the last block that begins at or before x
-        const uint32_t mid = (lo + hi + 1) / 2;
-        if (s.before(mid) * kv_heads <= x) lo = mid;
-        else hi = mid - 1;
+        const uint32_t step = (hi - lo + 31u) / 32u;
+        const uint32_t past = count([&](uint32_t i) {
+            const uint32_t mid = lo + (i + 1u) * step;
+            return mid <= hi && s.before(mid) * kv_heads <= x;
+        });
+        lo += past * step;
+        hi = hi < lo + step - 1u ? hi : lo + step - 1u;
     }
     return attn_place_in_block(s, kv_heads, x, lo);
 }
@@ -155,5 +168,12 @@ struct AttnRanges {
         return x < longer ? uint32_t(attn_quotient(x, each + 1)) : uint32_t(more + attn_quotient(x - longer, each));
     }
 };
+
+// How many pieces the item has that range c, beginning at `begin` and there at place `at`, cuts for the first time; 0 if it cuts none so.  A
+// piece of an item is what a range has of its tiles: a cut among the places ahead of the first tile is none.
+ATLAS_HD inline uint32_t attn_cut_pieces(const AttnRanges& r, uint32_t c, uint64_t begin, const AttnPlace& at, uint32_t extra) {
+    const uint64_t first_tile = begin - at.place + extra;
+    return c > 0 && begin > first_tile && r.begin(c - 1) <= first_tile ? r.of(first_tile + at.tiles - 1) - c + 2u : 0u;
+}
 
 }  // namespace atlas

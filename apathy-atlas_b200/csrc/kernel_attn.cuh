@@ -129,14 +129,7 @@ __device__ __forceinline__ void attn_begin_at(const AttnParams& p, const AttnRan
         at.place = 0;
         at.tiles = plan.tiles(at.block);
     } else {
-        uint32_t lo = 0, hi = plan.blocks - 1;                               // the last block that begins at or before x: 32 looked at at once
-        while (lo < hi) {
-            const uint32_t step = (hi - lo + 31u) / 32u, mid = lo + (lane + 1u) * step;
-            const uint32_t past = __popc(__ballot_sync(0xFFFFFFFFu, mid <= hi && plan.before(mid) * p.kv_heads <= x));
-            lo += past * step;
-            hi = min(hi, lo + step - 1u);
-        }
-        at = attn_place_in_block(plan, p.kv_heads, x, lo);
+        at = attn_locate(plan, p.kv_heads, x, [lane](auto holds) { return uint32_t(__popc(__ballot_sync(0xFFFFFFFFu, holds(lane)))); });
     }
     if (lane != 0) return;
     start->left = end - begin;
@@ -144,10 +137,7 @@ __device__ __forceinline__ void attn_begin_at(const AttnParams& p, const AttnRan
     start->sq = sq;
     start->seq = seq;
     if (p.by_item) return;
-    const uint64_t first_tile = begin - at.place + p.shape.extra;
-    AttnCut cut{0u, seq, at.block, at.head};
-    if (c > 0 && begin > first_tile && ranges.begin(c - 1) <= first_tile) cut.pieces = ranges.of(first_tile + at.tiles - 1) - c + 2u;
-    p.cuts[c] = cut;
+    p.cuts[c] = AttnCut{attn_cut_pieces(ranges, c, begin, at, p.shape.extra), seq, at.block, at.head};
 }
 // By all THREADS threads of a CTA; `sh`: THREADS / 32 words of 64 bits.  Ends with a barrier.
 constexpr uint32_t ATTN_WARP_SEQS = 256;
