@@ -201,11 +201,12 @@ uint32_t tc_box_rows(uint32_t block_size) {
     return r;
 }
 bool rows_pay_for_tc(const atlas_b200_attention_desc& d) {
-    // Rows of a KV head from which on the tensor cores' 256-row blocks pay, although most of such a block is empty.  16 sequences of 4000
-    // tokens, 8 KV heads of 128, this form / mma.sync: BF16, 12 rows 64 / 56 us, 24 rows 64 / 89, 40 rows 66 / 129; E4M3, whose tiles
-    // are converted by four warps, 24 rows 92 / 79.
-    // Over pages that are copied row by row it costs half as much again (pages of 5: BF16 head_dim 128, 20 rows 136 / 93, 48 rows 136 / 131,
-    // 64 rows 136 / 168; head_dim 256, 209 / 266 with 20 rows; E4M3 head_dim 128, 111 / 112 with 48 rows).
+    // Rows of a KV head from which on the tensor cores' 256-row blocks pay, although most of such a block is empty.  Sequences of 4000 tokens, 8 KV
+    // heads of 128, this form / mma.sync.  BF16, 12 rows: 4 sequences 28 / 21 us, 16 54 / 56, 64 188 / 180; 20 rows, two blocks to
+    // mma.sync: 16 sequences 54 / 95 (the latter over pages of 5).  E4M3, whose tiles are converted by four warps, 12 rows: 31 / 23, 70 / 53, 249 / 147; 20 rows: 32 / 36, 71 / 84, 252 / 270;
+    // 32 rows: 34 / 36, 71 / 86, 255 / 273: from 17 rows on this form would be the shorter there too, by a seventh at most.
+    // Over pages that are copied row by row it costs half as much again (pages of 5, 16 sequences: BF16 head_dim 128, 20 rows 138 / 95, 48 rows
+    // 141 / 136; head_dim 256, 20 rows 212 / 266; E4M3 head_dim 128, 20 rows 104 / 86, 48 rows 104 / 112; head_dim 256, 20 rows 190 / 169).
     const bool fp8 = d.cache_dtype == ATLAS_B200_CACHE_E4M3, boxes = tc_box_rows(d.block_size) >= 8;
     const uint64_t from = boxes ? (fp8 ? 32 : 16) : !fp8 && d.head_dim > 128 ? 16 : 48;
     return chunk_rows(d) > from;

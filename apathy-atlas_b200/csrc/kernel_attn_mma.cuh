@@ -39,8 +39,8 @@ template <int DP, bool FP8, int RT> struct MmaCfg {
     static constexpr int UNIT = ROW_BYTES <= 128 ? 32 : 16, TILE = UNIT * MMA_WARPS;
     static constexpr int SIDE = UNIT * ROW_BYTES;                            // K or V of a unit
     // CTAs on an SM, and the ring as deep as that leaves room for.  Short rows and conversions mean more arithmetic for a byte, so three:
-    // what a unit waits for is its own instructions (256 sequences of up to 4096 over E4M3: 278 us with two, 252 with three; with units of
-    // 16 tokens 299, and 290 with four CTAs).
+    // what a unit waits for is its own instructions (256 sequences of up to 4096 over E4M3, before other changes that brought it to 242 us: 278 with
+    // two, 252 with three; with units of 16 tokens 299, and 290 with four CTAs).
     static constexpr int CTAS = attn_mma_ctas(ROW_BYTES, FP8, RT);
     static constexpr int RING_BYTES = CTAS == 1 ? 196608 : CTAS == 2 ? 98304 : 65536;
     static constexpr int STAGES = RING_BYTES / MMA_WARPS / (2 * SIDE) > 8 ? 8 : RING_BYTES / MMA_WARPS / (2 * SIDE);

@@ -503,6 +503,8 @@ ATLAS_B200_API int32_t atlas_b200_registry_select_victim(const atlas_b200_regist
  *   ws           scratch of atlas_b200_paged_attention_ws_bytes(desc) bytes, 32-byte aligned, holding nothing between calls: calls
  *                that may overlap on the GPU need one each.  Less than the call's kernel takes is refused (-2).  NULL: no sequence's cache is split over several SMs, which is slow where
  *                there are few sequences.
+ * Chunks of many tokens run on kernels that move q and out sixteen bytes at a time: q and out 16-byte aligned, both strides multiples of 8.  Others
+ * are computed by the kernels for single tokens, five to ten times as slowly (512 tokens over 4096, 8192 over 8192, 32 + 8 heads of 128).
  * head_dim a multiple of 32 up to 256, any group and block_size; scales positive and finite, and softmax_scale * k_scale * log2(e) finite (-1).  n_pages * block_size and
  * table_stride * block_size below 2^31 (-5).  Caches 16-byte aligned, q 4-byte with an even stride (-3).  A block table entry outside
  * the pool reads as zeros and is recorded in the device status word (4), so is a kv_len beyond the table's row (5; what fits is
